@@ -35,7 +35,8 @@ COMMON += [d for d in os.environ.get("FISH_NVCC_DEFINES", "").split() if d.start
 
 SOURCES = [
     "kernels/quant_act.cu", "kernels/gemv.cu", "kernels/attention.cu", "kernels/misc.cu", "kernels/step.cu", "kernels/gemm.cu", "kernels/gemm_tc.cu",
-    "gguf.cpp", "tokenizer.cpp", "sampler.cpp", "engine.cpp", "c_api.cpp", "kernel_api.cpp",
+    "kernels/kv4.cu", "kernels/attention_packed.cu",
+    "gguf.cpp", "tokenizer.cpp", "sampler.cpp", "engine.cpp", "c_api.cpp", "kernel_api.cpp", "device_api.cpp",
     "attention_static.cu",
 ]
 

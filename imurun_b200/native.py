@@ -17,6 +17,8 @@ from . import libpath
 P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
+L = ctypes.c_int64
+S = ctypes.c_size_t
 CP = ctypes.c_char_p
 
 FISH_TOKEN_CB = ctypes.CFUNCTYPE(None, ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p)
@@ -72,7 +74,8 @@ ABI5_FUNCTIONS = [
 KERNEL_FUNCTIONS = [
     "fbx_quantize_acts", "fbx_rmsnorm", "fbx_matmul", "fbx_block_sums", "fbx_attention", "fbx_rope",
     "fbx_argmax", "fbx_argmax_penalized", "fbx_layer_probe", "fbx_tp_plan", "fbx_moe_localize_host", "fbx_embed", "fbx_time_matmul", "fbx_attention_static", "fbx_attention_decode",
-    "fbx_profiler", "fbx_attention_prefill",
+    "fbx_profiler", "fbx_attention_prefill", "fbx_kv4_layer_bytes", "fbx_kv4_append", "fbx_kv4_attention",
+    "fbx_kv4_attention_workspace", "fbx_attention_packed",
 ]
 
 
@@ -81,6 +84,14 @@ class LayerProbeOut(ctypes.Structure):
     _fields_ = [
         ("f", P * 4), ("qk", P * 4), ("q32", P * 4), ("gate3", P), ("up3", P),
         ("rows", I * 4), ("K", I * 4), ("has_k", I * 4), ("has_32", I * 4), ("silu_in_prologue", I),
+    ]
+
+
+class Kv4Cache(ctypes.Structure):
+    """fbx_kv4_cache (include/fish/fish_kernels.h): one layer of a paged cache held in 4 bits."""
+    _fields_ = [
+        ("pool", P), ("page_table", P), ("err", P), ("page_stride", ctypes.c_int64), ("layer_offset", ctypes.c_int64),
+        ("n_pages", I), ("table_stride", I), ("n_seqs", I), ("n_head_kv", I), ("head_dim", I),
     ]
 
 
@@ -127,6 +138,12 @@ def load_library(path: str | Path | None = None) -> ctypes.CDLL:
         "fbx_profiler": ([I], I),
         "fbx_attention_prefill": ([P, P, P, I, I, I, I, I, I, P], I),
         "fbx_attention_static": ([P, P, P, I, I, I, I, I, I, I, P, P], I),
+        "fbx_kv4_layer_bytes": ([I, I], S),
+        "fbx_kv4_append": ([ctypes.POINTER(Kv4Cache), I, P, P, P, L, L, I, I, P, P, I, I, P, P, I, I, P, L, P, P, L, P],
+                           I),
+        "fbx_kv4_attention_workspace": ([I, I, I, I, I], S),
+        "fbx_kv4_attention": ([ctypes.POINTER(Kv4Cache), I, P, L, I, I, P, P, I, F, F, I, P, L, P, S, P], I),
+        "fbx_attention_packed": ([I, P, L, P, P, L, I, P, I, I, I, I, F, F, I, P, L, P], I),
         "fbx_attention_decode": ([P, P, P, P, P, I, I, I, I, I, I, F, I, P, P, P], I),
     }
     for name, (args, res) in sig.items():

@@ -3,13 +3,14 @@
  * Kernel-level entry points of the B200 engine (libfish.so), for parity tests
  * and for callers that want a single hot-path step without a model.
  *
- * Every function takes HOST buffers, runs the same device code the engine's
- * forward pass runs, and copies the result back. Return 0 on success, a
- * negative value on bad arguments, or a positive CUDA error code.
+ * Unless it says otherwise, a function takes HOST buffers, runs the same device
+ * code the engine's forward pass runs, and copies the result back. Return 0 on
+ * success, a negative value on bad arguments, or a positive CUDA error code.
  *
  * Type ids are ggml's (GGUF specification): 0 F32, 1 F16, 8 Q8_0, 12 Q4_K,
  * 14 Q6_K. Weight rows are passed in GGUF block order.
  */
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -119,6 +120,92 @@ FISH_API int fbx_profiler(int start);
  * them) race and corrupt each other's output. */
 FISH_API int fbx_attention_static(const float* q, const void* k, const void* v, int kv_f16, int n_keys, int H,
                                   int HKV, int D, int pos0, int T, float* out, void* stream);
+
+/* ---- A paged KV cache held in 4 bits, and attention of packed prompts.
+ *
+ * These entry points take DEVICE buffers and queue their work on `stream` (a
+ * cudaStream_t of the current device, NULL = default stream) without waiting
+ * for it; they allocate nothing, so they can be captured into a graph from the
+ * first call on. They return 0, -1 for arguments that cannot be right
+ * (including a buffer that is not memory of the current device, and an address
+ * or row stride that is not a multiple of 16 bytes), or a positive CUDA error.
+ * `type` is an element type: 0 F32, 1 F16, 30 BF16 (ggml's ids). Row strides
+ * (ld..) are in elements. No counterpart in the reference, whose cache is f32
+ * (model/fish/include/fish/model.h:279-280) and whose attention takes one
+ * sequence (model/fish/src/ops.cpp:303-356).
+ *
+ * Format of the cache. The values of one position and kv head are cut into
+ * groups of 32 dimensions; a group stores lo = f16(min), d = f16((max - lo) /
+ * 15) and per value the code rint((x - lo) * (1 / d)) clamped to 0..15 (0
+ * where d = 0), and stands for lo + d * code. min and max are clamped to the
+ * f16 range first, and a NaN counts as nothing in them and takes code 0. A page holds 16
+ * positions; the caller places each layer at an offset inside it, and there a
+ * kv head has one record of fbx_kv4_layer_bytes(1, D) bytes: K codes
+ * [16][D/2], K d [16][GP], K lo [16][GP], then the same three for V, GP =
+ * D/32 rounded up to even. In a row of codes, with NG = D/32, K dimension
+ * 32 g + 8 t + n sits in byte 4 NG t + 4 g + n/2 and V dimension
+ * 32 g + 4 h + n in byte 2 NG h' + 2 g + n/2, where h' = h ^ 4 in rows with
+ * bit 1 of the position set and h in the others; even n in the low nibble. */
+typedef struct {
+    void* pool;                  /* the pages; 16-byte aligned */
+    const int32_t* page_table;   /* [n_seqs][table_stride]: page of position 16 i of sequence s at s * table_stride + i */
+    int32_t* err;                /* nullable, one int, set on the device: 5 a page outside the pool, 6 a token's
+                                    sequence or position outside the tables; nothing out of range is read or written */
+    int64_t page_stride;         /* bytes from page to page, a multiple of 16 */
+    int64_t layer_offset;        /* bytes from a page's start to this layer's records, a multiple of 16 */
+    int32_t n_pages, table_stride, n_seqs;
+    int32_t n_head_kv, head_dim; /* head_dim 64, 96 or 128 */
+} fbx_kv4_cache;
+
+/* Bytes that one layer of a page takes; 0 for shapes that the cache does not hold. */
+FISH_API size_t fbx_kv4_layer_bytes(int n_head_kv, int head_dim);
+
+/* A step's T tokens into the cache: RoPE (the first `rot` dimensions, pairs
+ * (2i, 2i+1) or with neox (i, i + rot/2), from the f32 tables [n_rope][rot/2]
+ * at the token's position; rot 0 turns nothing) of q and k in 32 bits, then the
+ * quantised k and v into the row of each token's position. Token t belongs to
+ * sequence tok_seq[t] and sits at tok_pos[t]; a negative tok_pos marks a
+ * padding row, which is skipped. Tokens may come in any order; no (sequence,
+ * position) may appear twice in a call, and a page that sequences share must
+ * not be written through two of them. q_out (type out_type, may be NULL
+ * together with q) receives the rotated queries, k_out and v_out (out_type,
+ * nullable) the values that the cache now holds for these tokens, so that
+ * attention of a prompt can run on the same keys that later tokens will see.
+ * In-place operation (q_out == q of the same type and stride) is fine. A
+ * token outside the tables sets *err and is skipped, outputs included. */
+FISH_API int fbx_kv4_append(const fbx_kv4_cache* cache, int type, const void* q, const void* k, const void* v,
+                            int64_t ldq, int64_t ldkv, int T, int H, const int32_t* tok_seq, const int32_t* tok_pos,
+                            int rot, int neox, const float* rope_cos, const float* rope_sin, int n_rope, int out_type,
+                            void* q_out, int64_t ldq_out, void* k_out, void* v_out, int64_t ldkv_out, void* stream);
+
+/* Attention of T query tokens over the cache: token t (rotated queries q, H
+ * heads in groups of H / n_head_kv) sees the positions 0..tok_pos[t] of its
+ * sequence, or the last `window` of them (0: all); scores are scale * q.k,
+ * then with softcap > 0 softcap * tanh(score / softcap). out has q's type;
+ * rows of padding tokens (negative tok_pos) stay as they were, and a token
+ * that sees nothing that can be read gets zeros. max_keys, an upper bound on
+ * tok_pos + 1, sizes the split of long contexts (any value gives the right
+ * result). workspace: 16-byte aligned, at least
+ * fbx_kv4_attention_workspace bytes (NULL where that is 0), not shared by calls
+ * that may overlap; needs no clearing. */
+FISH_API size_t fbx_kv4_attention_workspace(int T, int H, int n_head_kv, int head_dim, int max_keys);
+FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void* q, int64_t ldq, int T, int H,
+                               const int32_t* tok_seq, const int32_t* tok_pos, int max_keys, float scale, float softcap,
+                               int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Causal attention of n_seqs whole prompts packed one after another in the
+ * rows of q [n_rows][H*D], k and v [n_rows][HKV*D] (F16 or BF16; D 64, 96 or
+ * 128; H a multiple of HKV): sequence s has the rows cu_seqlens[s] ..
+ * cu_seqlens[s+1] - 1 (device array of n_seqs + 1 non-decreasing values from
+ * 0.. to at most n_rows; empty sequences are fine), and row i sees the rows of
+ * its sequence up to itself, or with window > 0 the last `window` of them. scale
+ * and softcap as above. Nothing in rows that a query does not see reaches its
+ * output, infinities and NaN included. Rows of out outside every sequence
+ * stay as they were. */
+FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
+                                  int n_rows, const int32_t* cu_seqlens, int n_seqs, int H, int HKV, int D, float scale,
+                                  float softcap, int window, void* out, int64_t ldo, void* stream);
 
 /* First index of the maximum per row (reference model.cpp:1939-1946). */
 FISH_API int fbx_argmax(const float* x, int rows, int n, int32_t* out);

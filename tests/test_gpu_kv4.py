@@ -1,0 +1,603 @@
+"""The paged cache held in 4 bits, attention over it, and attention of packed
+prompts (fbx_kv4_append, fbx_kv4_attention, fbx_attention_packed) against
+plain forms, on device buffers of torch."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import kv4_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from imurun_b200 import native
+    return native.load_library(), torch, native
+
+
+def dtype(torch, t):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[t]
+
+
+def dev(torch, x, t=None):
+    y = torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    return y.to(dtype(torch, t)) if t else y
+
+
+def host(x):
+    return x.float().cpu().numpy()
+
+
+class Cache:
+    """A pool with its page tables on the device, and what a record's first byte is."""
+
+    def __init__(self, env, lens, HKV, D, layers=1, layer=0, gap=0, fill=None, seed=0, page_stride=None, spare=2):
+        self.lib, self.torch, native = env
+        self.HKV, self.D, self.layer = HKV, D, layer
+        rng = np.random.default_rng(seed)
+        need = [-(-n // plain.PAGE) for n in lens]
+        self.n_pages = sum(need) + spare
+        order = rng.permutation(self.n_pages).astype(np.int32)
+        self.table = np.full((len(lens), max(need + [1]) + 1), -7, np.int32)   # entries past a sequence's end: no page
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = order[at:at + n]
+            at += n
+        part = HKV * plain.record_bytes(D)
+        assert self.lib.fbx_kv4_layer_bytes(HKV, D) == part
+        self.stride = page_stride or layers * part + gap
+        self.offset = layer * part
+        size = self.n_pages * self.stride
+        if page_stride:
+            self.pool = self.torch.empty(size, dtype=self.torch.uint8, device="cuda")
+        else:
+            self.pool = dev(self.torch, np.full(size, 0 if fill is None else fill, np.uint8))
+        self.dtable = dev(self.torch, self.table)
+        self.err = self.torch.zeros(1, dtype=self.torch.int32, device="cuda")
+        self.handle = native.Kv4Cache(pool=self.pool.data_ptr(), page_table=self.dtable.data_ptr(),
+                                      err=self.err.data_ptr(), page_stride=self.stride, layer_offset=self.offset,
+                                      n_pages=self.n_pages, table_stride=self.table.shape[1], n_seqs=len(lens),
+                                      n_head_kv=HKV, head_dim=D)
+
+    def record(self, seq, pos, head):
+        return int(self.table[seq, pos // plain.PAGE]) * self.stride + self.offset + head * plain.record_bytes(self.D)
+
+    def put(self, pool, seq, pos, k, v):
+        """Rows k, v [HKV][D] of one position into the host image `pool`."""
+        for head in range(self.HKV):
+            for x, is_v in ((k, False), (v, True)):
+                plain.store(pool, self.record(seq, pos, head), pos % plain.PAGE, is_v, self.D, *plain.quantise(x[head][None]))
+
+    def random(self, lens, rng, spread=1.0):
+        """Fills the sequences with random rows, on host and device; padding rows of the last pages hold what 0xFF means: NaN scales."""
+        image = np.full(self.pool.numel(), 0xFF, np.uint8)
+        for s, n in enumerate(lens):
+            for p in range(n):
+                self.put(image, s, p, (rng.standard_normal((self.HKV, self.D)) * spread).astype(np.float32),
+                         (rng.standard_normal((self.HKV, self.D)) * spread + 0.3).astype(np.float32))
+        self.pool.copy_(dev(self.torch, image))
+        return image
+
+    def held(self, image, seq, n, head):
+        """K and V [n][D] in 64 bits of a sequence's first n positions."""
+        k, v = np.zeros((n, self.D)), np.zeros((n, self.D))
+        for i in range(0, n, plain.PAGE):
+            a, b = plain.fetch(image, self.record(seq, i, head), self.D)
+            k[i:i + plain.PAGE], v[i:i + plain.PAGE] = a[:n - i], b[:n - i]
+        return k, v
+
+
+def tables(n, rot, base=10000.0):
+    f = base ** (-np.arange(0, max(rot, 2), 2) / max(rot, 2))
+    a = np.arange(n)[:, None] * f[None, :]
+    return np.cos(a).astype(np.float32), np.sin(a).astype(np.float32)
+
+
+def call_append(env, c, t, qkv, H, seq, pos, rot, neox, cos, sin, out, told=True, stream=0):
+    """fbx_kv4_append on rows q | k | v; returns rc and the outputs (pre-filled with 7)."""
+    lib, torch, _ = env
+    D, HKV, T = c.D, c.HKV, len(seq)
+    q_out, k_out, v_out = (torch.full((T, w * D), 7.0, dtype=dtype(torch, out), device="cuda") for w in (H, HKV, HKV))
+    dseq, dpos = dev(torch, np.asarray(seq, np.int32)), dev(torch, np.asarray(pos, np.int32))
+    x, es, ld = qkv.data_ptr(), qkv.element_size(), qkv.stride(0)
+    rc = lib.fbx_kv4_append(c.handle, plain.TYPE[t], x, x + H * D * es, x + (H + HKV) * D * es, ld, ld, T, H,
+                            dseq.data_ptr(), dpos.data_ptr(), rot, int(neox), cos.data_ptr(), sin.data_ptr(),
+                            cos.shape[0], plain.TYPE[out], q_out.data_ptr(), H * D, k_out.data_ptr() if told else None,
+                            v_out.data_ptr() if told else None, HKV * D, stream)
+    torch.cuda.synchronize()
+    return rc, q_out, k_out, v_out
+
+
+APPENDS = [  # type, out, T, lens, H, HKV, D, rot, neox, layers, layer
+    ("f32", "f32", 1, [7], 8, 2, 128, 128, False, 1, 0),
+    ("f32", "f16", 37, [30, 21], 6, 2, 96, 96, True, 2, 1),
+    ("f16", "f16", 50, [20, 17, 40], 5, 5, 64, 64, True, 3, 1),
+    ("bf16", "bf16", 33, [50], 14, 2, 128, 64, False, 1, 0),
+    ("bf16", "f32", 20, [33, 1], 3, 1, 128, 128, True, 2, 0),
+    ("f16", "bf16", 16, [16], 12, 4, 96, 20, False, 1, 0),
+    ("f32", "bf16", 9, [9], 2, 2, 64, 22, True, 1, 0),
+    ("f16", "f32", 170, [170], 4, 1, 96, 0, False, 1, 0),
+    ("bf16", "f16", 5, [90], 8, 8, 64, 2, True, 1, 0),
+]
+
+
+@pytest.mark.parametrize("t,out,T,lens,H,HKV,D,rot,neox,layers,layer", APPENDS)
+def test_append_matches_the_format_bit_for_bit(env, t, out, T, lens, H, HKV, D, rot, neox, layers, layer):
+    """Cache bytes equal to the plain form's, everything around them untouched;
+    stored values and rotated queries rounded once to the output type."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(T + D + H)
+    c = Cache(env, lens, HKV, D, layers, layer, gap=48, fill=0xAB, seed=D)
+    where = [(s, p) for s, n in enumerate(lens) for p in range(n)]
+    where = [where[i] for i in rng.permutation(len(where))[:T]]   # any order, holes left
+    T = len(where)
+    seq, pos = [s for s, _ in where], [p for _, p in where]
+    # rows in the middle of wider ones, 16 values in front
+    wide = dev(torch, plain.round_to(rng.standard_normal((T, (H + 2 * HKV) * D + 32)).astype(np.float32) * 2, t), t)
+    qkv = wide[:, 16:16 + (H + 2 * HKV) * D]
+    cos, sin = tables(max(lens) + 3, rot)
+    rc, q_out, k_out, v_out = call_append(env, c, t, qkv, H, seq, pos, rot, neox, dev(torch, cos), dev(torch, sin), out)
+    assert rc == 0 and int(c.err) == 0
+    x = host(qkv).reshape(T, H + 2 * HKV, D)
+    image = np.full(c.pool.numel(), 0xAB, np.uint8)
+    for i, (s, p) in enumerate(where):
+        turned = plain.rope(x[i, :H + HKV], cos[p], sin[p], rot, neox)
+        c.put(image, s, p, turned[H:], x[i, H + HKV:])
+        assert np.array_equal(host(q_out[i]), plain.round_to(turned[:H].reshape(-1), out))
+        for got, want in ((k_out, turned[H:]), (v_out, x[i, H + HKV:])):
+            assert np.array_equal(host(got[i]), plain.round_to(plain.values(*plain.quantise(want)).reshape(-1), out))
+    assert np.array_equal(c.pool.cpu().numpy(), image)
+
+
+def test_append_stores_what_the_format_says_for_odd_values(env):
+    """Constants, zeros, one-sided groups, tiny and huge values, infinities and NaN."""
+    lib, torch, _ = env
+    D, rows = 64, []
+    rng = np.random.default_rng(3)
+    for base in (np.zeros(32), np.full(32, 0.1), np.full(32, -3.3), np.arange(32) / 7, np.arange(32) * 1e-7,
+                 rng.standard_normal(32) * 1e-9, rng.standard_normal(32) * 3e4, rng.standard_normal(32) * 1e30,
+                 np.where(np.arange(32) == 5, np.inf, 1.0), np.where(np.arange(32) == 6, -np.inf, np.arange(32)),
+                 np.where(np.arange(32) % 3 == 0, np.nan, np.arange(32) * 0.5), np.full(32, np.nan),
+                 np.where(np.arange(32) == 0, 100.0, 1e-3), 1000 + np.arange(32) * 1e-3, np.full(32, 65519.0),
+                 np.where(np.arange(32) < 16, np.inf, -np.inf)):
+        rows.append(base)
+    x = np.concatenate([np.stack(rows), np.stack(rows[::-1])], 1).astype(np.float32)   # two groups a row
+    T = len(x)
+    c = Cache(env, [T], 1, D, fill=0)
+    qkv = dev(torch, np.concatenate([np.zeros((T, D), np.float32), x, x], 1))
+    cos, sin = tables(T, 2)
+    rc, _, k_out, v_out = call_append(env, c, "f32", qkv, 1, [0] * T, list(range(T)), 0, False, dev(torch, cos),
+                                      dev(torch, sin), "f32")
+    assert rc == 0
+    image = np.zeros(c.pool.numel(), np.uint8)
+    for p in range(T):
+        c.put(image, 0, p, x[p][None], x[p][None])
+    assert np.array_equal(c.pool.cpu().numpy(), image)
+    want = plain.values(*plain.quantise(x))
+    assert np.array_equal(host(k_out), want) and np.array_equal(host(v_out), want) and np.isfinite(want).all()
+
+
+def test_append_skips_padding_and_flags_what_is_outside(env):
+    lib, torch, _ = env
+    H, HKV, D = 4, 2, 128
+    c = Cache(env, [20, 20], HKV, D, fill=0x5A)
+    cos, sin = tables(64, D)
+    qkv = torch.randn((6, (H + 2 * HKV) * D), device="cuda")
+    before = c.pool.clone()
+
+    def call(seq, pos):
+        c.err.zero_()
+        c.pool.copy_(before)
+        rc, q, k, v = call_append(env, c, "f32", qkv[:len(seq)], H, seq, pos, D, False, dev(torch, cos), dev(torch, sin), "f32")
+        assert rc == 0
+        kept = [bool((x[i] == 7).all()) for i in range(len(seq)) for x in (q, k, v)]
+        return int(c.err), bool(torch.equal(c.pool, before)), kept
+
+    # padding: nothing written, nothing flagged
+    assert call([0, 5, -1], [-1, -1, -9]) == (0, True, [True] * 9)
+    # a sequence outside the tables, a position past the rotation's or the page table
+    assert call([2, -1, 0], [0, 0, 64]) == (6, True, [True] * 9)
+    assert call([0], [63]) == (6, True, [True] * 3)
+    # a table entry that names no page
+    assert call([0, 1], [47, 40]) == (5, True, [True] * 6)
+    # good tokens beside bad ones are stored
+    flag, same, kept = call([0, 9, 1], [3, 0, 19])
+    assert flag == 6 and not same and kept == [False] * 3 + [True] * 3 + [False] * 3
+
+
+def test_append_in_place_and_without_outputs(env):
+    """Rotating q in its own rows, K and V replaced by what the cache holds; no
+    outputs at all: the same cache."""
+    lib, torch, _ = env
+    for D, rot in ((128, 128), (96, 96), (64, 32)):
+        H, HKV, T = 7, 2, 21
+        cos, sin = (dev(torch, x) for x in tables(T, rot))
+        seq, pos = dev(torch, np.zeros(T, np.int32)), dev(torch, np.arange(T, dtype=np.int32))
+        qkv = torch.randn((T, (H + 2 * HKV) * D), device="cuda").to(torch.bfloat16)
+        a, b, e = (Cache(env, [T], HKV, D, seed=1) for _ in range(3))
+        rc, q_out, k_out, v_out = call_append(env, a, "bf16", qkv, H, [0] * T, list(range(T)), rot, True, cos, sin, "bf16")
+        assert rc == 0
+        x, ld = qkv.clone(), qkv.shape[1]
+        p = [x.data_ptr() + 2 * D * o for o in (0, H, H + HKV)]
+        assert lib.fbx_kv4_append(b.handle, 30, *p, ld, ld, T, H, seq.data_ptr(), pos.data_ptr(), rot, 1, cos.data_ptr(),
+                                  sin.data_ptr(), T, 30, p[0], ld, p[1], p[2], ld, None) == 0
+        y = qkv.clone()
+        p = [y.data_ptr() + 2 * D * o for o in (0, H, H + HKV)]
+        assert lib.fbx_kv4_append(e.handle, 30, None, p[1], p[2], 0, ld, T, 0, seq.data_ptr(), pos.data_ptr(), rot, 1,
+                                  cos.data_ptr(), sin.data_ptr(), T, 30, None, 0, None, None, 0, None) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(x, torch.cat((q_out, k_out, v_out), 1)) and torch.equal(y, qkv)
+        assert torch.equal(a.pool, b.pool) and torch.equal(a.pool, e.pool)
+
+
+def attention(env, c, t, q, H, seq, pos, max_keys, scale, softcap=0.0, window=0, stream=None, fill=7.0):
+    lib, torch, _ = env
+    T = len(seq)
+    out = torch.full((T, H * c.D), fill, dtype=dtype(torch, t), device="cuda")
+    dseq, dpos = dev(torch, np.asarray(seq, np.int32)), dev(torch, np.asarray(pos, np.int32))
+    size = lib.fbx_kv4_attention_workspace(T, H, c.HKV, c.D, max_keys)
+    ws = torch.full((max(size, 16),), 0xFF, dtype=torch.uint8, device="cuda")
+    rc = lib.fbx_kv4_attention(c.handle, plain.TYPE[t], q.data_ptr(), q.stride(0), T, H, dseq.data_ptr(), dpos.data_ptr(),
+                               max_keys, scale, softcap, window, out.data_ptr(), H * c.D, ws.data_ptr(), size, stream)
+    torch.cuda.synchronize()
+    assert rc == 0
+    return out
+
+
+# a weight times its group's scale is rounded to f16 for 16-bit types, to two f16 parts for f32
+def weight_rounding(t):
+    return 2.0 ** -22 if t == "f32" else 2.0 ** -11
+
+
+ATTENTIONS = [  # type, H, HKV, D, positions, softcap, window
+    ("f32", 8, 2, 128, [0, 1, 14, 15, 16, 17, 31, 32, 100], 0.0, 0),
+    ("f16", 8, 8, 64, [0, 63, 64, 200, 257], 0.0, 0),
+    ("bf16", 14, 2, 128, [300, 5, 0], 0.0, 0),
+    ("f32", 12, 4, 96, [77, 33, 15], 0.0, 0),
+    ("bf16", 9, 1, 96, [129, 0, 48], 30.0, 0),
+    ("f32", 24, 2, 64, [260, 19], 5.0, 50),
+    ("f16", 16, 2, 128, [500, 40, 16, 15], 0.0, 17),
+    ("f32", 5, 1, 128, [400, 3], 0.0, 1),
+    ("bf16", 4, 4, 64, [90, 31], 0.0, 1000),
+]
+
+
+@pytest.mark.parametrize("t,H,HKV,D,pos,softcap,window", ATTENTIONS)
+def test_attention_over_the_cache(env, t, H, HKV, D, pos, softcap, window):
+    """Against 64 bits; stale rows of the last page hold NaN scales, page-table entries past the end no page."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(H + D + len(pos))
+    lens = [p + 1 for p in pos]
+    c = Cache(env, lens, HKV, D, layers=2, layer=1, gap=16, seed=2)
+    image = c.random(lens, rng)
+    T, G = len(pos), H // HKV
+    order = rng.permutation(T)
+    seq, at = [int(i) for i in order], [pos[i] for i in order]
+    q = dev(torch, plain.round_to(rng.standard_normal((T, H * D + 8)).astype(np.float32) * 1.5, t), t)[:, 8:] \
+        if t != "f32" else dev(torch, rng.standard_normal((T, H * D + 8)).astype(np.float32) * 1.5)[:, 8:]
+    scale = 1.0 / np.sqrt(D)
+    for most in (max(lens), 1, 100000):   # any bound gives the right result
+        out = host(attention(env, c, t, q, H, seq, at, most, scale, softcap, window))
+        assert int(c.err) == 0
+        x = host(q).reshape(T, H, D)
+        for i in range(T):
+            for hk in range(HKV):
+                k, v = c.held(image, seq[i], at[i] + 1, hk)
+                want, mean, ext = plain.attend(x[i, hk * G:(hk + 1) * G], k, v, [at[i]] * G, scale, softcap, window)
+                got = out[i].reshape(H, D)[hk * G:(hk + 1) * G]
+                assert (np.abs(got - want) <= plain.allowed(want, mean, ext, t, weight_rounding(t), softcap)).all()
+
+
+@pytest.mark.parametrize("t,spread,size", [("f32", 1e-4, 1e4), ("f16", 1e-4, 1e3), ("bf16", 1e-6, 1e6), ("f32", 300.0, 1e-3),
+                                            ("bf16", 3000.0, 1e-5), ("f32", 1.0, 0.0)])
+def test_attention_of_tiny_and_huge_values(env, t, spread, size):
+    """Cache values and queries far from 1: no part of the sum may leave the range of 16 bits."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(9)
+    H, HKV, D, pos = 4, 1, 128, [250]
+    c = Cache(env, [251], HKV, D)
+    image = c.random([251], rng, spread)
+    q = dev(torch, plain.round_to((rng.standard_normal((1, H * D)) * size).astype(np.float32), t), t)
+    out = host(attention(env, c, t, q, H, [0], pos, 251, 1.0 / np.sqrt(D))).reshape(H, D)
+    k, v = c.held(image, 0, 251, 0)
+    want, mean, ext = plain.attend(host(q).reshape(H, D), k, v, pos * H, 1.0 / np.sqrt(D))
+    # f16 outputs below its normal range: half of its smallest step, 2^-25, in allowed()
+    assert (np.abs(out - want) <= plain.allowed(want, mean, ext, t, weight_rounding(t))).all()
+
+
+def test_attention_padding_and_bad_pages(env):
+    lib, torch, _ = env
+    H, HKV, D = 8, 2, 128
+    rng = np.random.default_rng(4)
+    c = Cache(env, [40, 40], HKV, D)
+    image = c.random([40, 40], rng)
+    q = torch.randn((3, H * D), device="cuda")
+    # padding rows stay, whatever their sequence
+    out = attention(env, c, "f32", q, H, [0, -3, 1], [-1, -1, 39], 40, 0.1)
+    assert int(c.err) == 0 and bool((out[:2] == 7).all()) and bool((out[2] != 7).any())
+    # an unknown sequence: flagged, nothing seen, zeros
+    out = attention(env, c, "f32", q, H, [2, 1, 0], [5, 39, 39], 40, 0.1)
+    assert int(c.err) == 6 and bool((out[0] == 0).all()) and bool(torch.isfinite(out).all())
+    c.err.zero_()
+    # a page that is not in the pool, in the middle: its keys are not seen
+    c.dtable[0, 1] = c.n_pages
+    out = host(attention(env, c, "f32", q[:1], H, [0], [39], 40, 0.1)).reshape(H, D)
+    assert int(c.err) == 5
+    keep = np.r_[0:16, 32:40]
+    for hk in range(HKV):
+        k, v = c.held(image, 0, 40, hk)
+        want, mean, ext = plain.attend(host(q)[0].reshape(H, D)[hk * 4:hk * 4 + 4], k[keep], v[keep], [23] * 4, 0.1)
+        assert (np.abs(out[hk * 4:hk * 4 + 4] - want) <= plain.allowed(want, mean, ext, "f32", 2.0 ** -22)).all()
+    # a position past the page table: its keys are not seen either
+    c.err.zero_()
+    out = attention(env, c, "f32", q[:1], H, [1], [1000], 1001, 0.1)
+    assert int(c.err) in (5, 6) and bool(torch.isfinite(out).all())
+
+
+def test_cache_past_four_gigabytes(env):
+    """Pages 1.5 GiB apart: byte offsets past 32 bits in the append and in the attention."""
+    lib, torch, _ = env
+    H, HKV, D, n = 4, 2, 128, 60
+    c = Cache(env, [n], HKV, D, page_stride=3 << 29, spare=0)
+    rng = np.random.default_rng(5)
+    x = torch.from_numpy(rng.standard_normal((n, (H + 2 * HKV) * D)).astype(np.float32)).cuda()
+    cos, sin = (dev(torch, a) for a in tables(n, D))
+    rc, q, k, v = call_append(env, c, "f32", x, H, [0] * n, list(range(n)), D, True, cos, sin, "f32")
+    assert rc == 0 and int(c.err) == 0
+    out = host(attention(env, c, "f32", q[-1:], H, [0], [n - 1], n, 0.08)).reshape(H, D)
+    kk, vv = (host(y).reshape(n, HKV, D) for y in (k, v))
+    for hk in range(HKV):
+        want, mean, ext = plain.attend(host(q)[-1].reshape(H, D)[hk * 2:hk * 2 + 2], kk[:, hk], vv[:, hk], [n - 1] * 2, 0.08)
+        assert (np.abs(out[hk * 2:hk * 2 + 2] - want) <= plain.allowed(want, mean, ext, "f32", 2.0 ** -22)).all()
+
+
+# ------------------------------------------------------------------ packed prompts
+
+def packed(env, t, q, k, v, cu, H, HKV, D, scale, softcap=0.0, window=0, out=None, stream=None, rows=None):
+    lib, torch, _ = env
+    if out is None:
+        out = torch.full((q.shape[0], H * D), 7.0, dtype=q.dtype, device="cuda")
+    rc = lib.fbx_attention_packed(plain.TYPE[t], q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(0),
+                                  q.shape[0] if rows is None else rows, cu.data_ptr(), cu.numel() - 1, H, HKV, D, scale,
+                                  softcap, window, out.data_ptr(), out.stride(0), stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    return out
+
+
+PACKED = [  # type, lens, H, HKV, D, softcap, window
+    ("bf16", [1], 4, 2, 128, 0.0, 0),
+    ("f16", [0, 1, 0, 2, 17, 0], 3, 1, 64, 0.0, 0),
+    ("bf16", [127, 128, 129], 2, 2, 128, 0.0, 0),
+    ("f16", [255, 256, 257], 4, 1, 128, 0.0, 0),
+    ("f16", [300, 40, 131], 6, 2, 96, 0.0, 0),
+    ("bf16", [64, 65, 63, 1, 513], 2, 1, 64, 0.0, 0),
+    ("bf16", [385, 5], 8, 1, 128, 20.0, 0),
+    ("f16", [400, 33], 4, 4, 64, 0.0, 1),
+    ("f16", [390, 200], 2, 1, 128, 0.0, 100),
+    ("bf16", [520, 128], 4, 2, 96, 8.0, 128),
+    ("bf16", [600], 2, 2, 64, 0.0, 257),
+]
+
+
+def packed_reference(q, k, v, lens, H, HKV, D, scale, softcap, window):
+    G, at = H // HKV, 0
+    want, bound = np.zeros(q.shape), np.zeros(q.shape)
+    mean, ext = np.zeros(q.shape), np.zeros((len(q), H))
+    for n in lens:
+        for h in range(H):
+            a, b = slice(h * D, h * D + D), slice(h // G * D, h // G * D + D)
+            want[at:at + n, a], mean[at:at + n, a], ext[at:at + n, h] = plain.attend(
+                q[at:at + n, a], k[at:at + n, b], v[at:at + n, b], range(n), scale, softcap, window)
+        at += n
+    return want, mean, ext
+
+
+def check_packed(got, want, mean, ext, H, D, t, softcap, rows):
+    for h in range(H):
+        a = slice(h * D, h * D + D)
+        # a weight is rounded to the type before its product with v
+        tol = plain.allowed(want[:rows, a], mean[:rows, a], ext[:rows, h], t, plain.HALF[t], softcap)
+        assert (np.abs(got[:rows, a] - want[:rows, a]) <= tol).all(), (h, np.abs(got[:rows, a] - want[:rows, a]).max())
+
+
+@pytest.mark.parametrize("t,lens,H,HKV,D,softcap,window", PACKED)
+def test_packed_prompts(env, t, lens, H, HKV, D, softcap, window):
+    """Rows inside wider ones; rows after the last sequence hold NaN and keep what out had."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(sum(lens) + D + H)
+    N, extra = sum(lens), 5
+    cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    wide = rng.standard_normal((N + extra, (H + 2 * HKV) * D + 8)).astype(np.float32)
+    wide[N:] = np.nan
+    wide = dev(torch, wide, t)
+    q, k, v = wide[:, 8:8 + H * D], wide[:, 8 + H * D:8 + (H + HKV) * D], wide[:, 8 + (H + HKV) * D:]
+    scale = 1.7 / np.sqrt(D)
+    out = packed(env, t, q, k, v, dev(torch, cu), H, HKV, D, scale, softcap, window)
+    assert bool((out[N:] == 7).all())
+    ref = packed_reference(host(q)[:N], host(k)[:N], host(v)[:N], lens, H, HKV, D, scale, softcap, window)
+    check_packed(host(out), *ref, H, D, t, softcap, N)
+
+
+@pytest.mark.parametrize("t,D", [("f16", 64), ("bf16", 128), ("f16", 96)])
+def test_packed_masked_infinities_and_nan(env, t, D):
+    """A row's output does not depend on what later rows, or other sequences,
+    hold, even where that is not finite; rows that see it follow the formula."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(D)
+    lens, H, HKV = [150, 90, 300], 4, 2
+    N = sum(lens)
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    q, k, v = (dev(torch, rng.standard_normal((N, h * D)).astype(np.float32), t) for h in (H, HKV, HKV))
+    scale = 1.0 / np.sqrt(D)
+    clean = packed(env, t, q, k, v, cu, H, HKV, D, scale)
+    for row, what in ((149, np.nan), (100, np.inf), (239, -np.inf), (240 + 17, np.nan), (240 + 200, np.inf)):
+        seq_end = next(e for e in np.cumsum(lens) if row < e)
+        vv, kk = v.clone(), k.clone()
+        vv[row, D + 3] = what          # kv head 1, dimension 3
+        out = packed(env, t, q, k, vv, cu, H, HKV, D, scale)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        for h in (2, 3):
+            hit[row:seq_end, h * D + 3] = True
+        assert torch.equal(out[~hit], clean[~hit]), (row, what)
+        want = torch.full_like(out, what)
+        assert torch.equal(torch.isnan(out[hit]), torch.isnan(want[hit])) and torch.equal(
+            out[hit][~torch.isnan(want[hit])], want[hit][~torch.isnan(want[hit])])
+        kk[row, 5] = np.nan            # a key of head 0: every row from it on loses heads 0 and 1
+        out = packed(env, t, q, kk, v, cu, H, HKV, D, scale)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[row:seq_end, :2 * D] = True
+        assert torch.equal(out[~hit], clean[~hit]) and bool(torch.isnan(out[hit]).all())
+    # under a window, rows behind it stop seeing the row
+    vv = v.clone()
+    vv[160, 7] = np.inf
+    a = packed(env, t, q, k, v, cu, H, HKV, D, scale, window=20)
+    b = packed(env, t, q, k, vv, cu, H, HKV, D, scale, window=20)
+    hit = torch.zeros_like(a, dtype=torch.bool)
+    for h in (0, 1):
+        hit[160:180, h * D + 7] = True
+    assert torch.equal(a[~hit], b[~hit]) and bool(torch.isinf(b[hit]).all())
+
+
+def test_packed_large_scores_and_bad_lengths(env):
+    lib, torch, _ = env
+    H, HKV, D, N = 2, 1, 128, 300
+    q = torch.randn((N, H * D), device="cuda").bfloat16() * 60
+    k, v = (torch.randn((N, HKV * D), device="cuda").bfloat16() for _ in range(2))
+    cu = dev(torch, np.array([0, N], np.int32))
+    out = host(packed(env, "bf16", q, k, v, cu, H, HKV, D, 1.0))       # scores of several hundred
+    ref = packed_reference(host(q), host(k), host(v), [N], H, HKV, D, 1.0, 0.0, 0)
+    check_packed(out, *ref, H, D, "bf16", 0.0, N)
+    # ends past the rows and ends before starts: read and written inside the buffers only
+    cu = dev(torch, np.array([0, 100, 90, 5000, 20], np.int32))
+    out = packed(env, "bf16", q, k, v, cu, H, HKV, D, 0.1)
+    assert bool(torch.isfinite(out).all())
+
+
+# ---------------------------------------------------- as they are used, together
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_prompts_then_tokens(env, t):
+    """Prompts of a batch are appended and attended, then tokens one by one:
+    every output against 64 bits over the values that the cache holds."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(11)
+    H, HKV, D, rot, lens, steps = 8, 2, 128, 128, [45, 3, 130], 20
+    G, scale, B = H // HKV, 1.0 / np.sqrt(D), len(lens)
+    c = Cache(env, [n + steps for n in lens], HKV, D)
+    cos, sin = (dev(torch, x) for x in tables(200, rot))
+    seq = [s for s, n in enumerate(lens) for _ in range(n)]
+    pos = [p for n in lens for p in range(n)]
+    qkv = dev(torch, rng.standard_normal((len(seq), (H + 2 * HKV) * D)).astype(np.float32), t)
+    rc, q, k, v = call_append(env, c, t, qkv, H, seq, pos, rot, True, cos, sin, t)
+    assert rc == 0
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    out = host(packed(env, t, q, k, v, cu, H, HKV, D, scale))
+    check_packed(out, *packed_reference(host(q), host(k), host(v), lens, H, HKV, D, scale, 0.0, 0), H, D, t, 0.0, len(seq))
+    for step in range(steps):
+        at = [n + step for n in lens]
+        qkv = dev(torch, rng.standard_normal((B, (H + 2 * HKV) * D)).astype(np.float32), t)
+        rc, q, _, _ = call_append(env, c, t, qkv, H, list(range(B)), at, rot, True, cos, sin, t)
+        assert rc == 0
+        if step % 5 and step != steps - 1:
+            continue
+        got = host(attention(env, c, t, q, H, list(range(B)), at, max(at) + 1, scale)).reshape(B, H, D)
+        image = c.pool.cpu().numpy()
+        for s in range(B):
+            for hk in range(HKV):
+                kk, vv = c.held(image, s, at[s] + 1, hk)
+                hs = slice(hk * G, hk * G + G)
+                want, mean, ext = plain.attend(host(q)[s].reshape(H, D)[hs], kk, vv, [at[s]] * G, scale)
+                assert (np.abs(got[s, hs] - want) <= plain.allowed(want, mean, ext, t, weight_rounding(t))).all()
+    assert int(c.err) == 0
+
+
+def test_captured_and_replayed_on_a_side_stream(env):
+    """append -> attention, and packed attention, captured once on a side
+    stream and replayed on new inputs in the same buffers; two graphs with
+    workspaces of their own, replayed at the same time, give what eager calls give."""
+    lib, torch, _ = env
+    H, HKV, D, T, n = 8, 2, 128, 3, 400
+    rng = np.random.default_rng(12)
+    cos, sin = (dev(torch, x) for x in tables(n + 8, D))
+    graphs = []
+    for g in range(2):
+        c = Cache(env, [n + 8] * T, HKV, D, seed=g)
+        c.random([n] * T, rng)
+        b = {"c": c, "qkv": torch.randn((T, (H + 2 * HKV) * D), device="cuda").half(),
+             "seq": torch.arange(T, dtype=torch.int32, device="cuda"),
+             "pos": torch.full((T,), n, dtype=torch.int32, device="cuda"),
+             "q": torch.zeros((T, H * D), dtype=torch.float16, device="cuda"),
+             "out": torch.zeros((T, H * D), dtype=torch.float16, device="cuda"),
+             "cu": dev(torch, np.array([0, 1, T], np.int32)),
+             "ws": torch.zeros(max(16, lib.fbx_kv4_attention_workspace(T, H, HKV, D, n + 8)), dtype=torch.uint8, device="cuda")}
+        b["pk"] = torch.zeros_like(b["out"])
+
+        def calls(b=b, c=c, st=None):
+            x = b["qkv"].data_ptr()
+            ld = b["qkv"].shape[1]
+            p = (x, x + 2 * H * D, x + 2 * (H + HKV) * D)
+            assert lib.fbx_kv4_append(c.handle, 1, *p, ld, ld, T, H, b["seq"].data_ptr(), b["pos"].data_ptr(), D, 0,
+                                      cos.data_ptr(), sin.data_ptr(), n + 8, 1, b["q"].data_ptr(), H * D, None, None, 0, st) == 0
+            assert lib.fbx_kv4_attention(c.handle, 1, b["q"].data_ptr(), H * D, T, H, b["seq"].data_ptr(),
+                                         b["pos"].data_ptr(), n + 8, 0.09, 0.0, 0, b["out"].data_ptr(), H * D,
+                                         b["ws"].data_ptr(), b["ws"].numel(), st) == 0
+            assert lib.fbx_attention_packed(1, *(p[0], ld, p[1], p[2], ld), T, b["cu"].data_ptr(), 2, H, HKV, D, 0.09,
+                                            0.0, 0, b["pk"].data_ptr(), H * D, st) == 0
+
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            calls(st=torch.cuda.current_stream().cuda_stream)   # the very first call of these shapes may be captured
+        graphs.append((graph, stream, b, calls))
+    torch.cuda.synchronize()
+    for step in range(4):
+        for graph, stream, b, _ in graphs:
+            b["qkv"].copy_(torch.randn(b["qkv"].shape, device="cuda"))
+            b["pos"].fill_(n + step)
+            b["out"].fill_(7)
+        torch.cuda.synchronize()
+        for graph, stream, b, _ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, stream, b, calls in graphs:
+            got, pk, pool = b["out"].clone(), b["pk"].clone(), b["c"].pool.clone()
+            b["out"].fill_(3)
+            b["pk"].fill_(3)
+            calls()
+            torch.cuda.synchronize()
+            assert torch.equal(got, b["out"]) and torch.equal(pk, b["pk"]) and torch.equal(pool, b["c"].pool)
+            assert int(b["c"].err) == 0
+
+
+def test_calls_allocate_nothing_and_refuse_foreign_memory(env):
+    lib, torch, _ = env
+    H, HKV, D, n = 8, 2, 128, 64
+    c = Cache(env, [n], HKV, D)
+    q = torch.randn((1, H * D), device="cuda")
+    host_q = np.zeros((1, H * D + 8), np.float32)
+    addr = (host_q.ctypes.data + 15) // 16 * 16
+    seq = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.zeros_like(q)
+    ws = torch.zeros(max(16, lib.fbx_kv4_attention_workspace(1, H, HKV, D, n)), dtype=torch.uint8, device="cuda")
+
+    def call(qp):
+        return lib.fbx_kv4_attention(c.handle, 0, qp, H * D, 1, H, seq.data_ptr(), seq.data_ptr(), n, 0.1, 0.0, 0,
+                                     out.data_ptr(), H * D, ws.data_ptr(), ws.numel(), None)
+
+    assert call(q.data_ptr()) == 0
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(20):
+        assert call(q.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] == free
+    assert call(addr) == -1   # a host array
+    torch.cuda.synchronize()
