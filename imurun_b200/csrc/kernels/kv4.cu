@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
             if (!(lo <= hi)) lo = hi = 0.0f;   // nothing but NaN
             const __half lo16 = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
             lo = __half2float(lo16);
-            const __half d16 = __float2half_rn(__fdiv_rn(__fsub_rn(fminf(fmaxf(hi, -65504.0f), 65504.0f), lo), 15.0f));
+            const __half d16 = __float2half_rn(__fmul_rn(__fsub_rn(fminf(fmaxf(hi, -65504.0f), 65504.0f), lo), 1.0f / 15.0f));
             const float d = __half2float(d16), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
             uint32_t word = 0;
 #pragma unroll

@@ -8,6 +8,7 @@ the check that IMURUN's own binding will load the library unchanged.
 from __future__ import annotations
 
 import ctypes
+import functools
 from pathlib import Path
 
 import numpy as np
@@ -99,8 +100,9 @@ def _p(a):
     return None if a is None else a.ctypes.data
 
 
-def load_library(path: str | Path | None = None) -> ctypes.CDLL:
-    lib = ctypes.CDLL(str(path or libpath("libfish.so")))
+@functools.lru_cache(maxsize=None)
+def _library(path: str) -> ctypes.CDLL:
+    lib = ctypes.CDLL(path)
     sig = {
         "fish_version": ([], CP), "fish_abi_version": ([], I), "fish_supported_archs": ([], CP),
         "fish_create": ([], P), "fish_destroy": ([P], None), "fish_load": ([P, CP, I], I),
@@ -151,6 +153,11 @@ def load_library(path: str | Path | None = None) -> ctypes.CDLL:
         fn.argtypes = args
         fn.restype = res
     return lib
+
+
+def load_library(path: str | Path | None = None) -> ctypes.CDLL:
+    """The library with its signatures declared; a path is bound once, later calls get the same object."""
+    return _library(str(path or libpath("libfish.so")))
 
 
 class FishError(RuntimeError):

@@ -50,7 +50,7 @@ def quantise(x):
     mx = np.where(none, 0, np.where(nan, np.float32(-np.inf), x).max(-1)).astype(np.float32)
     lo = np.clip(mn, -big, big).astype(np.float16)
     with np.errstate(all="ignore"):
-        d = ((np.clip(mx, -big, big) - lo.astype(np.float32)) / np.float32(15)).astype(np.float16)
+        d = ((np.clip(mx, -big, big) - lo.astype(np.float32)) * np.float32(1 / 15)).astype(np.float16)
         inv = np.where(d > 0, np.float32(1) / d.astype(np.float32), np.float32(0)).astype(np.float32)
         c = np.rint((x - lo.astype(np.float32)[..., None]) * inv[..., None])
     codes = np.clip(np.where(np.isnan(c), 0, c), 0, 15).astype(np.uint8)
