@@ -15,6 +15,7 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t type_bytes(int type) { return type == T_F32 ? 4 : type == T_F16 || type == T_BF16 ? 2 : 0; }
+constexpr float kMost = 1e30f;   // scale and soft cap: no infinity
 bool head_dim_ok(int D) { return D == 64 || D == 96 || D == 128; }
 
 // a row stride that holds `width` values and keeps rows on 16-byte boundaries
@@ -91,7 +92,7 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* c, int type, const void* q, 
                                int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
     if (!cache_ok(c) || !type_bytes(type) || T < 0 || T > 65535 || !q || !out || !tok_seq || !tok_pos || max_keys <= 0) return -1;
     const int D = c->head_dim, HKV = c->n_head_kv;
-    if (H <= 0 || H > 65535 || H % HKV || !(softcap >= 0.0f) || !(scale == scale) || window < 0) return -1;
+    if (H <= 0 || H > 65535 || H % HKV || !(softcap >= 0.0f) || softcap > kMost || !(scale > 0.0f) || scale > kMost || window < 0) return -1;
     if (!stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldo, (int64_t)H * D, type)) return -1;
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
     if (T == 0) return 0;
@@ -109,7 +110,7 @@ FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const vo
     if ((type != T_F16 && type != T_BF16) || !q || !k || !v || !out || !cu_seqlens || n_rows < 0 || n_seqs <= 0 ||
         n_seqs > (1 << 20) || n_rows > (1 << 30))
         return -1;
-    if (!head_dim_ok(D) || HKV <= 0 || H <= 0 || H % HKV || H > 65535 || !(softcap >= 0.0f) || !(scale == scale) || window < 0)
+    if (!head_dim_ok(D) || HKV <= 0 || H <= 0 || H % HKV || H > 65535 || H / HKV > 128 || !(softcap >= 0.0f) || softcap > kMost || !(scale > 0.0f) || scale > kMost || window < 0)
         return -1;
     if (!stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldkv, (int64_t)HKV * D, type) ||
         !stride_ok(ldo, (int64_t)H * D, type))

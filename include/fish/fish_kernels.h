@@ -180,8 +180,8 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* cache, int type, const void* q,
 
 /* Attention of T query tokens over the cache: token t (rotated queries q, H
  * heads in groups of H / n_head_kv) sees the positions 0..tok_pos[t] of its
- * sequence, or the last `window` of them (0: all); scores are scale * q.k,
- * then with softcap > 0 softcap * tanh(score / softcap). out has q's type;
+ * sequence, or the last `window` of them (0: all); scores are scale * q.k
+ * (scale > 0), then with softcap > 0 softcap * tanh(score / softcap). out has q's type;
  * rows of padding tokens (negative tok_pos) stay as they were, and a token
  * that sees nothing that can be read gets zeros. max_keys, an upper bound on
  * tok_pos + 1, sizes the split of long contexts (any value gives the right
@@ -196,7 +196,7 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
 
 /* Causal attention of n_seqs whole prompts packed one after another in the
  * rows of q [n_rows][H*D], k and v [n_rows][HKV*D] (F16 or BF16; D 64, 96 or
- * 128; H a multiple of HKV): sequence s has the rows cu_seqlens[s] ..
+ * 128; H a multiple of HKV, at most 128 times it): sequence s has the rows cu_seqlens[s] ..
  * cu_seqlens[s+1] - 1 (device array of n_seqs + 1 non-decreasing values from
  * 0.. to at most n_rows; empty sequences are fine), and row i sees the rows of
  * its sequence up to itself, or with window > 0 the last `window` of them. scale

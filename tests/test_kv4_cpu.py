@@ -81,7 +81,7 @@ def test_append_refuses(lib, bad):
 
 @pytest.mark.parametrize("bad", [dict(type=12), dict(T=-1), dict(T=70000), dict(q=None), dict(out=None), dict(seq=None),
                                  dict(pos=None), dict(max_keys=0), dict(H=0), dict(H=5), dict(ldq=511), dict(ldq=514),
-                                 dict(ldo=100), dict(softcap=-1.0), dict(softcap=float("nan")), dict(scale=float("nan")),
+                                 dict(ldo=100), dict(softcap=-1.0), dict(softcap=float("nan")), dict(scale=float("nan")), dict(scale=-1.0),
                                  dict(window=-1), dict(q=4100), dict(out=4100), dict(ws=4100)])
 def test_attention_refuses(lib, bad):
     assert attend(lib, **bad) == -1
@@ -98,7 +98,7 @@ def test_attention_refuses_a_small_workspace(lib):
 @pytest.mark.parametrize("bad", [dict(type=0), dict(type=8), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
                                  dict(cu=None), dict(rows=-1), dict(B=0), dict(B=-2), dict(H=0), dict(HKV=0), dict(H=5),
                                  dict(D=80), dict(D=256), dict(ldq=504), dict(ldq=516), dict(ldkv=248), dict(ldkv=260),
-                                 dict(ldo=511), dict(softcap=-0.5), dict(scale=float("nan")), dict(window=-3), dict(q=4100),
+                                 dict(ldo=511), dict(softcap=-0.5), dict(scale=float("nan")), dict(scale=0.0), dict(scale=float("inf")), dict(H=258, ldq=33024, ldo=33024), dict(window=-3), dict(q=4100),
                                  dict(k=4104), dict(v=8), dict(out=4097)])
 def test_packed_refuses(lib, bad):
     assert packed(lib, **bad) == -1
