@@ -1,7 +1,10 @@
 // kv4.cu — the paged cache held in 4 bits: append with RoPE, and attention of
 // single tokens over it.
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "launch.cuh"
+#include "tma.cuh"
 
 namespace fb {
 
@@ -128,96 +131,464 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 }
 
 // ================================================================ attention
-// One CTA a (token, kv head, 8 of its query heads); warp w takes the pages
-// w, w + 8, .. of the token's context, lane l the dimensions l, l + 32, ..
-constexpr int kV1Warps = 8;
+//   s_j = scale q . k_j,  k_j = lo_jg + d_jg c_j  (g the group of a dimension)
+//       = scale (sum_g d_jg (q_g . c_jg) + sum_g lo_jg sum(q_g))
+//   O   = sum_j p_j v_j = sum_j (p_j d_jg) (c_j - 8) + sum_j p_j (lo_jg + 8 d_jg)
+// so the 4-bit codes themselves go through the tensor cores (mma.sync
+// m16n8k16, f16 operands, exact), and scales meet sums, not values.
+//
+// CTA = (a run of the token's pages, kv head, up to 8 of its query heads,
+// token); each of its 8 warps takes every eighth page of the run, one bulk copy
+// a page and kv head (K and V codes and scales lie together, 2560 B at D = 128)
+// into the warp's own ring of kSlots. Per page:
+//   S^T[16 keys][8 heads] = K[16][D] Q^T: a k-step of 16 stays inside one
+//     group, and the group's two steps' sums are scaled by d of the row;
+//   O^T[16 dims][8 heads] += V^T P'^T, P' = p d per group, transposed in
+//     registers (movmatrix).
+// A row of an operand tile and its key differ by kv4_key (bank conflicts).
+// The weights' reference is kept per head and raised lazily; it counts the
+// largest d of the page too, so that p d, rounded to f16, keeps to 2^-14..2^15
+// whatever the values' scale is. f32 queries go in as two f16 parts, and so
+// do their weights (PL = 2); 16-bit ones are exact as one part.
+constexpr int kAtWarps = 8, kSlots = 4;
 
-__device__ __forceinline__ float code_at(const uint8_t* row, int byte, int n) { return (float)((row[byte] >> (4 * (n & 1))) & 15); }
+// key of row r of the 16-row operand tiles
+__device__ __forceinline__ int kv4_key(int r) { return (r & 8) | (r & 1 ? 4 + (((r >> 1) & 3) ^ 1) : (r >> 1) & 3); }
 
-template <class E, int D>
-__global__ void __launch_bounds__(32 * kV1Warps) k_kv4_attention(const __grid_constant__ fbx_kv4_cache c,
-                                                                 const E* __restrict__ q, int64_t ldq, int H,
-                                                                 const int32_t* __restrict__ tok_seq,
-                                                                 const int32_t* __restrict__ tok_pos, float scale,
-                                                                 float softcap, int window, E* out, int64_t ldo) {
+__device__ __forceinline__ float at_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// the 8 codes of w less `Mid` (0 or 8) as f16: r[n] = (code n, code n + 4). A
+// code dropped into the mantissa of 1024 or of 64 is off by that constant,
+// which is taken off exactly.
+template <int Mid>
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
+    const __half2 k1024 = bits_h2(Mid ? 0x64086408u : 0x64006400u), k64 = bits_h2(Mid ? 0x54805480u : 0x54005400u);
+    const uint32_t u = w >> 8;
+    r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), k1024));
+    r[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | 0x54005400u), k64));
+    r[2] = h2_bits(__hsub2(bits_h2((u & 0x000F000Fu) | 0x64006400u), k1024));
+    r[3] = h2_bits(__hsub2(bits_h2((u & 0x00F000F0u) | 0x54005400u), k64));
+}
+// n words (1..4) at p, aligned to the largest power of two that divides 4 n
+template <int N>
+__device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x; w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+// the V codes of one row piece: NG 16-bit words, two a 32-bit word
+template <int NG>
+__device__ __forceinline__ void halves(const uint8_t* p, uint32_t (&w)[(NG + 1) / 2]) {
+    if constexpr (NG == 3) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+        w[0] = h[0] | (uint32_t)h[1] << 16;
+        w[1] = h[2];
+    } else {
+        words<NG / 2>(p, w);
+    }
+}
+
+struct AtArgs {
+    fbx_kv4_cache c;
+    const void* q;
+    int64_t ldq;
+    int H;
+    const int32_t *tok_seq, *tok_pos;
+    float scale, softcap;
+    int window;
+    void* out;
+    int64_t ldo;
+    float* part;   // [token][kv head and run of 8 heads][split]: ref[8], sum[8], O[8][D]; null: one split, straight to out
+};
+
+template <int D>
+struct AtSmem {
     using R = Kv4Rec<D>;
+    static constexpr int q = kAtWarps * kSlots * R::bytes;     // f16 queries [2 parts][8][D]
+    static constexpr int qs = q + 2 * 8 * D * 2;               // sums of a group's queries [2 parts][8][4] f16
+    static constexpr int ex = qs + 2 * 8 * 4 * 2;              // the heads' exponents as factors [8]
+    static constexpr int bar = ex + 32;
+    static constexpr int bytes = bar + 8 * kAtWarps * kSlots;
+    // at the end, over the rings: [warps][8] ref, [warps][8] sum, [warps][8][D + 4] O
+    static constexpr int ml = 0, o = kAtWarps * 8 * 8;
+    static_assert(o + kAtWarps * 8 * (D + 4) * 4 <= q, "merge area");
+};
+
+template <class E, int D, int PL>
+__global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid_constant__ AtArgs A) {
+    using R = Kv4Rec<D>;
+    using M = AtSmem<D>;
+    constexpr int NG = R::NG, GP = R::GP;
+    extern __shared__ __align__(128) uint8_t sm[];
+    const fbx_kv4_cache& c = A.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int tok = blockIdx.z, G = A.H / c.n_head_kv, runs = (G + 7) / 8;
+    const int hk = blockIdx.y / runs, g0 = blockIdx.y % runs * 8, gn = min(8, G - g0), S = gridDim.x;
+    uint64_t* bar = reinterpret_cast<uint64_t*>(sm + M::bar) + warp * kSlots;
+    uint8_t* ring = sm + warp * kSlots * R::bytes;
     pdl_trigger();
+    if (lane < kSlots) mbar_init(&bar[lane], 1);
+    mbar_fence_init();
     pdl_wait();
-    const int t = blockIdx.z, hk = blockIdx.y, G = H / c.n_head_kv, g0 = blockIdx.x * 8, gn = min(8, G - g0);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int pos = tok_pos[t];
-    if (pos < 0) return;
-    const int seq = tok_seq[t];
+    const int pos = A.tok_pos[tok];
+    if (pos < 0) return;   // padding
+    const int seq = A.tok_seq[tok];
     const bool known = seq >= 0 && seq < c.n_seqs;
     if (!known && c.err && threadIdx.x == 0) atomicExch(c.err, 6);
-    __shared__ float sq[8][D], sm[kV1Warps][8], sl[kV1Warps][8], so[kV1Warps][8][D];
-    for (int i = threadIdx.x; i < 8 * D; i += blockDim.x)
-        sq[i / D][i % D] = i / D < gn ? to_f32<E>(q[t * ldq + (int64_t)(hk * G + g0 + i / D) * D + i % D]) : 0.0f;
-    __syncthreads();
-    float m[8], l[8], o[8][R::NG];
+
+    // this warp's pages: first, first + 8, .. below last; lane l holds the page of its l-th (of 32)
+    const int key0 = A.window > 0 ? max(0, pos - A.window + 1) : 0;
+    const int p0 = key0 / kKv4Page, p1 = min(pos / kKv4Page + 1, c.table_stride);
+    if (pos / kKv4Page >= c.table_stride && c.err && threadIdx.x == 0) atomicExch(c.err, 6);
+    const int per = (max(p1 - p0, 0) + S - 1) / S;
+    const int first = p0 + blockIdx.x * per + warp, last = min(p0 + ((int)blockIdx.x + 1) * per, p1);
+    const int n = known && first < last ? (last - first + kAtWarps - 1) / kAtWarps : 0;
+    auto look_up = [&](int k0) { return k0 + lane < n ? kv4_page(c, seq, first + (k0 + lane) * kAtWarps) : -1; };
+    int ids = look_up(0), ids_next = -1;
+    __syncwarp();
+    auto issue = [&](int k, int page) {
+        if (page >= 0 && lane == 0) {
+            mbar_expect_tx(&bar[k % kSlots], R::bytes);
+            bulk_g2s(ring + (k % kSlots) * R::bytes, kv4_record(c, page, hk, R::bytes), R::bytes, &bar[k % kSlots]);
+        }
+    };
+    for (int k = 0; k < kSlots && k < n; ++k) issue(k, __shfl_sync(0xffffffffu, ids, k));
+
+    // the queries: warp w brings head g0 + w to at most 2 in size, as f16 parts
+    {
+        float x[NG], top = 0.0f;
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.0f;
+        for (int e = 0; e < NG; ++e) {
+            x[e] = warp < gn ? to_f32<E>(static_cast<const E*>(A.q)[tok * A.ldq + (int64_t)(hk * G + g0 + warp) * D + 32 * e + lane]) : 0.0f;
+            top = fmaxf(top, fabsf(x[e]));
+        }
+        top = warp_max(top);
+        int ex = (int)(__float_as_uint(top) >> 23) - 127;
+        if (ex == 128 || top == 0.0f) ex = 0;
+        ex = min(max(ex, -120), 120);
+        const float down = __int_as_float((127 - ex) << 23);
+        __half* sq = reinterpret_cast<__half*>(sm + M::q);
+        __half* ss = reinterpret_cast<__half*>(sm + M::qs);
 #pragma unroll
-        for (int e = 0; e < R::NG; ++e) o[g][e] = 0.0f;
-    }
-    const int first = window > 0 ? max(0, pos - window + 1) : 0;
-    for (int i = first / kKv4Page + warp; known && i <= pos / kKv4Page; i += kV1Warps) {
-        const int page = kv4_page(c, seq, i);
-        if (page < 0) continue;
-        const uint8_t* rec = kv4_record(c, page, hk, R::bytes);
-        for (int j = 0; j < kKv4Page; ++j) {
-            const int key = i * kKv4Page + j;
-            if (key < first || key > pos) continue;
-            const int n = lane % 8, u = lane / 8, h = lane / 4;
-            float kx[R::NG], vx[R::NG];
-#pragma unroll
-            for (int e = 0; e < R::NG; ++e) {
-                const __half* sk = reinterpret_cast<const __half*>(rec + R::kd) + j * R::GP + e;
-                const __half* sv = reinterpret_cast<const __half*>(rec + R::vd) + j * R::GP + e;
-                kx[e] = __half2float(sk[kKv4Page * R::GP]) +
-                        __half2float(sk[0]) * code_at(rec + j * R::row, 4 * R::NG * u + 4 * e + n / 2, n);
-                const int hh = h ^ (((j >> 1) & 1) * 4);
-                vx[e] = __half2float(sv[kKv4Page * R::GP]) +
-                        __half2float(sv[0]) * code_at(rec + R::v + j * R::row, 2 * R::NG * hh + 2 * e + (lane % 4) / 2, lane);
-            }
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                if (g >= gn) break;
-                float s = 0.0f;
-#pragma unroll
-                for (int e = 0; e < R::NG; ++e) s += sq[g][32 * e + lane] * kx[e];
-                s = warp_sum(s) * scale;
-                if (softcap > 0.0f) s = softcap * tanhf(s / softcap);
-                const float mn = fmaxf(m[g], s), a = expf(m[g] - mn), p = expf(s - mn);
-                m[g] = mn;
-                l[g] = l[g] * a + p;
-#pragma unroll
-                for (int e = 0; e < R::NG; ++e) o[g][e] = o[g][e] * a + p * vx[e];
+        for (int e = 0; e < NG; ++e) {
+            const float y = x[e] * down;
+            const __half hi = __float2half_rn(y);
+            sq[warp * D + 32 * e + lane] = hi;
+            if (PL == 2) sq[(8 + warp) * D + 32 * e + lane] = __float2half_rn(y - __half2float(hi));
+            const float sum = warp_sum(y);
+            if (lane == 0) {
+                const __half h = __float2half_rn(sum);
+                ss[warp * 4 + e] = h;
+                ss[32 + warp * 4 + e] = __float2half_rn(sum - __half2float(h));
             }
         }
-    }
-    for (int g = 0; g < gn; ++g) {
         if (lane == 0) {
-            sm[warp][g] = m[g];
-            sl[warp][g] = l[g];
+            for (int e = NG; e < 4; ++e) ss[warp * 4 + e] = ss[32 + warp * 4 + e] = __float2half_rn(0.0f);
+            reinterpret_cast<float*>(sm + M::ex)[warp] = __int_as_float((127 + ex) << 23);
         }
-        for (int e = 0; e < R::NG; ++e) so[warp][g][32 * e + lane] = o[g][e];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < gn * D; i += blockDim.x) {
-        const int g = i / D, d = i % D;
-        float M = -INFINITY, S = 0.0f, O = 0.0f;
-        for (int w = 0; w < kV1Warps; ++w) M = fmaxf(M, sm[w][g]);
-        for (int w = 0; w < kV1Warps; ++w) {
-            if (sm[w][g] == -INFINITY) continue;
-            const float a = expf(sm[w][g] - M);
-            S += sl[w][g] * a;
-            O += so[w][g][d] * a;
+    // B operands of the scores: head g, dimensions 32 e + 8 t + (0, 4), (1, 5), (2, 6), (3, 7)
+    uint32_t qb[PL][NG][4];
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+        for (int e = 0; e < NG; ++e) {
+            const __half* s = reinterpret_cast<const __half*>(sm + M::q) + (8 * p + g) * D + 32 * e + 8 * t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qb[p][e][i] = h2_bits(__halves2half2(s[i], s[i + 4]));
         }
-        out[t * ldo + (int64_t)(hk * G + g0 + g) * D + d] = from_f32<E>(S > 0.0f ? O / S : 0.0f);
+    // and of sum_g lo sum(q_g): the sums' high parts against k = 0..3, their low parts against k = 4..7
+    const uint32_t qsb = *reinterpret_cast<const uint32_t*>(sm + M::qs + (t >> 1) * 64 + g * 8 + (t & 1) * 4);
+    constexpr float kLog2e = 1.4426950408889634f;
+    float cs[2];   // log2 units of the heads 2 t, 2 t + 1
+    const bool cap = A.softcap > 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) cs[i] = A.scale * reinterpret_cast<const float*>(sm + M::ex)[2 * t + i] * (cap ? 1.0f / A.softcap : kLog2e);
+    __syncthreads();   // the merge below writes over nothing that is still read
+
+    float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    float o[NG][2][4], olo[NG][2];   // O^T: dims 32 e + 4 g + 2 u + (0, 1), heads 2 t + (0, 1)
+#pragma unroll
+    for (int e = 0; e < NG; ++e) {
+        olo[e][0] = olo[e][1] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[e][u][i] = 0.0f;
     }
+    const int row = kv4_key(g);   // and row + 8
+    const int vrow = kv4_key(2 * t), vrow2 = kv4_key(2 * t + 1), piece = 2 * NG * (g ^ ((vrow & 2) << 1));
+    uint32_t phases = 0;
+    bool ok = true;
+    for (int k = 0; k < n; ++k) {
+        if ((k & 31) == 0 && k) ids = ids_next;
+        if ((k & 31) == 32 - kSlots) ids_next = look_up((k & ~31) + 32);
+        const int page = __shfl_sync(0xffffffffu, ids, k & 31);
+        const int slot = k % kSlots;
+        if (page >= 0) {
+            ok = ok && (mbar_try_wait(&bar[slot], (phases >> slot) & 1) || mbar_wait_bounded(&bar[slot], (phases >> slot) & 1));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            phases ^= 1u << slot;
+            const uint8_t* rec = ring + slot * R::bytes;
+            // ---- scores of keys row and row + 8 (accumulators 0, 1 and 2, 3), heads 2 t, 2 t + 1
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            {
+                const uint8_t* lo = rec + R::klo + (t & 1) * 4;
+                uint32_t l0 = 0, l1 = 0;
+                if (2 * (t & 1) < GP) {
+                    l0 = *reinterpret_cast<const uint32_t*>(lo + row * GP * 2);
+                    l1 = *reinterpret_cast<const uint32_t*>(lo + (row + 8) * GP * 2);
+                }
+                if (NG == 3 && (t & 1)) l0 &= 0xFFFFu, l1 &= 0xFFFFu;   // the padding
+                mma8(s, l0, l1, qsb);
+            }
+            uint32_t w0[NG], w1[NG], d0[GP / 2], d1[GP / 2];
+            words<NG>(rec + row * R::row + 4 * NG * t, w0);
+            words<NG>(rec + (row + 8) * R::row + 4 * NG * t, w1);
+            words<GP / 2>(rec + R::kd + row * GP * 2, d0);
+            words<GP / 2>(rec + R::kd + (row + 8) * GP * 2, d1);
+#pragma unroll
+            for (int e = 0; e < NG; ++e) {
+                uint32_t a[4], b[4];
+                codes8<0>(w0[e], a);
+                codes8<0>(w1[e], b);
+                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = 0; p < PL; ++p) {
+                    mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
+                    mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
+                }
+                const float da = __half2float(e & 1 ? __high2half(bits_h2(d0[e / 2])) : __low2half(bits_h2(d0[e / 2])));
+                const float db = __half2float(e & 1 ? __high2half(bits_h2(d1[e / 2])) : __low2half(bits_h2(d1[e / 2])));
+                s[0] = fmaf(da, x[0], s[0]);
+                s[1] = fmaf(da, x[1], s[1]);
+                s[2] = fmaf(db, x[2], s[2]);
+                s[3] = fmaf(db, x[3], s[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[i] *= cs[i & 1];
+                if (cap) s[i] = A.softcap * kLog2e * tanhf(s[i]);
+            }
+            // ---- V scales; at the edges of what the token sees, keys outside have no weight and no scale
+            uint32_t v0[GP / 2], v1[GP / 2], u0[GP / 2], u1[GP / 2];
+            words<GP / 2>(rec + R::vd + row * GP * 2, v0);
+            words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1);
+            words<GP / 2>(rec + R::vlo + row * GP * 2, u0);
+            words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1);
+            const int kb = (first + k * kAtWarps) * kKv4Page;
+            if (kb + kKv4Page - 1 > pos || kb < key0) {
+                const bool in0 = kb + row <= pos && kb + row >= key0, in1 = kb + row + 8 <= pos && kb + row + 8 >= key0;
+                if (!in0) s[0] = s[1] = -INFINITY;
+                if (!in1) s[2] = s[3] = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < GP / 2; ++e) {
+                    v0[e] = in0 ? v0[e] : 0u;
+                    u0[e] = in0 ? u0[e] : 0u;
+                    v1[e] = in1 ? v1[e] : 0u;
+                    u1[e] = in1 ? u1[e] : 0u;
+                }
+            }
+            // ---- the heads' references: the page's largest score and largest d, in log2 units
+            float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+            __half2 dm = __hmax2(bits_h2(v0[0]), bits_h2(v1[0]));
+#pragma unroll
+            for (int e = 1; e < GP / 2; ++e) {
+                // D = 96: the padding counts for nothing
+                const uint32_t keep = NG == 3 && e == 1 ? 0xFFFFu : 0xFFFFFFFFu;
+                dm = __hmax2(dm, __hmax2(bits_h2(v0[e] & keep), bits_h2(v1[e] & keep)));
+            }
+            dm = __hmax2(dm, __lowhigh2highlow(dm));
+#pragma unroll
+            for (int w = 4; w <= 16; w <<= 1) {
+                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
+                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
+                dm = __hmax2(dm, bits_h2(__shfl_xor_sync(0xffffffffu, h2_bits(dm), w)));
+            }
+            const float dtop = fmaxf(__low2float(dm), 5.9604645e-8f);
+            const float up = (float)((int)(__float_as_uint(dtop) >> 23) - 127);   // d < 2^(up + 1)
+            bool raise = false;
+            float to[2], f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool r = !(mx[i] + up <= ref[i] + 14.0f);   // NaN too
+                to[i] = r ? mx[i] + up - 10.0f : ref[i];
+                raise |= r;
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    f[i] = to[i] == ref[i] ? 1.0f : at_ex2(ref[i] - to[i]);
+                    ref[i] = to[i];
+                    sum[i] *= f[i];
+                }
+#pragma unroll
+                for (int e = 0; e < NG; ++e) {
+                    olo[e][0] *= f[0];
+                    olo[e][1] *= f[1];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        o[e][u][0] *= f[0];
+                        o[e][u][1] *= f[1];
+                        o[e][u][2] *= f[0];
+                        o[e][u][3] *= f[1];
+                    }
+                }
+            }
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = s[i] == -INFINITY ? 0.0f : at_ex2(s[i] - ref[i & 1]);
+            sum[0] += p[0] + p[2];
+            sum[1] += p[1] + p[3];
+            // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
+            uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
+            const uint8_t* vr = rec + R::v + piece;
+            halves<NG>(vr + vrow * R::row, va);
+            halves<NG>(vr + vrow2 * R::row, vb);
+            halves<NG>(vr + (vrow + 8) * R::row, vc);
+            halves<NG>(vr + (vrow2 + 8) * R::row, vd);
+#pragma unroll
+            for (int e = 0; e < NG; ++e) {
+                const float da = __half2float(e & 1 ? __high2half(bits_h2(v0[e / 2])) : __low2half(bits_h2(v0[e / 2])));
+                const float db = __half2float(e & 1 ? __high2half(bits_h2(v1[e / 2])) : __low2half(bits_h2(v1[e / 2])));
+                // codes of -8..7 around lo + 8 d: p d is rounded, so what it multiplies should be small
+                const float la = fmaf(8.0f, da, __half2float(e & 1 ? __high2half(bits_h2(u0[e / 2])) : __low2half(bits_h2(u0[e / 2]))));
+                const float lb = fmaf(8.0f, db, __half2float(e & 1 ? __high2half(bits_h2(u1[e / 2])) : __low2half(bits_h2(u1[e / 2]))));
+                olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
+                olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
+                const float x0 = p[0] * da, x1 = p[1] * da, x2 = p[2] * db, x3 = p[3] * db;
+                const __half2 hi0 = __floats2half2_rn(x0, x1), hi1 = __floats2half2_rn(x2, x3);
+                const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
+                uint32_t ra[4], rc[4];
+                codes8<8>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
+                codes8<8>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
+                if (PL == 2) {
+                    const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
+                    const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x0 - y0.x, x1 - y0.y)));
+                    const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x2 - y1.x, x3 - y1.y)));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
+                }
+            }
+            __syncwarp();   // the slot is read
+        }
+        if (k + kSlots < n) {
+            const int kn = k + kSlots;
+            const int next = __shfl_sync(0xffffffffu, (kn & ~31) == (k & ~31) ? ids : ids_next, kn & 31);
+            issue(kn, next);
+        }
+    }
+    if (!__all_sync(0xffffffffu, ok)) {   // a copy did not arrive in time: wait for what is in flight, report, go on with what there is
+        for (int i = 0; i < kSlots; ++i) mbar_wait_bounded(&bar[i], (phases >> i) & 1);
+        if (c.err && lane == 0) atomicExch(c.err, 7);
+    }
+    // ---- the lanes' sums over keys (those of other g), then the warps
+#pragma unroll
+    for (int w = 4; w <= 16; w <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], w);
+#pragma unroll
+            for (int e = 0; e < NG; ++e) olo[e][i] += __shfl_xor_sync(0xffffffffu, olo[e][i], w);
+        }
+    }
+    __syncthreads();   // every ring is done with
+    float* ml = reinterpret_cast<float*>(sm + M::ml);
+    float* so = reinterpret_cast<float*>(sm + M::o);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int h = 2 * t + i;
+        if (g == 0) {
+            ml[warp * 8 + h] = ref[i];
+            ml[64 + warp * 8 + h] = sum[i];
+        }
+#pragma unroll
+        for (int e = 0; e < NG; ++e)
+            *reinterpret_cast<float4*>(so + (warp * 8 + h) * (D + 4) + 32 * e + 4 * g) =
+                make_float4(o[e][0][i] + olo[e][i], o[e][0][2 + i] + olo[e][i], o[e][1][i] + olo[e][i], o[e][1][2 + i] + olo[e][i]);
+    }
+    __syncthreads();
+    float* part = A.part ? A.part + ((size_t)(tok * gridDim.y + blockIdx.y) * S + blockIdx.x) * (16 + 8 * D) : nullptr;
+    for (int i = threadIdx.x; i < gn * (D / 4); i += 32 * kAtWarps) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY, l = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kAtWarps; ++w) top = fmaxf(top, ml[w * 8 + h]);
+#pragma unroll
+        for (int w = 0; w < kAtWarps; ++w) {
+            const float f = ml[w * 8 + h] == -INFINITY ? 0.0f : at_ex2(ml[w * 8 + h] - top);
+            const float4 y = *reinterpret_cast<const float4*>(so + (w * 8 + h) * (D + 4) + d);
+            l = fmaf(f, ml[64 + w * 8 + h], l);
+            x.x = fmaf(f, y.x, x.x);
+            x.y = fmaf(f, y.y, x.y);
+            x.z = fmaf(f, y.z, x.z);
+            x.w = fmaf(f, y.w, x.w);
+        }
+        if (part) {
+            if (d == 0) {
+                part[h] = top;
+                part[8 + h] = l;
+            }
+            *reinterpret_cast<float4*>(part + 16 + h * D + d) = x;
+        } else {
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // NaN stays NaN
+            store4(static_cast<E*>(A.out) + tok * A.ldo + (int64_t)(hk * G + g0 + h) * D + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        }
+    }
+}
+
+// The splits of one (token, query head) joined: out = sum_s 2^(ref_s - top) O_s / sum_s 2^(ref_s - top) sum_s.
+template <class E, int D>
+__global__ void __launch_bounds__(D) k_kv4_join(const float* __restrict__ part, int S, int H, int HKV,
+                                                const int32_t* __restrict__ tok_pos, E* out, int64_t ldo) {
+    pdl_trigger();
+    pdl_wait();
+    const int tok = blockIdx.y, h = blockIdx.x, G = H / HKV, runs = (G + 7) / 8, d = threadIdx.x;
+    if (tok_pos[tok] < 0) return;
+    const int hk = h / G, hg = h % G;
+    const float* p = part + (size_t)(tok * HKV * runs + hk * runs + hg / 8) * S * (16 + 8 * D);
+    const int r = hg % 8;
+    float top = -INFINITY, l = 0.0f, o = 0.0f;
+    for (int s = 0; s < S; ++s) top = fmaxf(top, p[(size_t)s * (16 + 8 * D) + r]);
+    for (int s = 0; s < S; ++s) {
+        const float* ps = p + (size_t)s * (16 + 8 * D);
+        const float f = ps[r] == -INFINITY ? 0.0f : at_ex2(ps[r] - top);
+        l = fmaf(f, ps[8 + r], l);
+        o = fmaf(f, ps[16 + r * D + d], o);
+    }
+    out[tok * ldo + (int64_t)h * D + d] = from_f32<E>(l != 0.0f ? o / l : 0.0f);
 }
 
 // ---------------------------------------------------------------- launches
@@ -258,21 +629,35 @@ static cudaError_t append_o(const AppendArgs& a, int out_type, cudaStream_t st) 
          : out_type == T_F16 ? append_d<E, __half>(a, st) : append_d<E, __nv_bfloat16>(a, st);
 }
 
+// CTAs a token and kv head: as many as two an SM give, each warp of them with a page or more
+static int at_splits(int T, int H, int HKV, int max_keys) {
+    const int64_t pairs = (int64_t)T * HKV * ((H / HKV + 7) / 8);
+    const int pages = (max_keys - 1) / kKv4Page + 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * 148 / pairs, (pages + kAtWarps - 1) / kAtWarps));
+}
+
 template <class E, int D>
-static cudaError_t launch_kv4_attention(const fbx_kv4_cache& c, const void* q, int64_t ldq, int T, int H,
-                                        const int32_t* tok_seq, const int32_t* tok_pos, float scale, float softcap,
-                                        int window, void* out, int64_t ldo, cudaStream_t st) {
-    const int G = H / c.n_head_kv;
-    return fbk_launch(k_kv4_attention<E, D>, dim3((G + 7) / 8, c.n_head_kv, T), dim3(32 * kV1Warps), 0, st, c,
-                      (const E*)q, ldq, H, tok_seq, tok_pos, scale, softcap, window, (E*)out, ldo);
+static cudaError_t launch_kv4_attention(const AtArgs& a, int T, int S, cudaStream_t st) {
+    using M = AtSmem<D>;
+    constexpr int PL = sizeof(E) == 4 ? 2 : 1;
+    static uint64_t set = 0;   // one bit a device; setting it twice does no harm
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (!(__atomic_load_n(&set, __ATOMIC_RELAXED) >> (dev & 63) & 1)) {
+        e = cudaFuncSetAttribute(k_kv4_attention<E, D, PL>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::bytes);
+        if (e != cudaSuccess) return e;
+        __atomic_fetch_or(&set, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
+    }
+    const int HKV = a.c.n_head_kv;
+    e = fbk_launch(k_kv4_attention<E, D, PL>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
+    if (e != cudaSuccess || !a.part) return e;
+    return fbk_launch(k_kv4_join<E, D>, dim3(a.H, T), dim3(D), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
 }
 template <class E>
-static cudaError_t kv4_attention_d(const fbx_kv4_cache& c, const void* q, int64_t ldq, int T, int H,
-                                   const int32_t* tok_seq, const int32_t* tok_pos, float scale, float softcap,
-                                   int window, void* out, int64_t ldo, cudaStream_t st) {
-    return c.head_dim == 128 ? launch_kv4_attention<E, 128>(c, q, ldq, T, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, st)
-         : c.head_dim == 96 ? launch_kv4_attention<E, 96>(c, q, ldq, T, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, st)
-                            : launch_kv4_attention<E, 64>(c, q, ldq, T, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, st);
+static cudaError_t kv4_attention_d(const AtArgs& a, int T, int S, cudaStream_t st) {
+    return a.c.head_dim == 128 ? launch_kv4_attention<E, 128>(a, T, S, st)
+         : a.c.head_dim == 96 ? launch_kv4_attention<E, 96>(a, T, S, st) : launch_kv4_attention<E, 64>(a, T, S, st);
 }
 
 }  // namespace fb
@@ -289,12 +674,18 @@ extern "C" int fbk_kv4_append(const fbx_kv4_cache& c, int type, const void* q, c
                : type == T_F16 ? append_o<__half>(a, out_type, st) : append_o<__nv_bfloat16>(a, out_type, st));
 }
 
-extern "C" size_t fbk_kv4_attention_workspace(int, int, int, int, int) { return 0; }
+extern "C" size_t fbk_kv4_attention_workspace(int T, int H, int HKV, int D, int max_keys) {
+    const int S = at_splits(T, H, HKV, max_keys);
+    return S > 1 ? (size_t)T * HKV * ((H / HKV + 7) / 8) * S * (16 + 8 * D) * sizeof(float) : 0;
+}
 
 extern "C" int fbk_kv4_attention(const fbx_kv4_cache& c, int type, const void* q, int64_t ldq, int T, int H,
-                                 const int32_t* tok_seq, const int32_t* tok_pos, int, float scale, float softcap,
-                                 int window, void* out, int64_t ldo, void*, cudaStream_t st) {
-    return (int)(type == T_F32 ? kv4_attention_d<float>(c, q, ldq, T, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, st)
-               : type == T_F16 ? kv4_attention_d<__half>(c, q, ldq, T, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, st)
-                               : kv4_attention_d<__nv_bfloat16>(c, q, ldq, T, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, st));
+                                 const int32_t* tok_seq, const int32_t* tok_pos, int max_keys, float scale, float softcap,
+                                 int window, void* out, int64_t ldo, void* ws, cudaStream_t st) {
+    // a window bounds the keys too (it may begin inside a page); never more splits than the workspace was sized for
+    const int keys = window > 0 ? (int)std::min<int64_t>(max_keys, (int64_t)window + kKv4Page) : max_keys;
+    const int S = at_splits(T, H, c.n_head_kv, keys);
+    const AtArgs a{c, q, ldq, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, S > 1 ? (float*)ws : nullptr};
+    return (int)(type == T_F32 ? kv4_attention_d<float>(a, T, S, st)
+               : type == T_F16 ? kv4_attention_d<__half>(a, T, S, st) : kv4_attention_d<__nv_bfloat16>(a, T, S, st));
 }

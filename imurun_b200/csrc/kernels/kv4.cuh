@@ -86,6 +86,22 @@ __device__ __forceinline__ void store8(E* p, const float (&x)[8]) {
     }
 }
 
+// 4 consecutive values at a boundary of 4
+template <class E>
+__device__ __forceinline__ void store4(E* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(E) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+    } else {
+        uint2 raw;
+        E* e = reinterpret_cast<E*>(&raw);
+        e[0] = from_f32<E>(a);
+        e[1] = from_f32<E>(b);
+        e[2] = from_f32<E>(c);
+        e[3] = from_f32<E>(d);
+        *reinterpret_cast<uint2*>(p) = raw;
+    }
+}
+
 }  // namespace fb
 
 extern "C" {

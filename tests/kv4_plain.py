@@ -89,8 +89,8 @@ def store(pool, at, row, is_v, D, codes, d, lo):
     pool[sc: sc + 2 * (D // 32)] = lo.view(np.uint8)
 
 
-def fetch(pool, at, D):
-    """K and V [16][D] in 64 bits of the record at byte `at`."""
+def fetch(pool, at, D, steps=False):
+    """K and V [16][D] in 64 bits of the record at byte `at`; with steps, V's d of every value too."""
     gp, out = groups_padded(D), []
     for is_v in (False, True):
         base = at + (record_bytes(D) // 2 if is_v else 0)
@@ -102,14 +102,17 @@ def fetch(pool, at, D):
             c = (pool[base + row * D // 2 + at_b] >> (4 * (np.arange(D) & 1)).astype(np.uint8)) & 15
             x[row] = lo[row, np.arange(D) // 32] + d[row, np.arange(D) // 32] * c
         out.append(x)
+        if steps and is_v:
+            out.append(d[:, np.arange(D) // 32])
     return out
 
 
-def attend(q, k, v, pos, scale, softcap=0.0, window=0):
+def attend(q, k, v, pos, scale, softcap=0.0, window=0, steps=None):
     """Attention of queries q [rows][D] at positions pos over k, v [keys][D] in
-    64 bits, and what bounds its error: sum p |v| and the largest sum |q k|."""
+    64 bits, and what bounds its error: sum p |v| and the largest sum |q k|;
+    with steps [keys][D], sum p steps too."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
-    out, mean, ext = np.zeros_like(q), np.zeros_like(q), np.zeros(len(q))
+    out, mean, ext, coarse = np.zeros_like(q), np.zeros_like(q), np.zeros(len(q)), np.zeros_like(q)
     for r, p in enumerate(pos):
         a = max(0, p - window + 1) if window else 0
         kk, vv = k[a:p + 1], v[a:p + 1]
@@ -122,10 +125,12 @@ def attend(q, k, v, pos, scale, softcap=0.0, window=0):
         w = np.exp(s - s.max())
         w /= w.sum()
         out[r], mean[r] = w @ vv, w @ np.abs(vv)
-    return out, mean, ext
+        if steps is not None:
+            coarse[r] = w @ steps[a:p + 1]
+    return (out, mean, ext) if steps is None else (out, mean, ext, coarse)
 
 
-def allowed(out, mean, ext, t, weights, softcap=0.0):
+def allowed(out, mean, ext, t, weights, softcap=0.0, coarse=None):
     """How far an output of type t may be off. A score is a sum of products
     accumulated in 32 bits: off by 2^-20 of sum |q k| at most (operands of two
     f16 parts: 2^-22; sums of 128 terms in a truncating adder: under 2^-20), a
@@ -133,7 +138,15 @@ def allowed(out, mean, ext, t, weights, softcap=0.0):
     (itself and its share of the sum), plus 2^-20 for the exponential and the
     sums, plus `weights`, the rounding of a weight before its product with v.
     An output is off by that share of sum p |v|, then rounded to t (with the
-    smallest step of f16)."""
+    smallest step of f16).
+
+    Over the cache, v = (lo + 8 d) + d (code - 8) is summed in two parts: the
+    rounded weight p d meets |code - 8| <= 8, so `weights` is a share of sum p 8
+    d, and both parts together, |lo + 8 d| + 8 d <= |v| + 16 d, carry the 2^-20
+    of the sums. coarse is sum p d."""
     ds = 2.0 ** -20 * ext + 2.0 ** -21 * softcap
-    share = 2 * ds + 2.0 ** -20 + weights
-    return share[:, None] * mean * 1.01 + HALF[t] * np.abs(out) + 2.0 ** -25
+    if coarse is None:
+        off = (2 * ds + 2.0 ** -20 + weights)[:, None] * mean
+    else:
+        off = 2 * ds[:, None] * mean + 2.0 ** -20 * (mean + 16 * coarse) + weights * 8 * coarse
+    return off * 1.01 + HALF[t] * np.abs(out) + 2.0 ** -25
