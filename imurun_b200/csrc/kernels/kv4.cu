@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 // ================================================================ attention
 //   s_j = scale q . k_j,  k_j = lo_jg + d_jg c_j  (g the group of a dimension)
 //       = scale (sum_g d_jg (q_g . c_jg) + sum_g lo_jg sum(q_g))
-//   O   = sum_j p_j v_j = sum_j (p_j d_jg) (c_j - 8) + sum_j p_j (lo_jg + 8 d_jg)
+//   O   = sum_j p_j v_j = sum_j (p_j d_jg) c_j + sum_j p_j lo_jg
 // so the 4-bit codes themselves go through the tensor cores (mma.sync
 // m16n8k16, f16 operands, exact), and scales meet sums, not values.
 //
@@ -146,10 +146,25 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 //   O^T[16 dims][8 heads] += V^T P'^T, P' = p d per group, transposed in
 //     registers (movmatrix).
 // A row of an operand tile and its key differ by kv4_key (bank conflicts).
-// The weights' reference is kept per head and raised lazily; it counts the
-// largest d of the page too, so that p d, rounded to f16, keeps to 2^-14..2^15
-// whatever the values' scale is. f32 queries go in as two f16 parts, and so
-// do their weights (PL = 2); 16-bit ones are exact as one part.
+//
+// What bounds it is instructions: at the full HBM rate an SM has 111 cycles for
+// a page of 128 dimensions, that is 4096 values. So for 16-bit types a code is
+// moved to bits 4..7 of its half and used as it lies, the f16 subnormal c 2^-20
+// (tensor cores take subnormals as they are). A product's place in the adder
+// goes by the exponent field, so c 2^-20 keeps 6 to 10 bits less than a normal
+// operand would, about 2^-20 of the sum; f32 calls, which want more, take normal
+// operands at two more instructions a word. And no maximum is formed over a
+// page: the weights' reference is raised only when some lane's weight passes
+// 2^14, the common exponent 2^E of V's scales only when some d passes 2^(E + 1);
+// both rescale what was summed, a few times a context. With p <= 2^14 and
+// d 2^-E <= 2 the products stay in f16's range whatever the values' size is.
+//
+// Roundings: 16-bit queries are exact in one f16 part (scaled by a power of
+// two), f32 ones go in as two, and so do their weights p d (2^-22). For f16
+// outputs p d is rounded once and meets codes of -8..7 (8 sum(p d) is taken off
+// by one more MMA a group, and lo + 8 d stands for lo), else the rounding would
+// be the larger part of the error; for bf16, whose own step is 8 times as
+// wide, p is rounded first and codes stay 0..15.
 constexpr int kAtWarps = 8, kSlots = 4;
 
 // key of row r of the 16-row operand tiles
@@ -178,18 +193,27 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// the 8 codes of w less `Mid` (0 or 8) as f16: r[n] = (code n, code n + 4). A
-// code dropped into the mantissa of 1024 or of 64 is off by that constant,
-// which is taken off exactly.
-template <int Mid>
+// The 8 codes of w as f16, r[n] = (code n, code n + 4). Sub: as subnormals of
+// 2^-20; else as they are (dropped into the mantissa of 1024 or of 64, which is
+// taken off exactly).
+template <bool Sub>
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
-    const __half2 k1024 = bits_h2(Mid ? 0x64086408u : 0x64006400u), k64 = bits_h2(Mid ? 0x54805480u : 0x54005400u);
-    const uint32_t u = w >> 8;
-    r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), k1024));
-    r[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | 0x54005400u), k64));
-    r[2] = h2_bits(__hsub2(bits_h2((u & 0x000F000Fu) | 0x64006400u), k1024));
-    r[3] = h2_bits(__hsub2(bits_h2((u & 0x00F000F0u) | 0x54005400u), k64));
+    if (Sub) {
+        r[0] = (w << 4) & 0x00F000F0u;
+        r[1] = w & 0x00F000F0u;
+        r[2] = (w >> 4) & 0x00F000F0u;
+        r[3] = (w >> 8) & 0x00F000F0u;
+    } else {
+        const __half2 k1024 = bits_h2(0x64006400u), k64 = bits_h2(0x54005400u);
+        const uint32_t u = w >> 8;
+        r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), k1024));
+        r[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | 0x54005400u), k64));
+        r[2] = h2_bits(__hsub2(bits_h2((u & 0x000F000Fu) | 0x64006400u), k1024));
+        r[3] = h2_bits(__hsub2(bits_h2((u & 0x00F000F0u) | 0x54005400u), k64));
+    }
 }
+template <int I>   // half I of a pair as f32
+__device__ __forceinline__ float half_at(uint32_t u) { return I ? __high2float(bits_h2(u)) : __low2float(bits_h2(u)); }
 // n words (1..4) at p, aligned to the largest power of two that divides 4 n
 template <int N>
 __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
@@ -242,11 +266,19 @@ struct AtSmem {
     static_assert(o + kAtWarps * 8 * (D + 4) * 4 <= q, "merge area");
 };
 
-template <class E, int D, int PL>
+// how the weights of an element type go into the products with V (see above)
+enum : int { W_PAIR, W_MID, W_HALF };
+template <class E> struct AtWeights { static constexpr int mode = W_PAIR; };
+template <> struct AtWeights<__half> { static constexpr int mode = W_MID; };
+template <> struct AtWeights<__nv_bfloat16> { static constexpr int mode = W_HALF; };
+
+template <class E, int D>
 __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid_constant__ AtArgs A) {
     using R = Kv4Rec<D>;
     using M = AtSmem<D>;
-    constexpr int NG = R::NG, GP = R::GP;
+    constexpr int NG = R::NG, GP = R::GP, PL = sizeof(E) == 4 ? 2 : 1, W = AtWeights<E>::mode;
+    constexpr bool SUB = W != W_PAIR;
+    constexpr float kCode = SUB ? 1048576.0f : 1.0f;   // a code over its operand
     extern __shared__ __align__(128) uint8_t sm[];
     const fbx_kv4_cache& c = A.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -274,10 +306,14 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     auto look_up = [&](int k0) { return k0 + lane < n ? kv4_page(c, seq, first + (k0 + lane) * kAtWarps) : -1; };
     int ids = look_up(0), ids_next = -1;
     __syncwarp();
-    auto issue = [&](int k, int page) {
-        if (page >= 0 && lane == 0) {
-            mbar_expect_tx(&bar[k % kSlots], R::bytes);
-            bulk_g2s(ring + (k % kSlots) * R::bytes, kv4_record(c, page, hk, R::bytes), R::bytes, &bar[k % kSlots]);
+    auto issue = [&](int k, int page) {   // no page: the slot's phase passes empty
+        if (lane == 0) {
+            if (page >= 0) {
+                mbar_expect_tx(&bar[k % kSlots], R::bytes);
+                bulk_g2s(ring + (k % kSlots) * R::bytes, kv4_record(c, page, hk, R::bytes), R::bytes, &bar[k % kSlots]);
+            } else {
+                mbar_arrive(&bar[k % kSlots]);
+            }
         }
     };
     for (int k = 0; k < kSlots && k < n; ++k) issue(k, __shfl_sync(0xffffffffu, ids, k));
@@ -329,38 +365,42 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     // and of sum_g lo sum(q_g): the sums' high parts against k = 0..3, their low parts against k = 4..7
     const uint32_t qsb = *reinterpret_cast<const uint32_t*>(sm + M::qs + (t >> 1) * 64 + g * 8 + (t & 1) * 4);
     constexpr float kLog2e = 1.4426950408889634f;
-    float cs[2];   // log2 units of the heads 2 t, 2 t + 1
+    float cs[2], csc[2];   // log2 units of the heads 2 t, 2 t + 1, and of the code products
     const bool cap = A.softcap > 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) cs[i] = A.scale * reinterpret_cast<const float*>(sm + M::ex)[2 * t + i] * (cap ? 1.0f / A.softcap : kLog2e);
-    __syncthreads();   // the merge below writes over nothing that is still read
-
+    for (int i = 0; i < 2; ++i) {
+        cs[i] = A.scale * reinterpret_cast<const float*>(sm + M::ex)[2 * t + i] * (cap ? 1.0f / A.softcap : kLog2e);
+        csc[i] = cs[i] * kCode;
+    }
     float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    float o[NG][2][4], olo[NG][2];   // O^T: dims 32 e + 4 g + 2 u + (0, 1), heads 2 t + (0, 1)
+    int top_e = 0;                          // E
+    __half2 down_e = __float2half2_rn(0.0f), limit_e = down_e;   // 2^-E, 2^(E + 1); a limit of 0 is passed by the first page
+    // O^T 2^-E / kCode: dims 32 e + 4 g + 2 u (accumulators 0, 1) and the next (2, 3), heads 2 t + (0, 1)
+    float o[NG][2][4], olo[NG][2], mid[W == W_MID ? NG : 1][4];
 #pragma unroll
     for (int e = 0; e < NG; ++e) {
         olo[e][0] = olo[e][1] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[e][u][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            o[e][0][i] = o[e][1][i] = 0.0f;
+            if (W == W_MID) mid[e][i] = 0.0f;
+        }
     }
     const int row = kv4_key(g);   // and row + 8
     const int vrow = kv4_key(2 * t), vrow2 = kv4_key(2 * t + 1), piece = 2 * NG * (g ^ ((vrow & 2) << 1));
-    uint32_t phases = 0;
     bool ok = true;
     for (int k = 0; k < n; ++k) {
         if ((k & 31) == 0 && k) ids = ids_next;
         if ((k & 31) == 32 - kSlots) ids_next = look_up((k & ~31) + 32);
         const int page = __shfl_sync(0xffffffffu, ids, k & 31);
         const int slot = k % kSlots;
+        const uint32_t parity = (uint32_t)(k / kSlots) & 1u;
+        ok = ok && (mbar_try_wait(&bar[slot], parity) || mbar_wait_bounded(&bar[slot], parity));
+        __syncwarp();
         if (page >= 0) {
-            ok = ok && (mbar_try_wait(&bar[slot], (phases >> slot) & 1) || mbar_wait_bounded(&bar[slot], (phases >> slot) & 1));
-            if (!__all_sync(0xffffffffu, ok)) break;
-            phases ^= 1u << slot;
             const uint8_t* rec = ring + slot * R::bytes;
             // ---- scores of keys row and row + 8 (accumulators 0, 1 and 2, 3), heads 2 t, 2 t + 1
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float sl[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s[4];
             {
                 const uint8_t* lo = rec + R::klo + (t & 1) * 4;
                 uint32_t l0 = 0, l1 = 0;
@@ -369,7 +409,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                     l1 = *reinterpret_cast<const uint32_t*>(lo + (row + 8) * GP * 2);
                 }
                 if (NG == 3 && (t & 1)) l0 &= 0xFFFFu, l1 &= 0xFFFFu;   // the padding
-                mma8(s, l0, l1, qsb);
+                mma8(sl, l0, l1, qsb);
             }
             uint32_t w0[NG], w1[NG], d0[GP / 2], d1[GP / 2];
             words<NG>(rec + row * R::row + 4 * NG * t, w0);
@@ -379,25 +419,26 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
 #pragma unroll
             for (int e = 0; e < NG; ++e) {
                 uint32_t a[4], b[4];
-                codes8<0>(w0[e], a);
-                codes8<0>(w1[e], b);
+                codes8<SUB>(w0[e], a);
+                codes8<SUB>(w1[e], b);
                 float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int p = 0; p < PL; ++p) {
                     mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
                     mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
                 }
-                const float da = __half2float(e & 1 ? __high2half(bits_h2(d0[e / 2])) : __low2half(bits_h2(d0[e / 2])));
-                const float db = __half2float(e & 1 ? __high2half(bits_h2(d1[e / 2])) : __low2half(bits_h2(d1[e / 2])));
-                s[0] = fmaf(da, x[0], s[0]);
-                s[1] = fmaf(da, x[1], s[1]);
-                s[2] = fmaf(db, x[2], s[2]);
-                s[3] = fmaf(db, x[3], s[3]);
+                const float da = e & 1 ? half_at<1>(d0[e / 2]) : half_at<0>(d0[e / 2]);
+                const float db = e & 1 ? half_at<1>(d1[e / 2]) : half_at<0>(d1[e / 2]);
+                s[0] = e ? fmaf(da, x[0], s[0]) : da * x[0];
+                s[1] = e ? fmaf(da, x[1], s[1]) : da * x[1];
+                s[2] = e ? fmaf(db, x[2], s[2]) : db * x[2];
+                s[3] = e ? fmaf(db, x[3], s[3]) : db * x[3];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[i] *= cs[i & 1];
-                if (cap) s[i] = A.softcap * kLog2e * tanhf(s[i]);
+            for (int i = 0; i < 4; ++i) s[i] = fmaf(s[i], csc[i & 1], sl[i] * cs[i & 1]);
+            if (cap) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = A.softcap * kLog2e * tanhf(s[i]);
             }
             // ---- V scales; at the edges of what the token sees, keys outside have no weight and no scale
             uint32_t v0[GP / 2], v1[GP / 2], u0[GP / 2], u1[GP / 2];
@@ -405,6 +446,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1);
             words<GP / 2>(rec + R::vlo + row * GP * 2, u0);
             words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1);
+            if (NG == 3) v0[1] &= 0xFFFFu, v1[1] &= 0xFFFFu;
             const int kb = (first + k * kAtWarps) * kKv4Page;
             if (kb + kKv4Page - 1 > pos || kb < key0) {
                 const bool in0 = kb + row <= pos && kb + row >= key0, in1 = kb + row + 8 <= pos && kb + row + 8 >= key0;
@@ -418,57 +460,54 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                     u1[e] = in1 ? u1[e] : 0u;
                 }
             }
-            // ---- the heads' references: the page's largest score and largest d, in log2 units
-            float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+            // ---- the references, raised when a weight passes 2^14 or a scale 2^(E + 1)
             __half2 dm = __hmax2(bits_h2(v0[0]), bits_h2(v1[0]));
 #pragma unroll
-            for (int e = 1; e < GP / 2; ++e) {
-                // D = 96: the padding counts for nothing
-                const uint32_t keep = NG == 3 && e == 1 ? 0xFFFFu : 0xFFFFFFFFu;
-                dm = __hmax2(dm, __hmax2(bits_h2(v0[e] & keep), bits_h2(v1[e] & keep)));
-            }
-            dm = __hmax2(dm, __lowhigh2highlow(dm));
+            for (int e = 1; e < GP / 2; ++e) dm = __hmax2(dm, __hmax2(bits_h2(v0[e]), bits_h2(v1[e])));
+            const bool wide = !__hble2(dm, limit_e);
+            const bool high = fmaxf(fmaxf(s[0], s[2]) - ref[0], fmaxf(s[1], s[3]) - ref[1]) > 14.0f;
+            if (__any_sync(0xffffffffu, wide || high)) {
+                float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])}, dtop = fmaxf(__low2float(dm), __high2float(dm));
 #pragma unroll
-            for (int w = 4; w <= 16; w <<= 1) {
-                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
-                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
-                dm = __hmax2(dm, bits_h2(__shfl_xor_sync(0xffffffffu, h2_bits(dm), w)));
-            }
-            const float dtop = fmaxf(__low2float(dm), 5.9604645e-8f);
-            const float up = (float)((int)(__float_as_uint(dtop) >> 23) - 127);   // d < 2^(up + 1)
-            bool raise = false;
-            float to[2], f[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool r = !(mx[i] + up <= ref[i] + 14.0f);   // NaN too
-                to[i] = r ? mx[i] + up - 10.0f : ref[i];
-                raise |= r;
-            }
-            if (__any_sync(0xffffffffu, raise)) {
+                for (int w = 4; w <= 16; w <<= 1) {
+                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
+                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
+                    dtop = fmaxf(dtop, __shfl_xor_sync(0xffffffffu, dtop, w));
+                }
+                const int e_new = max((int)(__float_as_uint(fmaxf(dtop, 0.0f)) >> 23) - 127, -15);   // d < 2^(e_new + 1)
+                float f_e = 1.0f;
+                if (limit_e.x == __half(0.0f) || e_new > top_e) {
+                    f_e = limit_e.x == __half(0.0f) ? 1.0f : __int_as_float((127 + top_e - e_new) << 23);
+                    top_e = e_new;
+                    down_e = __float2half2_rn(__int_as_float((127 - e_new) << 23));
+                    limit_e = __float2half2_rn(__int_as_float((128 + e_new) << 23));
+                }
+                float f[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    f[i] = to[i] == ref[i] ? 1.0f : at_ex2(ref[i] - to[i]);
-                    ref[i] = to[i];
+                    const float to = mx[i] - ref[i] > 14.0f ? mx[i] - 8.0f : ref[i];   // from -inf too
+                    f[i] = to == ref[i] ? 1.0f : at_ex2(ref[i] - to);
+                    ref[i] = to;
                     sum[i] *= f[i];
                 }
 #pragma unroll
                 for (int e = 0; e < NG; ++e) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[e][0][i] *= f[i & 1] * f_e;
+                        o[e][1][i] *= f[i & 1] * f_e;
+                        if (W == W_MID) mid[e][i] *= f[i & 1] * f_e;
+                    }
                     olo[e][0] *= f[0];
                     olo[e][1] *= f[1];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        o[e][u][0] *= f[0];
-                        o[e][u][1] *= f[1];
-                        o[e][u][2] *= f[0];
-                        o[e][u][3] *= f[1];
-                    }
                 }
             }
             float p[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = s[i] == -INFINITY ? 0.0f : at_ex2(s[i] - ref[i & 1]);
+            for (int i = 0; i < 4; ++i) p[i] = at_ex2(s[i] - ref[i & 1]);
             sum[0] += p[0] + p[2];
             sum[1] += p[1] + p[3];
+            const __half2 p0 = __floats2half2_rn(p[0], p[1]), p1 = __floats2half2_rn(p[2], p[3]);
             // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
             uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
             const uint8_t* vr = rec + R::v + piece;
@@ -478,25 +517,40 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             halves<NG>(vr + (vrow2 + 8) * R::row, vd);
 #pragma unroll
             for (int e = 0; e < NG; ++e) {
-                const float da = __half2float(e & 1 ? __high2half(bits_h2(v0[e / 2])) : __low2half(bits_h2(v0[e / 2])));
-                const float db = __half2float(e & 1 ? __high2half(bits_h2(v1[e / 2])) : __low2half(bits_h2(v1[e / 2])));
-                // codes of -8..7 around lo + 8 d: p d is rounded, so what it multiplies should be small
-                const float la = fmaf(8.0f, da, __half2float(e & 1 ? __high2half(bits_h2(u0[e / 2])) : __low2half(bits_h2(u0[e / 2]))));
-                const float lb = fmaf(8.0f, db, __half2float(e & 1 ? __high2half(bits_h2(u1[e / 2])) : __low2half(bits_h2(u1[e / 2]))));
+                const __half2 n0 = __hmul2(bits_h2(v0[e / 2]), down_e), n1 = __hmul2(bits_h2(v1[e / 2]), down_e);   // d 2^-E
+                float la = e & 1 ? half_at<1>(u0[e / 2]) : half_at<0>(u0[e / 2]);
+                float lb = e & 1 ? half_at<1>(u1[e / 2]) : half_at<0>(u1[e / 2]);
+                if (W == W_MID) {
+                    la = fmaf(8.0f, e & 1 ? half_at<1>(v0[e / 2]) : half_at<0>(v0[e / 2]), la);
+                    lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[e / 2]) : half_at<0>(v1[e / 2]), lb);
+                }
                 olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
                 olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
-                const float x0 = p[0] * da, x1 = p[1] * da, x2 = p[2] * db, x3 = p[3] * db;
-                const __half2 hi0 = __floats2half2_rn(x0, x1), hi1 = __floats2half2_rn(x2, x3);
-                const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
                 uint32_t ra[4], rc[4];
-                codes8<8>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
-                codes8<8>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+                codes8<SUB>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
+                codes8<SUB>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+                __half2 hi0, hi1;
+                float x[4];
+                if (W == W_HALF) {
+                    hi0 = __hmul2(p0, e & 1 ? __high2half2(n0) : __low2half2(n0));
+                    hi1 = __hmul2(p1, e & 1 ? __high2half2(n1) : __low2half2(n1));
+                } else {
+                    const float da = e & 1 ? __high2float(n0) : __low2float(n0), db = e & 1 ? __high2float(n1) : __low2float(n1);
+                    x[0] = p[0] * da;
+                    x[1] = p[1] * da;
+                    x[2] = p[2] * db;
+                    x[3] = p[3] * db;
+                    hi0 = __floats2half2_rn(x[0], x[1]);
+                    hi1 = __floats2half2_rn(x[2], x[3]);
+                }
+                const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
-                if (PL == 2) {
+                if (W == W_MID) mma16(mid[e], 0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u, b0, b1);   // -8
+                if (W == W_PAIR) {
                     const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
-                    const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x0 - y0.x, x1 - y0.y)));
-                    const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x2 - y1.x, x3 - y1.y)));
+                    const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x[0] - y0.x, x[1] - y0.y)));
+                    const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x[2] - y1.x, x[3] - y1.y)));
 #pragma unroll
                     for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
                 }
@@ -509,10 +563,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             issue(kn, next);
         }
     }
-    if (!__all_sync(0xffffffffu, ok)) {   // a copy did not arrive in time: wait for what is in flight, report, go on with what there is
-        for (int i = 0; i < kSlots; ++i) mbar_wait_bounded(&bar[i], (phases >> i) & 1);
-        if (c.err && lane == 0) atomicExch(c.err, 7);
-    }
+    if (!__all_sync(0xffffffffu, ok) && c.err && lane == 0) atomicExch(c.err, 7);   // a copy did not arrive in time
     // ---- the lanes' sums over keys (those of other g), then the warps
 #pragma unroll
     for (int w = 4; w <= 16; w <<= 1) {
@@ -534,9 +585,11 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             ml[64 + warp * 8 + h] = sum[i];
         }
 #pragma unroll
-        for (int e = 0; e < NG; ++e)
+        for (int e = 0; e < NG; ++e) {
+            const float up = __int_as_float((127 + top_e) << 23) * kCode, l = olo[e][i] + (W == W_MID ? up * mid[e][i] : 0.0f);
             *reinterpret_cast<float4*>(so + (warp * 8 + h) * (D + 4) + 32 * e + 4 * g) =
-                make_float4(o[e][0][i] + olo[e][i], o[e][0][2 + i] + olo[e][i], o[e][1][i] + olo[e][i], o[e][1][2 + i] + olo[e][i]);
+                make_float4(fmaf(up, o[e][0][i], l), fmaf(up, o[e][0][2 + i], l), fmaf(up, o[e][1][i], l), fmaf(up, o[e][1][2 + i], l));
+        }
     }
     __syncthreads();
     float* part = A.part ? A.part + ((size_t)(tok * gridDim.y + blockIdx.y) * S + blockIdx.x) * (16 + 8 * D) : nullptr;
@@ -548,7 +601,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         for (int w = 0; w < kAtWarps; ++w) top = fmaxf(top, ml[w * 8 + h]);
 #pragma unroll
         for (int w = 0; w < kAtWarps; ++w) {
-            const float f = ml[w * 8 + h] == -INFINITY ? 0.0f : at_ex2(ml[w * 8 + h] - top);
+            const float f = ml[w * 8 + h] == -INFINITY && ml[64 + w * 8 + h] == 0.0f ? 0.0f : at_ex2(ml[w * 8 + h] - top);   // NaN stays
             const float4 y = *reinterpret_cast<const float4*>(so + (w * 8 + h) * (D + 4) + d);
             l = fmaf(f, ml[64 + w * 8 + h], l);
             x.x = fmaf(f, y.x, x.x);
@@ -584,7 +637,7 @@ __global__ void __launch_bounds__(D) k_kv4_join(const float* __restrict__ part, 
     for (int s = 0; s < S; ++s) top = fmaxf(top, p[(size_t)s * (16 + 8 * D) + r]);
     for (int s = 0; s < S; ++s) {
         const float* ps = p + (size_t)s * (16 + 8 * D);
-        const float f = ps[r] == -INFINITY ? 0.0f : at_ex2(ps[r] - top);
+        const float f = ps[r] == -INFINITY && ps[8 + r] == 0.0f ? 0.0f : at_ex2(ps[r] - top);
         l = fmaf(f, ps[8 + r], l);
         o = fmaf(f, ps[16 + r * D + d], o);
     }
@@ -639,18 +692,17 @@ static int at_splits(int T, int H, int HKV, int max_keys) {
 template <class E, int D>
 static cudaError_t launch_kv4_attention(const AtArgs& a, int T, int S, cudaStream_t st) {
     using M = AtSmem<D>;
-    constexpr int PL = sizeof(E) == 4 ? 2 : 1;
     static uint64_t set = 0;   // one bit a device; setting it twice does no harm
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!(__atomic_load_n(&set, __ATOMIC_RELAXED) >> (dev & 63) & 1)) {
-        e = cudaFuncSetAttribute(k_kv4_attention<E, D, PL>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::bytes);
+        e = cudaFuncSetAttribute(k_kv4_attention<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::bytes);
         if (e != cudaSuccess) return e;
         __atomic_fetch_or(&set, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
     }
     const int HKV = a.c.n_head_kv;
-    e = fbk_launch(k_kv4_attention<E, D, PL>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
+    e = fbk_launch(k_kv4_attention<E, D>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
     if (e != cudaSuccess || !a.part) return e;
     return fbk_launch(k_kv4_join<E, D>, dim3(a.H, T), dim3(D), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
 }
