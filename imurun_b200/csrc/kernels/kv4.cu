@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 // be the larger part of the error; for bf16, whose own step is 8 times as
 // wide, p is rounded first and codes stay 0..15.
 constexpr int kAtWarps = 8, kSlots = 4;
+constexpr float kNoRef = -1e30f;   // before the first key: finite, so that a key outside (-inf) weighs 0 against it
 
 // key of row r of the 16-row operand tiles
 __device__ __forceinline__ int kv4_key(int r) { return (r & 8) | (r & 1 ? 4 + (((r >> 1) & 3) ^ 1) : (r >> 1) & 3); }
@@ -199,10 +200,12 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cas
 template <bool Sub>
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
     if (Sub) {
-        r[0] = (w << 4) & 0x00F000F0u;
+        // the left shifts as products: they run beside the logic
+        const uint32_t u = w >> 8;
+        r[0] = (w * 16u) & 0x00F000F0u;
         r[1] = w & 0x00F000F0u;
-        r[2] = (w >> 4) & 0x00F000F0u;
-        r[3] = (w >> 8) & 0x00F000F0u;
+        r[2] = (u * 16u) & 0x00F000F0u;
+        r[3] = u & 0x00F000F0u;
     } else {
         const __half2 k1024 = bits_h2(0x64006400u), k64 = bits_h2(0x54005400u);
         const uint32_t u = w >> 8;
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         cs[i] = A.scale * reinterpret_cast<const float*>(sm + M::ex)[2 * t + i] * (cap ? 1.0f / A.softcap : kLog2e);
         csc[i] = cs[i] * kCode;
     }
-    float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    float ref[2] = {kNoRef, kNoRef}, sum[2] = {0.0f, 0.0f};
     int top_e = 0;                          // E
     __half2 down_e = __float2half2_rn(0.0f), limit_e = down_e;   // 2^-E, 2^(E + 1); a limit of 0 is passed by the first page
     // O^T 2^-E / kCode: dims 32 e + 4 g + 2 u (accumulators 0, 1) and the next (2, 3), heads 2 t + (0, 1)
@@ -389,179 +392,197 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     const int row = kv4_key(g);   // and row + 8
     const int vrow = kv4_key(2 * t), vrow2 = kv4_key(2 * t + 1), piece = 2 * NG * (g ^ ((vrow & 2) << 1));
     bool ok = true;
-    for (int k = 0; k < n; ++k) {
-        if ((k & 31) == 0 && k) ids = ids_next;
-        if ((k & 31) == 32 - kSlots) ids_next = look_up((k & ~31) + 32);
-        const int page = __shfl_sync(0xffffffffu, ids, k & 31);
-        const int slot = k % kSlots;
-        const uint32_t parity = (uint32_t)(k / kSlots) & 1u;
-        ok = ok && (mbar_try_wait(&bar[slot], parity) || mbar_wait_bounded(&bar[slot], parity));
-        __syncwarp();
-        if (page >= 0) {
-            const uint8_t* rec = ring + slot * R::bytes;
-            // ---- scores of keys row and row + 8 (accumulators 0, 1 and 2, 3), heads 2 t, 2 t + 1
-            float sl[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s[4];
-            {
-                const uint8_t* lo = rec + R::klo + (t & 1) * 4;
-                uint32_t l0 = 0, l1 = 0;
-                if (2 * (t & 1) < GP) {
-                    l0 = *reinterpret_cast<const uint32_t*>(lo + row * GP * 2);
-                    l1 = *reinterpret_cast<const uint32_t*>(lo + (row + 8) * GP * 2);
-                }
-                if (NG == 3 && (t & 1)) l0 &= 0xFFFFu, l1 &= 0xFFFFu;   // the padding
-                mma8(sl, l0, l1, qsb);
-            }
-            uint32_t w0[NG], w1[NG], d0[GP / 2], d1[GP / 2];
-            words<NG>(rec + row * R::row + 4 * NG * t, w0);
-            words<NG>(rec + (row + 8) * R::row + 4 * NG * t, w1);
-            words<GP / 2>(rec + R::kd + row * GP * 2, d0);
-            words<GP / 2>(rec + R::kd + (row + 8) * GP * 2, d1);
+    const int lrow = 4 * (t & 1);
+    const bool lhas = 2 * (t & 1) < GP;
+    const uint32_t lkeep = NG == 3 && (t & 1) ? 0xFFFFu : 0xFFFFFFFFu;   // not the padding
+    // Scores of keys row and row + 8 (accumulators 0, 1 and 2, 3), heads 2 t, 2 t + 1, in two steps: what lo gives,
+    // then group by group. Called for page k + 1 between the groups of page k's values, so that a warp has two
+    // chains of products to go on with.
+    float sl[4], s[4], sn[4] = {};
+    uint32_t w0[NG], w1[NG], d0[GP / 2], d1[GP / 2];
+    auto scores_begin = [&](const uint8_t* rec) {
+        const uint32_t l0 = lhas ? *reinterpret_cast<const uint32_t*>(rec + R::klo + row * GP * 2 + lrow) & lkeep : 0u;
+        const uint32_t l1 = lhas ? *reinterpret_cast<const uint32_t*>(rec + R::klo + (row + 8) * GP * 2 + lrow) & lkeep : 0u;
+        words<NG>(rec + row * R::row + 4 * NG * t, w0);
+        words<NG>(rec + (row + 8) * R::row + 4 * NG * t, w1);
+        words<GP / 2>(rec + R::kd + row * GP * 2, d0);
+        words<GP / 2>(rec + R::kd + (row + 8) * GP * 2, d1);
+        sl[0] = sl[1] = sl[2] = sl[3] = 0.0f;
+        mma8(sl, l0, l1, qsb);
+    };
+    auto scores_group = [&](int e) {
+        uint32_t a[4], b[4];
+        codes8<SUB>(w0[e], a);
+        codes8<SUB>(w1[e], b);
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < NG; ++e) {
-                uint32_t a[4], b[4];
-                codes8<SUB>(w0[e], a);
-                codes8<SUB>(w1[e], b);
-                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int p = 0; p < PL; ++p) {
-                    mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
-                    mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
-                }
-                const float da = e & 1 ? half_at<1>(d0[e / 2]) : half_at<0>(d0[e / 2]);
-                const float db = e & 1 ? half_at<1>(d1[e / 2]) : half_at<0>(d1[e / 2]);
-                s[0] = e ? fmaf(da, x[0], s[0]) : da * x[0];
-                s[1] = e ? fmaf(da, x[1], s[1]) : da * x[1];
-                s[2] = e ? fmaf(db, x[2], s[2]) : db * x[2];
-                s[3] = e ? fmaf(db, x[3], s[3]) : db * x[3];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = fmaf(s[i], csc[i & 1], sl[i] * cs[i & 1]);
-            if (cap) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i] = A.softcap * kLog2e * tanhf(s[i]);
-            }
-            // ---- V scales; at the edges of what the token sees, keys outside have no weight and no scale
-            uint32_t v0[GP / 2], v1[GP / 2], u0[GP / 2], u1[GP / 2];
-            words<GP / 2>(rec + R::vd + row * GP * 2, v0);
-            words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1);
-            words<GP / 2>(rec + R::vlo + row * GP * 2, u0);
-            words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1);
-            if (NG == 3) v0[1] &= 0xFFFFu, v1[1] &= 0xFFFFu;
-            const int kb = (first + k * kAtWarps) * kKv4Page;
-            if (kb + kKv4Page - 1 > pos || kb < key0) {
-                const bool in0 = kb + row <= pos && kb + row >= key0, in1 = kb + row + 8 <= pos && kb + row + 8 >= key0;
-                if (!in0) s[0] = s[1] = -INFINITY;
-                if (!in1) s[2] = s[3] = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < GP / 2; ++e) {
-                    v0[e] = in0 ? v0[e] : 0u;
-                    u0[e] = in0 ? u0[e] : 0u;
-                    v1[e] = in1 ? v1[e] : 0u;
-                    u1[e] = in1 ? u1[e] : 0u;
-                }
-            }
-            // ---- the references, raised when a weight passes 2^14 or a scale 2^(E + 1)
-            __half2 dm = __hmax2(bits_h2(v0[0]), bits_h2(v1[0]));
-#pragma unroll
-            for (int e = 1; e < GP / 2; ++e) dm = __hmax2(dm, __hmax2(bits_h2(v0[e]), bits_h2(v1[e])));
-            const bool wide = !__hble2(dm, limit_e);
-            const bool high = fmaxf(fmaxf(s[0], s[2]) - ref[0], fmaxf(s[1], s[3]) - ref[1]) > 14.0f;
-            if (__any_sync(0xffffffffu, wide || high)) {
-                float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])}, dtop = fmaxf(__low2float(dm), __high2float(dm));
-#pragma unroll
-                for (int w = 4; w <= 16; w <<= 1) {
-                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
-                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
-                    dtop = fmaxf(dtop, __shfl_xor_sync(0xffffffffu, dtop, w));
-                }
-                const int e_new = max((int)(__float_as_uint(fmaxf(dtop, 0.0f)) >> 23) - 127, -15);   // d < 2^(e_new + 1)
-                float f_e = 1.0f;
-                if (limit_e.x == __half(0.0f) || e_new > top_e) {
-                    f_e = limit_e.x == __half(0.0f) ? 1.0f : __int_as_float((127 + top_e - e_new) << 23);
-                    top_e = e_new;
-                    down_e = __float2half2_rn(__int_as_float((127 - e_new) << 23));
-                    limit_e = __float2half2_rn(__int_as_float((128 + e_new) << 23));
-                }
-                float f[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float to = mx[i] - ref[i] > 14.0f ? mx[i] - 8.0f : ref[i];   // from -inf too
-                    f[i] = to == ref[i] ? 1.0f : at_ex2(ref[i] - to);
-                    ref[i] = to;
-                    sum[i] *= f[i];
-                }
-#pragma unroll
-                for (int e = 0; e < NG; ++e) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[e][0][i] *= f[i & 1] * f_e;
-                        o[e][1][i] *= f[i & 1] * f_e;
-                        if (W == W_MID) mid[e][i] *= f[i & 1] * f_e;
-                    }
-                    olo[e][0] *= f[0];
-                    olo[e][1] *= f[1];
-                }
-            }
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = at_ex2(s[i] - ref[i & 1]);
-            sum[0] += p[0] + p[2];
-            sum[1] += p[1] + p[3];
-            const __half2 p0 = __floats2half2_rn(p[0], p[1]), p1 = __floats2half2_rn(p[2], p[3]);
-            // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
-            uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
-            const uint8_t* vr = rec + R::v + piece;
-            halves<NG>(vr + vrow * R::row, va);
-            halves<NG>(vr + vrow2 * R::row, vb);
-            halves<NG>(vr + (vrow + 8) * R::row, vc);
-            halves<NG>(vr + (vrow2 + 8) * R::row, vd);
-#pragma unroll
-            for (int e = 0; e < NG; ++e) {
-                const __half2 n0 = __hmul2(bits_h2(v0[e / 2]), down_e), n1 = __hmul2(bits_h2(v1[e / 2]), down_e);   // d 2^-E
-                float la = e & 1 ? half_at<1>(u0[e / 2]) : half_at<0>(u0[e / 2]);
-                float lb = e & 1 ? half_at<1>(u1[e / 2]) : half_at<0>(u1[e / 2]);
-                if (W == W_MID) {
-                    la = fmaf(8.0f, e & 1 ? half_at<1>(v0[e / 2]) : half_at<0>(v0[e / 2]), la);
-                    lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[e / 2]) : half_at<0>(v1[e / 2]), lb);
-                }
-                olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
-                olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
-                uint32_t ra[4], rc[4];
-                codes8<SUB>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
-                codes8<SUB>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
-                __half2 hi0, hi1;
-                float x[4];
-                if (W == W_HALF) {
-                    hi0 = __hmul2(p0, e & 1 ? __high2half2(n0) : __low2half2(n0));
-                    hi1 = __hmul2(p1, e & 1 ? __high2half2(n1) : __low2half2(n1));
-                } else {
-                    const float da = e & 1 ? __high2float(n0) : __low2float(n0), db = e & 1 ? __high2float(n1) : __low2float(n1);
-                    x[0] = p[0] * da;
-                    x[1] = p[1] * da;
-                    x[2] = p[2] * db;
-                    x[3] = p[3] * db;
-                    hi0 = __floats2half2_rn(x[0], x[1]);
-                    hi1 = __floats2half2_rn(x[2], x[3]);
-                }
-                const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
-#pragma unroll
-                for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
-                if (W == W_MID) mma16(mid[e], 0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u, b0, b1);   // -8
-                if (W == W_PAIR) {
-                    const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
-                    const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x[0] - y0.x, x[1] - y0.y)));
-                    const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x[2] - y1.x, x[3] - y1.y)));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
-                }
-            }
-            __syncwarp();   // the slot is read
+        for (int p = 0; p < PL; ++p) {
+            mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
+            mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
         }
+        const float da = e & 1 ? half_at<1>(d0[e / 2]) : half_at<0>(d0[e / 2]);
+        const float db = e & 1 ? half_at<1>(d1[e / 2]) : half_at<0>(d1[e / 2]);
+        sn[0] = e ? fmaf(da, x[0], sn[0]) : da * x[0];
+        sn[1] = e ? fmaf(da, x[1], sn[1]) : da * x[1];
+        sn[2] = e ? fmaf(db, x[2], sn[2]) : db * x[2];
+        sn[3] = e ? fmaf(db, x[3], sn[3]) : db * x[3];
+    };
+    // log2 units into s; at the edges of what the token sees (and where there is no page) keys outside get -inf and,
+    // by in0 and in1, no scale of V
+    bool edge = false, in0 = true, in1 = true;
+    auto scores_end = [&](int k, int page) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = fmaf(sn[i], csc[i & 1], sl[i] * cs[i & 1]);
+        if (cap) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = A.softcap * kLog2e * tanhf(s[i]);
+        }
+        const int kb = (first + k * kAtWarps) * kKv4Page;
+        edge = kb + kKv4Page - 1 > pos || kb < key0 || page < 0;
+        if (edge) {
+            in0 = page >= 0 && kb + row <= pos && kb + row >= key0;
+            in1 = page >= 0 && kb + row + 8 <= pos && kb + row + 8 >= key0;
+            if (!in0) s[0] = s[1] = -INFINITY;
+            if (!in1) s[2] = s[3] = -INFINITY;
+        }
+    };
+    auto arrived = [&](int k) {
+        const uint32_t parity = (uint32_t)(k / kSlots) & 1u;
+        ok = ok && (mbar_try_wait(&bar[k % kSlots], parity) || mbar_wait_bounded(&bar[k % kSlots], parity));
+        __syncwarp();
+    };
+    if (n > 0) {
+        arrived(0);
+        scores_begin(ring);
+#pragma unroll
+        for (int e = 0; e < NG; ++e) scores_group(e);
+        scores_end(0, __shfl_sync(0xffffffffu, ids, 0));
+    }
+    for (int k = 0; k < n; ++k) {
+        if ((k & 31) == 32 - kSlots) ids_next = look_up((k & ~31) + 32);
+        const int k1 = k + 1, slot1 = k1 % kSlots;
+        const int page1 = __shfl_sync(0xffffffffu, (k1 & 31) ? ids : ids_next, k1 & 31);
+        if (k1 < n) arrived(k1);
+        const uint8_t* rec = ring + (k % kSlots) * R::bytes;
+        uint32_t v0[GP / 2], v1[GP / 2], u0[GP / 2], u1[GP / 2];
+        words<GP / 2>(rec + R::vd + row * GP * 2, v0);
+        words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1);
+        words<GP / 2>(rec + R::vlo + row * GP * 2, u0);
+        words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1);
+        if (NG == 3) v0[1] &= 0xFFFFu, v1[1] &= 0xFFFFu;
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < GP / 2; ++e) {
+                v0[e] = in0 ? v0[e] : 0u;
+                u0[e] = in0 ? u0[e] : 0u;
+                v1[e] = in1 ? v1[e] : 0u;
+                u1[e] = in1 ? u1[e] : 0u;
+            }
+        }
+        // ---- the references, raised when a weight passes 2^14 or a scale 2^(E + 1)
+        __half2 dm = __hmax2(bits_h2(v0[0]), bits_h2(v1[0]));
+#pragma unroll
+        for (int e = 1; e < GP / 2; ++e) dm = __hmax2(dm, __hmax2(bits_h2(v0[e]), bits_h2(v1[e])));
+        const bool wide = !__hble2(dm, limit_e);
+        const bool high = fmaxf(fmaxf(s[0], s[2]) - ref[0], fmaxf(s[1], s[3]) - ref[1]) > 14.0f;
+        if (__any_sync(0xffffffffu, wide || high)) {
+            float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])}, dtop = fmaxf(__low2float(dm), __high2float(dm));
+#pragma unroll
+            for (int w = 4; w <= 16; w <<= 1) {
+                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
+                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
+                dtop = fmaxf(dtop, __shfl_xor_sync(0xffffffffu, dtop, w));
+            }
+            const int e_new = max((int)(__float_as_uint(fmaxf(dtop, 0.0f)) >> 23) - 127, -15);   // d < 2^(e_new + 1)
+            float f_e = 1.0f;
+            if (limit_e.x == __half(0.0f) || e_new > top_e) {
+                f_e = limit_e.x == __half(0.0f) ? 1.0f : __int_as_float((127 + top_e - e_new) << 23);
+                top_e = e_new;
+                down_e = __float2half2_rn(__int_as_float((127 - e_new) << 23));
+                limit_e = __float2half2_rn(__int_as_float((128 + e_new) << 23));
+            }
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float to = mx[i] - ref[i] > 14.0f ? mx[i] - 8.0f : ref[i];
+                f[i] = to == ref[i] ? 1.0f : at_ex2(ref[i] - to);
+                ref[i] = to;
+                sum[i] *= f[i];
+            }
+#pragma unroll
+            for (int e = 0; e < NG; ++e) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[e][0][i] *= f[i & 1] * f_e;
+                    o[e][1][i] *= f[i & 1] * f_e;
+                    if (W == W_MID) mid[e][i] *= f[i & 1] * f_e;
+                }
+                olo[e][0] *= f[0];
+                olo[e][1] *= f[1];
+            }
+        }
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = at_ex2(s[i] - ref[i & 1]);
+        sum[0] += p[0] + p[2];
+        sum[1] += p[1] + p[3];
+        const __half2 p0 = __floats2half2_rn(p[0], p[1]), p1 = __floats2half2_rn(p[2], p[3]);
+        // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
+        uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
+        const uint8_t* vr = rec + R::v + piece;
+        halves<NG>(vr + vrow * R::row, va);
+        halves<NG>(vr + vrow2 * R::row, vb);
+        halves<NG>(vr + (vrow + 8) * R::row, vc);
+        halves<NG>(vr + (vrow2 + 8) * R::row, vd);
+        scores_begin(ring + slot1 * R::bytes);   // of what lies there, past the last page too
+#pragma unroll
+        for (int e = 0; e < NG; ++e) {
+            scores_group(e);
+            const __half2 n0 = __hmul2(bits_h2(v0[e / 2]), down_e), n1 = __hmul2(bits_h2(v1[e / 2]), down_e);   // d 2^-E
+            float la = e & 1 ? half_at<1>(u0[e / 2]) : half_at<0>(u0[e / 2]);
+            float lb = e & 1 ? half_at<1>(u1[e / 2]) : half_at<0>(u1[e / 2]);
+            if (W == W_MID) {
+                la = fmaf(8.0f, e & 1 ? half_at<1>(v0[e / 2]) : half_at<0>(v0[e / 2]), la);
+                lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[e / 2]) : half_at<0>(v1[e / 2]), lb);
+            }
+            olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
+            olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
+            uint32_t ra[4], rc[4];
+            codes8<SUB>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
+            codes8<SUB>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+            __half2 hi0, hi1;
+            float x[4];
+            if (W == W_HALF) {
+                hi0 = __hmul2(p0, e & 1 ? __high2half2(n0) : __low2half2(n0));
+                hi1 = __hmul2(p1, e & 1 ? __high2half2(n1) : __low2half2(n1));
+            } else {
+                const float da = e & 1 ? __high2float(n0) : __low2float(n0), db = e & 1 ? __high2float(n1) : __low2float(n1);
+                x[0] = p[0] * da;
+                x[1] = p[1] * da;
+                x[2] = p[2] * db;
+                x[3] = p[3] * db;
+                hi0 = __floats2half2_rn(x[0], x[1]);
+                hi1 = __floats2half2_rn(x[2], x[3]);
+            }
+            const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
+            if (W == W_MID) mma16(mid[e], 0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u, b0, b1);   // -8
+            if (W == W_PAIR) {
+                const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
+                const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x[0] - y0.x, x[1] - y0.y)));
+                const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x[2] - y1.x, x[3] - y1.y)));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
+            }
+        }
+        scores_end(k1, page1);
+        __syncwarp();   // the slot is read
         if (k + kSlots < n) {
             const int kn = k + kSlots;
-            const int next = __shfl_sync(0xffffffffu, (kn & ~31) == (k & ~31) ? ids : ids_next, kn & 31);
-            issue(kn, next);
+            issue(kn, __shfl_sync(0xffffffffu, (kn & ~31) == (k & ~31) ? ids : ids_next, kn & 31));
         }
+        if ((k1 & 31) == 0) ids = ids_next;
     }
     if (!__all_sync(0xffffffffu, ok) && c.err && lane == 0) atomicExch(c.err, 7);   // a copy did not arrive in time
     // ---- the lanes' sums over keys (those of other g), then the warps
@@ -601,7 +622,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         for (int w = 0; w < kAtWarps; ++w) top = fmaxf(top, ml[w * 8 + h]);
 #pragma unroll
         for (int w = 0; w < kAtWarps; ++w) {
-            const float f = ml[w * 8 + h] == -INFINITY && ml[64 + w * 8 + h] == 0.0f ? 0.0f : at_ex2(ml[w * 8 + h] - top);   // NaN stays
+            const float f = at_ex2(ml[w * 8 + h] - top);
             const float4 y = *reinterpret_cast<const float4*>(so + (w * 8 + h) * (D + 4) + d);
             l = fmaf(f, ml[64 + w * 8 + h], l);
             x.x = fmaf(f, y.x, x.x);
@@ -623,25 +644,67 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
 }
 
 // The splits of one (token, query head) joined: out = sum_s 2^(ref_s - top) O_s / sum_s 2^(ref_s - top) sum_s.
+// Warp w takes the splits w, w + 8, .., a lane D / 32 dimensions; the loads do not wait for the reference.
+constexpr int kJoinWarps = 8;
 template <class E, int D>
-__global__ void __launch_bounds__(D) k_kv4_join(const float* __restrict__ part, int S, int H, int HKV,
-                                                const int32_t* __restrict__ tok_pos, E* out, int64_t ldo) {
+__global__ void __launch_bounds__(32 * kJoinWarps) k_kv4_join(const float* __restrict__ part, int S, int H, int HKV,
+                                                              const int32_t* __restrict__ tok_pos, E* out, int64_t ldo) {
+    constexpr int N = D / 32, U = 5;   // U splits of a warp in flight
     pdl_trigger();
     pdl_wait();
-    const int tok = blockIdx.y, h = blockIdx.x, G = H / HKV, runs = (G + 7) / 8, d = threadIdx.x;
+    const int tok = blockIdx.y, h = blockIdx.x, G = H / HKV, runs = (G + 7) / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (tok_pos[tok] < 0) return;
-    const int hk = h / G, hg = h % G;
-    const float* p = part + (size_t)(tok * HKV * runs + hk * runs + hg / 8) * S * (16 + 8 * D);
-    const int r = hg % 8;
-    float top = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int s = 0; s < S; ++s) top = fmaxf(top, p[(size_t)s * (16 + 8 * D) + r]);
-    for (int s = 0; s < S; ++s) {
-        const float* ps = p + (size_t)s * (16 + 8 * D);
-        const float f = ps[r] == -INFINITY && ps[8 + r] == 0.0f ? 0.0f : at_ex2(ps[r] - top);
-        l = fmaf(f, ps[8 + r], l);
-        o = fmaf(f, ps[16 + r * D + d], o);
+    const int hg = h % G, r = hg % 8;
+    const float* p = part + (size_t)(tok * HKV * runs + h / G * runs + hg / 8) * S * (16 + 8 * D);
+    __shared__ float st[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
+    float top = -INFINITY, l = 0.0f, o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0.0f;
+    for (int s0 = warp; s0 < S; s0 += kJoinWarps * U) {
+        float ref[U], sum[U], x[U][N], up = top;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + u * kJoinWarps;
+            const float* ps = p + (size_t)s * (16 + 8 * D);
+            ref[u] = s < S ? ps[r] : -INFINITY;
+            sum[u] = s < S ? ps[8 + r] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[u][e] = s < S ? ps[16 + r * D + 32 * e + lane] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) up = fmaxf(up, ref[u]);
+        const float f0 = at_ex2(top - up);
+        l *= f0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] *= f0;
+        top = up;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float f = at_ex2(ref[u] - top);
+            l = fmaf(f, sum[u], l);
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = fmaf(f, x[u][e], o[e]);
+        }
     }
-    out[tok * ldo + (int64_t)h * D + d] = from_f32<E>(l != 0.0f ? o / l : 0.0f);
+    if (lane == 0) {
+        st[warp] = top;
+        sl[warp] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) so[warp][32 * e + lane] = o[e];
+    __syncthreads();
+    if (threadIdx.x < D) {
+        top = -INFINITY;
+        l = 0.0f;
+        float y = 0.0f;
+        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, st[w]);
+        for (int w = 0; w < kJoinWarps; ++w) {
+            const float f = at_ex2(st[w] - top);
+            l = fmaf(f, sl[w], l);
+            y = fmaf(f, so[w][threadIdx.x], y);
+        }
+        out[tok * ldo + (int64_t)h * D + threadIdx.x] = from_f32<E>(l != 0.0f ? y / l : 0.0f);
+    }
 }
 
 // ---------------------------------------------------------------- launches
@@ -704,7 +767,7 @@ static cudaError_t launch_kv4_attention(const AtArgs& a, int T, int S, cudaStrea
     const int HKV = a.c.n_head_kv;
     e = fbk_launch(k_kv4_attention<E, D>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
     if (e != cudaSuccess || !a.part) return e;
-    return fbk_launch(k_kv4_join<E, D>, dim3(a.H, T), dim3(D), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
+    return fbk_launch(k_kv4_join<E, D>, dim3(a.H, T), dim3(32 * kJoinWarps), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
 }
 template <class E>
 static cudaError_t kv4_attention_d(const AtArgs& a, int T, int S, cudaStream_t st) {
