@@ -138,9 +138,9 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 // m16n8k16, f16 operands, exact), and scales meet sums, not values.
 //
 // CTA = (a run of the token's pages, kv head, up to 8 of its query heads,
-// token); each of its 8 warps takes every eighth page of the run, one bulk copy
-// a page and kv head (K and V codes and scales lie together, 2560 B at D = 128)
-// into the warp's own ring of kSlots. Per page:
+// token); each of its 8 warps takes every eighth two pages of the run, one bulk
+// copy a page and kv head (K and V codes and scales lie together, 2560 B at D =
+// 128) into the warp's own ring of kSlots. Per page:
 //   S^T[16 keys][8 heads] = K[16][D] Q^T: a k-step of 16 stays inside one
 //     group, and the group's two steps' sums are scaled by d of the row;
 //   O^T[16 dims][8 heads] += V^T P'^T, P' = p d per group, transposed in
@@ -149,11 +149,14 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 //
 // What bounds it is instructions: at the full HBM rate an SM has 111 cycles for
 // a page of 128 dimensions, that is 4096 values. So for 16-bit types a code is
-// moved to bits 4..7 of its half and used as it lies, the f16 subnormal c 2^-20
-// (tensor cores take subnormals as they are). A product's place in the adder
-// goes by the exponent field, so c 2^-20 keeps 6 to 10 bits less than a normal
-// operand would, about 2^-20 of the sum; f32 calls, which want more, take normal
-// operands at two more instructions a word. And no maximum is formed over a
+// masked out of its word and used where it lies: bits 0..3 of a half are the f16
+// subnormal c 2^-24, bits 4..7 are c 2^-20 (tensor cores take subnormals as they
+// are); even dimensions' queries are 16 times as large to even that out, odd
+// dimensions' outputs are 2^4 less. A product's place in the adder goes by the
+// exponent field, so a subnormal keeps up to 10 bits less than a normal operand
+// would: 2^-17 of the sum, against 2^-12 for f16's own rounding. f32 calls,
+// which want more, take normal operands at four more instructions a word. Two
+// pages a step share the waits and checks. And no maximum is formed over a
 // page: the weights' reference is raised only when some lane's weight passes
 // 2^14, the common exponent 2^E of V's scales only when some d passes 2^(E + 1);
 // both rescale what was summed, a few times a context. With p <= 2^14 and
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
 // by one more MMA a group, and lo + 8 d stands for lo), else the rounding would
 // be the larger part of the error; for bf16, whose own step is 8 times as
 // wide, p is rounded first and codes stay 0..15.
-constexpr int kAtWarps = 8, kSlots = 4;
+constexpr int kAtWarps = 8, kSlots = 2;
 constexpr float kNoRef = -1e30f;   // before the first key: finite, so that a key outside (-inf) weighs 0 against it
 
 // key of row r of the 16-row operand tiles
@@ -194,17 +197,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// The 8 codes of w as f16, r[n] = (code n, code n + 4). Sub: as subnormals of
-// 2^-20; else as they are (dropped into the mantissa of 1024 or of 64, which is
-// taken off exactly).
+// The 8 codes of w as f16, r[n] = (code n, code n + 4). Sub: as the subnormals
+// that they are where they lie, 2^-24 for even n and 2^-20 for odd; else as
+// they are (dropped into the mantissa of 1024 or of 64, which is taken off exactly).
 template <bool Sub>
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
     if (Sub) {
-        // the left shifts as products: they run beside the logic
         const uint32_t u = w >> 8;
-        r[0] = (w * 16u) & 0x00F000F0u;
+        r[0] = w & 0x000F000Fu;
         r[1] = w & 0x00F000F0u;
-        r[2] = (u * 16u) & 0x00F000F0u;
+        r[2] = u & 0x000F000Fu;
         r[3] = u & 0x00F000F0u;
     } else {
         const __half2 k1024 = bits_h2(0x64006400u), k64 = bits_h2(0x54005400u);
@@ -259,7 +261,7 @@ struct AtArgs {
 template <int D>
 struct AtSmem {
     using R = Kv4Rec<D>;
-    static constexpr int q = kAtWarps * kSlots * R::bytes;     // f16 queries [2 parts][8][D]
+    static constexpr int q = kAtWarps * kSlots * 2 * R::bytes;     // f16 queries [2 parts][8][D]
     static constexpr int qs = q + 2 * 8 * D * 2;               // sums of a group's queries [2 parts][8][4] f16
     static constexpr int ex = qs + 2 * 8 * 4 * 2;              // the heads' exponents as factors [8]
     static constexpr int bar = ex + 32;
@@ -288,9 +290,9 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     const int tok = blockIdx.z, G = A.H / c.n_head_kv, runs = (G + 7) / 8;
     const int hk = blockIdx.y / runs, g0 = blockIdx.y % runs * 8, gn = min(8, G - g0), S = gridDim.x;
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + M::bar) + warp * kSlots;
-    uint8_t* ring = sm + warp * kSlots * R::bytes;
+    uint8_t* ring = sm + warp * kSlots * 2 * R::bytes;
     pdl_trigger();
-    if (lane < kSlots) mbar_init(&bar[lane], 1);
+    if (lane < kSlots) mbar_init(&bar[lane], 2);
     mbar_fence_init();
     pdl_wait();
     const int pos = A.tok_pos[tok];
@@ -299,27 +301,33 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     const bool known = seq >= 0 && seq < c.n_seqs;
     if (!known && c.err && threadIdx.x == 0) atomicExch(c.err, 6);
 
-    // this warp's pages: first, first + 8, .. below last; lane l holds the page of its l-th (of 32)
+    // this warp's steps of two neighbouring pages: step j has the pages first + 16 j and the next, below last;
+    // lane l holds the page l & 1 of its (l / 2)-th step (of 16)
     const int key0 = A.window > 0 ? max(0, pos - A.window + 1) : 0;
     const int p0 = key0 / kKv4Page, p1 = min(pos / kKv4Page + 1, c.table_stride);
     if (pos / kKv4Page >= c.table_stride && c.err && threadIdx.x == 0) atomicExch(c.err, 6);
     const int per = (max(p1 - p0, 0) + S - 1) / S;
-    const int first = p0 + blockIdx.x * per + warp, last = min(p0 + ((int)blockIdx.x + 1) * per, p1);
-    const int n = known && first < last ? (last - first + kAtWarps - 1) / kAtWarps : 0;
-    auto look_up = [&](int k0) { return k0 + lane < n ? kv4_page(c, seq, first + (k0 + lane) * kAtWarps) : -1; };
+    const int first = p0 + blockIdx.x * per + 2 * warp, last = min(p0 + ((int)blockIdx.x + 1) * per, p1);
+    const int n = known && first < last ? (last - first + 2 * kAtWarps - 1) / (2 * kAtWarps) : 0;
+    auto look_up = [&](int j0) {
+        const int i = first + (j0 + lane / 2) * 2 * kAtWarps + (lane & 1);
+        return j0 + lane / 2 < n && i < last ? kv4_page(c, seq, i) : -1;
+    };
     int ids = look_up(0), ids_next = -1;
     __syncwarp();
-    auto issue = [&](int k, int page) {   // no page: the slot's phase passes empty
-        if (lane == 0) {
+    auto issue = [&](int j, int id) {   // lanes 0 and 1 bring a page each; without one the barrier's phase passes without it
+        const int page = __shfl_sync(0xffffffffu, id, 2 * (j & 15) + (lane & 1));
+        if (lane < 2) {
+            uint64_t* b = &bar[j % kSlots];
             if (page >= 0) {
-                mbar_expect_tx(&bar[k % kSlots], R::bytes);
-                bulk_g2s(ring + (k % kSlots) * R::bytes, kv4_record(c, page, hk, R::bytes), R::bytes, &bar[k % kSlots]);
+                mbar_expect_tx(b, R::bytes);
+                bulk_g2s(ring + ((j % kSlots) * 2 + lane) * R::bytes, kv4_record(c, page, hk, R::bytes), R::bytes, b);
             } else {
-                mbar_arrive(&bar[k % kSlots]);
+                mbar_arrive(b);
             }
         }
     };
-    for (int k = 0; k < kSlots && k < n; ++k) issue(k, __shfl_sync(0xffffffffu, ids, k));
+    for (int j = 0; j < kSlots && j < n; ++j) issue(j, ids);
 
     // the queries: warp w brings head g0 + w to at most 2 in size, as f16 parts
     {
@@ -339,9 +347,10 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
             const float y = x[e] * down;
-            const __half hi = __float2half_rn(y);
+            const float z = SUB && lane % 2 == 0 ? 16.0f * y : y;   // a code of an even dimension is 2^-4 less
+            const __half hi = __float2half_rn(z);
             sq[warp * D + 32 * e + lane] = hi;
-            if (PL == 2) sq[(8 + warp) * D + 32 * e + lane] = __float2half_rn(y - __half2float(hi));
+            if (PL == 2) sq[(8 + warp) * D + 32 * e + lane] = __float2half_rn(z - __half2float(hi));
             const float sum = warp_sum(y);
             if (lane == 0) {
                 const __half h = __float2half_rn(sum);
@@ -395,98 +404,86 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     const int lrow = 4 * (t & 1);
     const bool lhas = 2 * (t & 1) < GP;
     const uint32_t lkeep = NG == 3 && (t & 1) ? 0xFFFFu : 0xFFFFFFFFu;   // not the padding
-    // Scores of keys row and row + 8 (accumulators 0, 1 and 2, 3), heads 2 t, 2 t + 1, in two steps: what lo gives,
-    // then group by group. Called for page k + 1 between the groups of page k's values, so that a warp has two
-    // chains of products to go on with.
-    float sl[4], s[4], sn[4] = {};
-    uint32_t w0[NG], w1[NG], d0[GP / 2], d1[GP / 2];
-    auto scores_begin = [&](const uint8_t* rec) {
-        const uint32_t l0 = lhas ? *reinterpret_cast<const uint32_t*>(rec + R::klo + row * GP * 2 + lrow) & lkeep : 0u;
-        const uint32_t l1 = lhas ? *reinterpret_cast<const uint32_t*>(rec + R::klo + (row + 8) * GP * 2 + lrow) & lkeep : 0u;
-        words<NG>(rec + row * R::row + 4 * NG * t, w0);
-        words<NG>(rec + (row + 8) * R::row + 4 * NG * t, w1);
-        words<GP / 2>(rec + R::kd + row * GP * 2, d0);
-        words<GP / 2>(rec + R::kd + (row + 8) * GP * 2, d1);
-        sl[0] = sl[1] = sl[2] = sl[3] = 0.0f;
-        mma8(sl, l0, l1, qsb);
-    };
-    auto scores_group = [&](int e) {
-        uint32_t a[4], b[4];
-        codes8<SUB>(w0[e], a);
-        codes8<SUB>(w1[e], b);
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < n; ++j) {
+        if ((j & 15) == 16 - kSlots) ids_next = look_up((j & ~15) + 16);
+        const uint32_t parity = (uint32_t)(j / kSlots) & 1u;
+        ok = ok && (mbar_try_wait(&bar[j % kSlots], parity) || mbar_wait_bounded(&bar[j % kSlots], parity));
+        __syncwarp();
+        const uint8_t* rec0 = ring + (j % kSlots) * 2 * R::bytes;
+        // ---- scores of keys row and row + 8 (0, 1 and 2, 3) of both pages, heads 2 t, 2 t + 1, in log2 units
+        float s[2][4];
+        uint32_t v0[2][GP / 2], v1[2][GP / 2], u0[2][GP / 2], u1[2][GP / 2];
 #pragma unroll
-        for (int p = 0; p < PL; ++p) {
-            mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
-            mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
+        for (int h = 0; h < 2; ++h) {
+            const uint8_t* rec = rec0 + h * R::bytes;
+            const uint32_t l0 = lhas ? *reinterpret_cast<const uint32_t*>(rec + R::klo + row * GP * 2 + lrow) & lkeep : 0u;
+            const uint32_t l1 = lhas ? *reinterpret_cast<const uint32_t*>(rec + R::klo + (row + 8) * GP * 2 + lrow) & lkeep : 0u;
+            uint32_t w0[NG], w1[NG], d0[GP / 2], d1[GP / 2];
+            words<NG>(rec + row * R::row + 4 * NG * t, w0);
+            words<NG>(rec + (row + 8) * R::row + 4 * NG * t, w1);
+            words<GP / 2>(rec + R::kd + row * GP * 2, d0);
+            words<GP / 2>(rec + R::kd + (row + 8) * GP * 2, d1);
+            float sl[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma8(sl, l0, l1, qsb);
+#pragma unroll
+            for (int e = 0; e < NG; ++e) {
+                uint32_t a[4], b[4];
+                codes8<SUB>(w0[e], a);
+                codes8<SUB>(w1[e], b);
+                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = 0; p < PL; ++p) {
+                    mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
+                    mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
+                }
+                const float da = e & 1 ? half_at<1>(d0[e / 2]) : half_at<0>(d0[e / 2]);
+                const float db = e & 1 ? half_at<1>(d1[e / 2]) : half_at<0>(d1[e / 2]);
+                s[h][0] = e ? fmaf(da, x[0], s[h][0]) : da * x[0];
+                s[h][1] = e ? fmaf(da, x[1], s[h][1]) : da * x[1];
+                s[h][2] = e ? fmaf(db, x[2], s[h][2]) : db * x[2];
+                s[h][3] = e ? fmaf(db, x[3], s[h][3]) : db * x[3];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[h][i] = fmaf(s[h][i], csc[i & 1], sl[i] * cs[i & 1]);
+            words<GP / 2>(rec + R::vd + row * GP * 2, v0[h]);
+            words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1[h]);
+            words<GP / 2>(rec + R::vlo + row * GP * 2, u0[h]);
+            words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1[h]);
+            if (NG == 3) v0[h][1] &= 0xFFFFu, v1[h][1] &= 0xFFFFu;
         }
-        const float da = e & 1 ? half_at<1>(d0[e / 2]) : half_at<0>(d0[e / 2]);
-        const float db = e & 1 ? half_at<1>(d1[e / 2]) : half_at<0>(d1[e / 2]);
-        sn[0] = e ? fmaf(da, x[0], sn[0]) : da * x[0];
-        sn[1] = e ? fmaf(da, x[1], sn[1]) : da * x[1];
-        sn[2] = e ? fmaf(db, x[2], sn[2]) : db * x[2];
-        sn[3] = e ? fmaf(db, x[3], sn[3]) : db * x[3];
-    };
-    // log2 units into s; at the edges of what the token sees (and where there is no page) keys outside get -inf and,
-    // by in0 and in1, no scale of V
-    bool edge = false, in0 = true, in1 = true;
-    auto scores_end = [&](int k, int page) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = fmaf(sn[i], csc[i & 1], sl[i] * cs[i & 1]);
         if (cap) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = A.softcap * kLog2e * tanhf(s[i]);
+            for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = A.softcap * kLog2e * tanhf(s[i / 4][i % 4]);
         }
-        const int kb = (first + k * kAtWarps) * kKv4Page;
-        edge = kb + kKv4Page - 1 > pos || kb < key0 || page < 0;
-        if (edge) {
-            in0 = page >= 0 && kb + row <= pos && kb + row >= key0;
-            in1 = page >= 0 && kb + row + 8 <= pos && kb + row + 8 >= key0;
-            if (!in0) s[0] = s[1] = -INFINITY;
-            if (!in1) s[2] = s[3] = -INFINITY;
-        }
-    };
-    auto arrived = [&](int k) {
-        const uint32_t parity = (uint32_t)(k / kSlots) & 1u;
-        ok = ok && (mbar_try_wait(&bar[k % kSlots], parity) || mbar_wait_bounded(&bar[k % kSlots], parity));
-        __syncwarp();
-    };
-    if (n > 0) {
-        arrived(0);
-        scores_begin(ring);
+        // ---- at the edges of what the token sees, and where there is no page: keys outside have no weight and no scale
+        const int i0 = first + j * 2 * kAtWarps, kb = i0 * kKv4Page;
+        const unsigned here = __ballot_sync(0xffffffffu, ids >= 0) >> (2 * (j & 15));
+        if (kb + 2 * kKv4Page - 1 > pos || kb < key0 || (here & 3) != 3) {
 #pragma unroll
-        for (int e = 0; e < NG; ++e) scores_group(e);
-        scores_end(0, __shfl_sync(0xffffffffu, ids, 0));
-    }
-    for (int k = 0; k < n; ++k) {
-        if ((k & 31) == 32 - kSlots) ids_next = look_up((k & ~31) + 32);
-        const int k1 = k + 1, slot1 = k1 % kSlots;
-        const int page1 = __shfl_sync(0xffffffffu, (k1 & 31) ? ids : ids_next, k1 & 31);
-        if (k1 < n) arrived(k1);
-        const uint8_t* rec = ring + (k % kSlots) * R::bytes;
-        uint32_t v0[GP / 2], v1[GP / 2], u0[GP / 2], u1[GP / 2];
-        words<GP / 2>(rec + R::vd + row * GP * 2, v0);
-        words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1);
-        words<GP / 2>(rec + R::vlo + row * GP * 2, u0);
-        words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1);
-        if (NG == 3) v0[1] &= 0xFFFFu, v1[1] &= 0xFFFFu;
-        if (edge) {
+            for (int h = 0; h < 2; ++h) {
+                const int key = kb + h * kKv4Page + row;
+                const bool page = here >> h & 1, in0 = page && key <= pos && key >= key0, in1 = page && key + 8 <= pos && key + 8 >= key0;
+                if (!in0) s[h][0] = s[h][1] = -INFINITY;
+                if (!in1) s[h][2] = s[h][3] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < GP / 2; ++e) {
-                v0[e] = in0 ? v0[e] : 0u;
-                u0[e] = in0 ? u0[e] : 0u;
-                v1[e] = in1 ? v1[e] : 0u;
-                u1[e] = in1 ? u1[e] : 0u;
+                for (int e = 0; e < GP / 2; ++e) {
+                    v0[h][e] = in0 ? v0[h][e] : 0u;
+                    u0[h][e] = in0 ? u0[h][e] : 0u;
+                    v1[h][e] = in1 ? v1[h][e] : 0u;
+                    u1[h][e] = in1 ? u1[h][e] : 0u;
+                }
             }
         }
         // ---- the references, raised when a weight passes 2^14 or a scale 2^(E + 1)
-        __half2 dm = __hmax2(bits_h2(v0[0]), bits_h2(v1[0]));
+        __half2 dm = __hmax2(__hmax2(bits_h2(v0[0][0]), bits_h2(v1[0][0])), __hmax2(bits_h2(v0[1][0]), bits_h2(v1[1][0])));
 #pragma unroll
-        for (int e = 1; e < GP / 2; ++e) dm = __hmax2(dm, __hmax2(bits_h2(v0[e]), bits_h2(v1[e])));
-        const bool wide = !__hble2(dm, limit_e);
-        const bool high = fmaxf(fmaxf(s[0], s[2]) - ref[0], fmaxf(s[1], s[3]) - ref[1]) > 14.0f;
+        for (int e = 1; e < GP / 2; ++e)
+            dm = __hmax2(dm, __hmax2(__hmax2(bits_h2(v0[0][e]), bits_h2(v1[0][e])), __hmax2(bits_h2(v0[1][e]), bits_h2(v1[1][e]))));
+        const float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+        const float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+        const bool wide = !__hble2(dm, limit_e), high = fmaxf(mx0 - ref[0], mx1 - ref[1]) > 14.0f;
         if (__any_sync(0xffffffffu, wide || high)) {
-            float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])}, dtop = fmaxf(__low2float(dm), __high2float(dm));
+            float mx[2] = {mx0, mx1}, dtop = fmaxf(__low2float(dm), __high2float(dm));
 #pragma unroll
             for (int w = 4; w <= 16; w <<= 1) {
                 mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
@@ -521,68 +518,65 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 olo[e][1] *= f[1];
             }
         }
-        float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = at_ex2(s[i] - ref[i & 1]);
-        sum[0] += p[0] + p[2];
-        sum[1] += p[1] + p[3];
-        const __half2 p0 = __floats2half2_rn(p[0], p[1]), p1 = __floats2half2_rn(p[2], p[3]);
-        // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
-        uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
-        const uint8_t* vr = rec + R::v + piece;
-        halves<NG>(vr + vrow * R::row, va);
-        halves<NG>(vr + vrow2 * R::row, vb);
-        halves<NG>(vr + (vrow + 8) * R::row, vc);
-        halves<NG>(vr + (vrow2 + 8) * R::row, vd);
-        scores_begin(ring + slot1 * R::bytes);   // of what lies there, past the last page too
+        for (int h = 0; h < 2; ++h) {
+            float p[4];
 #pragma unroll
-        for (int e = 0; e < NG; ++e) {
-            scores_group(e);
-            const __half2 n0 = __hmul2(bits_h2(v0[e / 2]), down_e), n1 = __hmul2(bits_h2(v1[e / 2]), down_e);   // d 2^-E
-            float la = e & 1 ? half_at<1>(u0[e / 2]) : half_at<0>(u0[e / 2]);
-            float lb = e & 1 ? half_at<1>(u1[e / 2]) : half_at<0>(u1[e / 2]);
-            if (W == W_MID) {
-                la = fmaf(8.0f, e & 1 ? half_at<1>(v0[e / 2]) : half_at<0>(v0[e / 2]), la);
-                lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[e / 2]) : half_at<0>(v1[e / 2]), lb);
-            }
-            olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
-            olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
-            uint32_t ra[4], rc[4];
-            codes8<SUB>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
-            codes8<SUB>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
-            __half2 hi0, hi1;
-            float x[4];
-            if (W == W_HALF) {
-                hi0 = __hmul2(p0, e & 1 ? __high2half2(n0) : __low2half2(n0));
-                hi1 = __hmul2(p1, e & 1 ? __high2half2(n1) : __low2half2(n1));
-            } else {
-                const float da = e & 1 ? __high2float(n0) : __low2float(n0), db = e & 1 ? __high2float(n1) : __low2float(n1);
-                x[0] = p[0] * da;
-                x[1] = p[1] * da;
-                x[2] = p[2] * db;
-                x[3] = p[3] * db;
-                hi0 = __floats2half2_rn(x[0], x[1]);
-                hi1 = __floats2half2_rn(x[2], x[3]);
-            }
-            const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
+            for (int i = 0; i < 4; ++i) p[i] = at_ex2(s[h][i] - ref[i & 1]);
+            sum[0] += p[0] + p[2];
+            sum[1] += p[1] + p[3];
+            const __half2 p0 = __floats2half2_rn(p[0], p[1]), p1 = __floats2half2_rn(p[2], p[3]);
+            // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
+            uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
+            const uint8_t* vr = rec0 + h * R::bytes + R::v + piece;
+            halves<NG>(vr + vrow * R::row, va);
+            halves<NG>(vr + vrow2 * R::row, vb);
+            halves<NG>(vr + (vrow + 8) * R::row, vc);
+            halves<NG>(vr + (vrow2 + 8) * R::row, vd);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
-            if (W == W_MID) mma16(mid[e], 0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u, b0, b1);   // -8
-            if (W == W_PAIR) {
-                const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
-                const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x[0] - y0.x, x[1] - y0.y)));
-                const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x[2] - y1.x, x[3] - y1.y)));
+            for (int e = 0; e < NG; ++e) {
+                const __half2 n0 = __hmul2(bits_h2(v0[h][e / 2]), down_e), n1 = __hmul2(bits_h2(v1[h][e / 2]), down_e);   // d 2^-E
+                float la = e & 1 ? half_at<1>(u0[h][e / 2]) : half_at<0>(u0[h][e / 2]);
+                float lb = e & 1 ? half_at<1>(u1[h][e / 2]) : half_at<0>(u1[h][e / 2]);
+                if (W == W_MID) {
+                    la = fmaf(8.0f, e & 1 ? half_at<1>(v0[h][e / 2]) : half_at<0>(v0[h][e / 2]), la);
+                    lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[h][e / 2]) : half_at<0>(v1[h][e / 2]), lb);
+                }
+                olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
+                olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
+                uint32_t ra[4], rc[4];
+                codes8<SUB>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
+                codes8<SUB>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+                __half2 hi0, hi1;
+                float x[4];
+                if (W == W_HALF) {
+                    hi0 = __hmul2(p0, e & 1 ? __high2half2(n0) : __low2half2(n0));
+                    hi1 = __hmul2(p1, e & 1 ? __high2half2(n1) : __low2half2(n1));
+                } else {
+                    const float da = e & 1 ? __high2float(n0) : __low2float(n0), db = e & 1 ? __high2float(n1) : __low2float(n1);
+                    x[0] = p[0] * da;
+                    x[1] = p[1] * da;
+                    x[2] = p[2] * db;
+                    x[3] = p[3] * db;
+                    hi0 = __floats2half2_rn(x[0], x[1]);
+                    hi1 = __floats2half2_rn(x[2], x[3]);
+                }
+                const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
 #pragma unroll
-                for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
+                for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
+                if (W == W_MID) mma16(mid[e], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);   // -8, even and odd dims
+                if (W == W_PAIR) {
+                    const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
+                    const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x[0] - y0.x, x[1] - y0.y)));
+                    const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x[2] - y1.x, x[3] - y1.y)));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
+                }
             }
         }
-        scores_end(k1, page1);
         __syncwarp();   // the slot is read
-        if (k + kSlots < n) {
-            const int kn = k + kSlots;
-            issue(kn, __shfl_sync(0xffffffffu, (kn & ~31) == (k & ~31) ? ids : ids_next, kn & 31));
-        }
-        if ((k1 & 31) == 0) ids = ids_next;
+        if (j + kSlots < n) issue(j + kSlots, ((j + kSlots) & ~15) == (j & ~15) ? ids : ids_next);
+        if ((j & 15) == 15) ids = ids_next;
     }
     if (!__all_sync(0xffffffffu, ok) && c.err && lane == 0) atomicExch(c.err, 7);   // a copy did not arrive in time
     // ---- the lanes' sums over keys (those of other g), then the warps
@@ -607,9 +601,10 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         }
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
-            const float up = __int_as_float((127 + top_e) << 23) * kCode, l = olo[e][i] + (W == W_MID ? up * mid[e][i] : 0.0f);
+            const float up = __int_as_float((127 + top_e) << 23) * kCode, ev = SUB ? 16.0f * up : up;   // odd and even dimensions
+            const float lo = olo[e][i] + (W == W_MID ? ev * mid[e][i] : 0.0f), lo1 = olo[e][i] + (W == W_MID ? up * mid[e][2 + i] : 0.0f);
             *reinterpret_cast<float4*>(so + (warp * 8 + h) * (D + 4) + 32 * e + 4 * g) =
-                make_float4(fmaf(up, o[e][0][i], l), fmaf(up, o[e][0][2 + i], l), fmaf(up, o[e][1][i], l), fmaf(up, o[e][1][2 + i], l));
+                make_float4(fmaf(ev, o[e][0][i], lo), fmaf(up, o[e][0][2 + i], lo1), fmaf(ev, o[e][1][i], lo), fmaf(up, o[e][1][2 + i], lo1));
         }
     }
     __syncthreads();
@@ -745,11 +740,11 @@ static cudaError_t append_o(const AppendArgs& a, int out_type, cudaStream_t st) 
          : out_type == T_F16 ? append_d<E, __half>(a, st) : append_d<E, __nv_bfloat16>(a, st);
 }
 
-// CTAs a token and kv head: as many as two an SM give, each warp of them with a page or more
+// CTAs a token and kv head: as many as two an SM give, each warp of them with a step or more
 static int at_splits(int T, int H, int HKV, int max_keys) {
     const int64_t pairs = (int64_t)T * HKV * ((H / HKV + 7) / 8);
     const int pages = (max_keys - 1) / kKv4Page + 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * 148 / pairs, (pages + kAtWarps - 1) / kAtWarps));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * 148 / pairs, (pages + 2 * kAtWarps - 1) / (2 * kAtWarps)));
 }
 
 template <class E, int D>
