@@ -23,9 +23,10 @@ bool stride_ok(int64_t ld, int64_t width, int type) {
     return ld >= width && ld <= ((int64_t)1 << 40) && (ld * (int64_t)type_bytes(type)) % 16 == 0;
 }
 
-// Every pointer is memory that the current device can use as its own: a host
-// array or another GPU's buffer would fault in the kernel. 0, -1 or a CUDA
-// error.
+// A buffer is memory that the current device can use as its own: a host array
+// or another GPU's buffer would fault in the kernel. 0, -1 or a CUDA error. A
+// look at a pointer takes 0.2 us, so of buffers that come in pairs (k and v, cos
+// and sin) one is looked at.
 int on_device(std::initializer_list<const void*> ps) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -76,7 +77,7 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* c, int type, const void* q, con
     if (q && q == q_out && (type != out_type || ldq != ldq_out)) return -1;
     if ((k == k_out || v == v_out) && (type != out_type || ldkv != ldkv_out)) return -1;
     if (T == 0) return 0;
-    const int rc = on_device({c->pool, c->page_table, c->err, q, k, v, tok_seq, tok_pos, rope_cos, rope_sin, q_out, k_out, v_out});
+    const int rc = on_device({c->pool, c->page_table, q, k, tok_pos, rope_cos, q_out, k_out});
     if (rc) return rc;
     return fbk_kv4_append(*c, type, q, k, v, ldq, ldkv, T, H, tok_seq, tok_pos, rot, neox ? 1 : 0, rope_cos, rope_sin, n_rope,
                           out_type, q_out, ldq_out, k_out, v_out, ldkv_out, static_cast<cudaStream_t>(stream));
@@ -98,7 +99,7 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* c, int type, const void* q, 
     if (T == 0) return 0;
     const size_t need = fbk_kv4_attention_workspace(T, H, HKV, D, max_keys);
     if (need && (!workspace || workspace_bytes < need)) return -1;
-    const int rc = on_device({c->pool, c->page_table, c->err, q, tok_seq, tok_pos, out, need ? workspace : nullptr});
+    const int rc = on_device({c->pool, c->page_table, q, tok_pos, out, need ? workspace : nullptr});
     if (rc) return rc;
     return fbk_kv4_attention(*c, type, q, ldq, T, H, tok_seq, tok_pos, max_keys, scale, softcap, window, out, ldo, workspace,
                              static_cast<cudaStream_t>(stream));
@@ -117,7 +118,7 @@ FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const vo
         return -1;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return -1;
     if (n_rows == 0) return 0;
-    const int rc = on_device({q, k, v, cu_seqlens, out});
+    const int rc = on_device({q, k, cu_seqlens, out});
     if (rc) return rc;
     return fbk_attention_packed(type, q, ldq, k, v, ldkv, n_rows, cu_seqlens, n_seqs, H, HKV, D, scale, softcap, window, out,
                                 ldo, static_cast<cudaStream_t>(stream));

@@ -452,7 +452,7 @@ cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void*
     pk::Args a{cu, B, n_rows, HKV, G, R, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
                window, out, ldo, v, ldkv};
     const int64_t tiles = n_rows / (2 * R) + std::min<int64_t>(B, n_rows);
-    return fbk_launch(k_attention_packed<E, D, CAP>, dim3((unsigned)(tiles * HKV)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
+    return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)(tiles * HKV)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
                       km, vm, a);
 }
 

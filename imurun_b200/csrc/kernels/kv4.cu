@@ -725,7 +725,7 @@ static cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
     const int threads = D == 96 ? 192 : 256, per = threads / (D / 8);
     // few tokens: a CTA a run of heads; many: a token's heads in one CTA
     const int hpc = a.T >= 148 ? heads : per;
-    return fbk_launch(k_kv4_append<E, O, D>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(threads), 0, st, a.c,
+    return fbk_launch_early(k_kv4_append<E, O, D>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(threads), 0, st, a.c,
                       (const E*)a.q, (const E*)a.k, (const E*)a.v, a.ldq, a.ldkv, H, hpc, a.tok_seq, a.tok_pos, a.rot,
                       a.neox, a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
 }
@@ -760,9 +760,9 @@ static cudaError_t launch_kv4_attention(const AtArgs& a, int T, int S, cudaStrea
         __atomic_fetch_or(&set, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
     }
     const int HKV = a.c.n_head_kv;
-    e = fbk_launch(k_kv4_attention<E, D>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
+    e = fbk_launch_early(k_kv4_attention<E, D>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
     if (e != cudaSuccess || !a.part) return e;
-    return fbk_launch(k_kv4_join<E, D>, dim3(a.H, T), dim3(32 * kJoinWarps), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
+    return fbk_launch_early(k_kv4_join<E, D>, dim3(a.H, T), dim3(32 * kJoinWarps), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
 }
 template <class E>
 static cudaError_t kv4_attention_d(const AtArgs& a, int T, int S, cudaStream_t st) {

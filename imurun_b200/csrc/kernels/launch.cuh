@@ -9,6 +9,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <utility>
 
 #include "kernels.h"
@@ -28,5 +29,25 @@ static inline cudaError_t fbk_launch(void (*kern)(KArgs...), dim3 grid, dim3 blo
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// The same, with programmatic dependent launch also where no engine has turned
+// it on (entry points on device buffers; FISH_NO_PDL=1 turns it off). The
+// kernel keeps the rule above whatever runs before it on the stream.
+template <class... KArgs, class... Args>
+static inline cudaError_t fbk_launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                           Args&&... args) {
+    static const bool off = getenv("FISH_NO_PDL") && atoi(getenv("FISH_NO_PDL"));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = off ? 0 : 1;
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
