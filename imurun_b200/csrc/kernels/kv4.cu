@@ -261,8 +261,9 @@ struct AtArgs {
 template <int D>
 struct AtSmem {
     using R = Kv4Rec<D>;
-    static constexpr int q = kAtWarps * kSlots * 2 * R::bytes;     // f16 queries [2 parts][8][D]
-    static constexpr int qs = q + 2 * 8 * D * 2;               // sums of a group's queries [2 parts][8][4] f16
+    static constexpr int q = kAtWarps * kSlots * 2 * R::bytes;   // f16 queries [2 parts][8][q_row]
+    static constexpr int q_row = D + 8;
+    static constexpr int qs = q + 2 * 8 * q_row * 2;             // sums of a group's queries [2 parts][8][4] f16
     static constexpr int ex = qs + 2 * 8 * 4 * 2;              // the heads' exponents as factors [8]
     static constexpr int bar = ex + 32;
     static constexpr int bytes = bar + 8 * kAtWarps * kSlots;
@@ -329,12 +330,14 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     };
     for (int j = 0; j < kSlots && j < n; ++j) issue(j, ids);
 
-    // the queries: warp w brings head g0 + w to at most 2 in size, as f16 parts
-    {
+    // the queries: a warp brings head g0 + w to at most 2 in size, as f16 parts, dimensions 32 e + 8 t + n in the order
+    // (0, 4), (1, 5), (2, 6), (3, 7) of n that a lane's operands have
+    constexpr int QS = AtSmem<D>::q_row;
+    for (int w = warp; w < 8; w += kAtWarps) {
         float x[NG], top = 0.0f;
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
-            x[e] = warp < gn ? to_f32<E>(static_cast<const E*>(A.q)[tok * A.ldq + (int64_t)(hk * G + g0 + warp) * D + 32 * e + lane]) : 0.0f;
+            x[e] = w < gn ? to_f32<E>(static_cast<const E*>(A.q)[tok * A.ldq + (int64_t)(hk * G + g0 + w) * D + 32 * e + lane]) : 0.0f;
             top = fmaxf(top, fabsf(x[e]));
         }
         top = warp_max(top);
@@ -342,38 +345,34 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         if (ex == 128 || top == 0.0f) ex = 0;
         ex = min(max(ex, -120), 120);
         const float down = __int_as_float((127 - ex) << 23);
-        __half* sq = reinterpret_cast<__half*>(sm + M::q);
+        __half* sq = reinterpret_cast<__half*>(sm + M::q) + w * QS + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
         __half* ss = reinterpret_cast<__half*>(sm + M::qs);
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
             const float y = x[e] * down;
             const float z = SUB && lane % 2 == 0 ? 16.0f * y : y;   // a code of an even dimension is 2^-4 less
             const __half hi = __float2half_rn(z);
-            sq[warp * D + 32 * e + lane] = hi;
-            if (PL == 2) sq[(8 + warp) * D + 32 * e + lane] = __float2half_rn(z - __half2float(hi));
+            sq[32 * e] = hi;
+            if (PL == 2) sq[8 * QS + 32 * e] = __float2half_rn(z - __half2float(hi));
             const float sum = warp_sum(y);
             if (lane == 0) {
                 const __half h = __float2half_rn(sum);
-                ss[warp * 4 + e] = h;
-                ss[32 + warp * 4 + e] = __float2half_rn(sum - __half2float(h));
+                ss[w * 4 + e] = h;
+                ss[32 + w * 4 + e] = __float2half_rn(sum - __half2float(h));
             }
         }
         if (lane == 0) {
-            for (int e = NG; e < 4; ++e) ss[warp * 4 + e] = ss[32 + warp * 4 + e] = __float2half_rn(0.0f);
-            reinterpret_cast<float*>(sm + M::ex)[warp] = __int_as_float((127 + ex) << 23);
+            for (int e = NG; e < 4; ++e) ss[w * 4 + e] = ss[32 + w * 4 + e] = __float2half_rn(0.0f);
+            reinterpret_cast<float*>(sm + M::ex)[w] = __int_as_float((127 + ex) << 23);
         }
     }
     __syncthreads();
-    // B operands of the scores: head g, dimensions 32 e + 8 t + (0, 4), (1, 5), (2, 6), (3, 7)
+    // B operands of the scores
     uint32_t qb[PL][NG][4];
 #pragma unroll
     for (int p = 0; p < PL; ++p)
 #pragma unroll
-        for (int e = 0; e < NG; ++e) {
-            const __half* s = reinterpret_cast<const __half*>(sm + M::q) + (8 * p + g) * D + 32 * e + 8 * t;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qb[p][e][i] = h2_bits(__halves2half2(s[i], s[i + 4]));
-        }
+        for (int e = 0; e < NG; ++e) words<4>(sm + M::q + ((8 * p + g) * QS + 32 * e + 8 * t) * 2, qb[p][e]);
     // and of sum_g lo sum(q_g): the sums' high parts against k = 0..3, their low parts against k = 4..7
     const uint32_t qsb = *reinterpret_cast<const uint32_t*>(sm + M::qs + (t >> 1) * 64 + g * 8 + (t & 1) * 4);
     constexpr float kLog2e = 1.4426950408889634f;
@@ -597,7 +596,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         const int h = 2 * t + i;
         if (g == 0) {
             ml[warp * 8 + h] = ref[i];
-            ml[64 + warp * 8 + h] = sum[i];
+            ml[8 * kAtWarps + warp * 8 + h] = sum[i];
         }
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
@@ -619,7 +618,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         for (int w = 0; w < kAtWarps; ++w) {
             const float f = at_ex2(ml[w * 8 + h] - top);
             const float4 y = *reinterpret_cast<const float4*>(so + (w * 8 + h) * (D + 4) + d);
-            l = fmaf(f, ml[64 + w * 8 + h], l);
+            l = fmaf(f, ml[8 * kAtWarps + w * 8 + h], l);
             x.x = fmaf(f, y.x, x.x);
             x.y = fmaf(f, y.y, x.y);
             x.z = fmaf(f, y.z, x.z);
