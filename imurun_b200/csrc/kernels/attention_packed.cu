@@ -37,7 +37,7 @@ constexpr int kHalf = 128 * 128;         // 128 rows x 64 values of 16 bits: one
 constexpr int kSoft = 256, kThreads = kSoft + 64;
 constexpr float kRaise = 8.0f;
 
-enum { B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + NS, B_S = B_EMPTY + NS, B_P = B_S + 2, B_O = B_P + 2, B_DRAIN = B_O + 2,
+enum { B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + NS, B_S = B_EMPTY + NS, B_P = B_S + 2, B_O = B_P + 4, B_DRAIN = B_O + 2,
        B_COUNT = B_DRAIN + 1 };
 
 template <int D>
@@ -89,6 +89,22 @@ __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two f32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+          "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
 }
 template <class E> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
@@ -157,7 +173,8 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bar[B_S + x], 1);
-            mbar_init(&bar[B_P + x], 128);
+            mbar_init(&bar[B_P + 2 * x], 128);
+            mbar_init(&bar[B_P + 2 * x + 1], 128);
             mbar_init(&bar[B_O + x], 1);
         }
         mbar_init(&bar[B_DRAIN], 1);
@@ -237,14 +254,17 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                 ok = ok && full(iv);
                 for (int x = 0; x < 2 && ok; ++x) {
                     if (active(x, j)) {
-                        ok = mbar_wait(&bar[B_P + x], (uint32_t)(n[x] & 1), s_abort);
-                        if (!ok) break;
-                        tc_fence_after();
                         const uint64_t b = v0 + stage(iv);
+                        for (int h = 0; h < 2 && ok; ++h) {   // 64 keys as soon as their weights are there
+                            ok = mbar_wait(&bar[B_P + 2 * x + h], (uint32_t)(n[x] & 1), s_abort);
+                            if (!ok) break;
+                            tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < BK / 16; ++k)
-                            umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, b + (uint64_t)(k * 16 * 128 >> 4), kDescO,
-                                        n[x] > 0 || k > 0);
+                            for (int k = 4 * h; k < 4 * h + 4; ++k)
+                                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, b + (uint64_t)(k * 16 * 128 >> 4), kDescO,
+                                            n[x] > 0 || k > 0);
+                        }
+                        if (!ok) break;
                         ++n[x];
                         if (j + 1 == end[x]) umma_commit(&bar[B_O + x]);
                     }
@@ -315,11 +335,14 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     for (int e = 0; e < 32; ++e)
                         if (32 * c + e > top || 32 * c + e <= bottom) s[c][e] = -INFINITY;
             }
-            float mx = -INFINITY;
+            float mm[8];   // eight chains of three-operand maxima
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int e = 0; e < 8; ++e) mm[e] = fmaxf(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1]);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[c][e]);
+            for (int u = 2; u < 16; u += 2)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mm[e] = fmaxf(fmaxf(mm[e], s[e / 2][16 * (e % 2) + u]), s[e / 2][16 * (e % 2) + u + 1]);
+            const float mx = fmaxf(fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])), fmaxf(fmaxf(mm[4], mm[5]), fmaxf(mm[6], mm[7])));
             if (j == first[x]) {
                 m = mx;
             } else {
@@ -340,21 +363,27 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     }
                 }
             }
-            const float mc = m == -INFINITY ? 0.0f : m * A.c;
+            const float2 c2 = make_float2(A.c, A.c), mc2 = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m * A.c, -m * A.c);
+            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t u[16];
+            for (int h = 0; h < 2; ++h) {
+                uint32_t u[32];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float a = ex2(fmaf(s[c][2 * e], A.c, -mc)), b = ex2(fmaf(s[c][2 * e + 1], A.c, -mc));
-                    l += a + b;
-                    u[e] = pack2<E>(a, b);
+                for (int e = 0; e < 32; ++e) {
+                    float2 y = fma2(make_float2(s[2 * h + e / 16][2 * e % 32], s[2 * h + e / 16][2 * e % 32 + 1]), c2, mc2);
+                    y.x = ex2(y.x);
+                    y.y = ex2(y.y);
+                    if (e & 1) sum1 = add2(sum1, y);
+                    else sum0 = add2(sum0, y);
+                    u[e] = pack2<E>(y.x, y.y);
                 }
-                tmem_st16(ts + 16 * c, u);
+                tmem_st32(ts + 32 * h, u);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&bar[B_P + 2 * x + h]);
             }
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&bar[B_P + x]);
+            sum0 = add2(sum0, sum1);
+            l += sum0.x + sum0.y;
         }
         if (ok && end[x]) {
             ok = mbar_wait(&bar[B_O + x], 0, s_abort);
