@@ -6,8 +6,11 @@
 //
 // A tile is 128 MMA rows: R = 128 / G consecutive rows of one sequence times the
 // G query heads of one kv head, so grouped heads share a tile whatever G is and
-// short prompts still fill it. A CTA takes two neighbouring tiles (2 R rows),
-// which share every key and value tile that it loads. Warps:
+// short prompts still fill it. A job is two neighbouring tiles (2 R rows), which
+// share every key and value tile. A CTA an SM takes jobs blockIdx, blockIdx +
+// gridDim, ..; every role goes from one job to the next by itself, so loads and
+// scores of the next job run under the last weights and the output of this one.
+// Warps:
 //   0..3, 4..7  softmax of tile 0 and 1, a thread a row: scores from tensor
 //               memory, mask, row maximum, weights in 16 bits back over the
 //               scores' columns; at the end the rows of out;
@@ -15,7 +18,11 @@
 //               O_x += P_x V_j with P_x from tensor memory. While one tile's
 //               warps form weights, the tensor core works for the other:
 //               S0 S1 | O0 S0 O1 S1 | O0 S0 O1 S1 ..
-//   9           TMA: Q once, then K and V tiles of 128 rows through a ring.
+//   9           TMA: Q, then K and V tiles of 128 rows through a ring;
+//   10, 11      tiles of V in which some row does not see some key: values that
+//               are not finite are taken out before the product (0 x inf is
+//               NaN) and the job is marked; rows that do see them add them at
+//               the end.
 // Tensor memory: S0 S1 (128 columns each, P in their first 64) O0 O1.
 //
 // The reference m_i is raised only when a tile's maximum exceeds it by 2^8 (the
@@ -23,6 +30,8 @@
 // rescaled a few times a row, not once a tile.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+#include <climits>
 #include <mutex>
 
 #include "kv4.cuh"
@@ -34,11 +43,11 @@ namespace pk {
 
 constexpr int BK = 128, NS = 4;          // keys a tile, ring stages
 constexpr int kHalf = 128 * 128;         // 128 rows x 64 values of 16 bits: one SW128 box
-constexpr int kSoft = 256, kThreads = kSoft + 64;
+constexpr int kSoft = 256, kThreads = kSoft + 128;
 constexpr float kRaise = 8.0f;
 
-enum { B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + NS, B_S = B_EMPTY + NS, B_P = B_S + 2, B_O = B_P + 4, B_DRAIN = B_O + 2,
-       B_COUNT = B_DRAIN + 1 };
+enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + 2, B_P = B_S + 2, B_O = B_P + 4,
+       B_DRAIN = B_O + 2, B_COUNT };
 
 template <int D>
 struct Smem {
@@ -49,11 +58,31 @@ struct Smem {
 };
 
 struct Job {
-    int s0, s1, r0;   // the sequence's rows, the first row of the CTA's tiles
+    int s0, s1, r0;   // the sequence's rows, the first row of the job's tiles
+};
+// Key tiles [from[x], to[x]) of a job's tile x, counted from the sequence's start; `masked` where some row of it does not see
+// some key of the tile.
+struct Keys {
+    int lo[2], hi[2], from[2], to[2], j0, j1, window;
+    __device__ __forceinline__ Keys(const Job& job, int R, int w) : window(w) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            lo[x] = job.r0 + x * R - job.s0;
+            hi[x] = min(lo[x] + R, job.s1 - job.s0) - 1;   // rows of the tile
+            from[x] = w > 0 ? max(0, lo[x] - w + 1) / BK : 0;
+            to[x] = lo[x] < job.s1 - job.s0 ? hi[x] / BK + 1 : 0;
+        }
+        j0 = from[0];
+        j1 = max(to[0], to[1]);
+    }
+    __device__ __forceinline__ bool active(int x, int j) const { return j >= from[x] && j < to[x]; }
+    __device__ __forceinline__ bool masked(int x, int j) const {
+        return j * BK + BK - 1 > lo[x] || (window > 0 && j * BK <= hi[x] - window);
+    }
+    __device__ __forceinline__ bool any_masked(int j) const { return (active(0, j) && masked(0, j)) || (active(1, j) && masked(1, j)); }
 };
 
-// The CTA's tile: sequences in order, each from its last (longest) tile to its
-// first; 32 sequences at a time, one a lane. s1 = 0 past the last tile.
+// Job `tile`: sequences in order, each from its last (longest) job to its 32 sequences at a time, one a lane. s1 = 0 past the last one.
 __device__ __forceinline__ Job find_job(const int32_t* cu, int B, int n_rows, int tile, int rows) {
     const int lane = threadIdx.x & 31;
     for (int b = 0; b < B; b += 32) {
@@ -106,6 +135,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
     return *reinterpret_cast<float2*>(&r);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 template <class E> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     uint32_t r;
@@ -153,168 +187,201 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + M::bar);
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + M::bar + 8 * B_COUNT);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-    volatile int* s_odd = s_abort + 1;                       // values that are not finite were met
-    Job* s_job = reinterpret_cast<Job*>(s_tmem + 4);
+    volatile int* s_odd = s_abort + 1;   // [4] jobs (counted from 1) in which values that are not finite were met
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hk = blockIdx.x % A.HKV, R = A.R, G = A.G;
+    const int R = A.R, G = A.G;
     pdl_trigger();
-    pdl_wait();
-    if (warp == 0) {
-        const Job j = find_job(A.cu, A.B, A.n_rows, blockIdx.x / A.HKV, 2 * R);
-        if (lane == 0) *s_job = j;
-    }
     if (threadIdx.x == kSoft) {
         *s_abort = 0;
-        *s_odd = 0;
-        mbar_init(&bar[B_Q], 1);
-        for (int s = 0; s < NS; ++s) {
-            mbar_init(&bar[B_FULL + s], 1);
-            mbar_init(&bar[B_EMPTY + s], 1);
+        for (int i = 0; i < 4; ++i) s_odd[i] = 0;
+        for (int i = 0; i < B_COUNT; ++i) {
+            const bool v_place = i >= B_EMPTY && i < B_CLEAN && (i - B_EMPTY) % 2 == 1;
+            mbar_init(&bar[i], v_place ? 65 : i >= B_P && i < B_O ? 128 : i >= B_CLEAN && i < B_S ? 64 : 1);
         }
-        for (int x = 0; x < 2; ++x) {
-            mbar_init(&bar[B_S + x], 1);
-            mbar_init(&bar[B_P + 2 * x], 128);
-            mbar_init(&bar[B_P + 2 * x + 1], 128);
-            mbar_init(&bar[B_O + x], 1);
-        }
-        mbar_init(&bar[B_DRAIN], 1);
         mbar_fence_init();
     }
-    __syncthreads();
-    const int s0 = s_job->s0, s1 = s_job->s1, r0 = s_job->r0;
-    if (s1 == 0) return;
+    // tensor memory only after the wait: a kernel that this one follows, and waits for, may still need its own
+    pdl_wait();
     if (warp == 8) tmem_alloc(s_tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
-    // key tiles [first[x], end[x]) of tile x, counted from the sequence's start
-    int first[2], end[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int lo = r0 + x * R - s0, hi = min(lo + R, s1 - s0) - 1;   // rows of the tile
-        first[x] = A.window > 0 ? max(0, lo - A.window + 1) / BK : 0;
-        end[x] = lo < s1 - s0 ? hi / BK + 1 : 0;
-    }
-    const int j0 = first[0], j1 = max(end[0], end[1]);
-    const int tiles = end[1] ? 2 : 1;
+    // job n of this CTA; false past the last
+    auto find = [&](int n, Job* job, int* hk) {
+        const int64_t id = blockIdx.x + (int64_t)n * gridDim.x;
+        *hk = (int)(id % A.HKV);
+        *job = find_job(A.cu, A.B, A.n_rows, (int)min(id / A.HKV, (int64_t)INT_MAX / 2), 2 * R);
+        return job->s1 != 0;
+    };
+    // ring place i (counted over all jobs)
+    auto stage = [&](int i) { return (i % NS) * M::tile; };
+    auto full = [&](int i) { return mbar_wait_soon(&bar[B_FULL + i % NS], (uint32_t)((i / NS) & 1), s_abort); };
 
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");   // 256 x 208 + 128 x 80 <= 384 x 168
+    Job job;
+    int hk;
     if (warp == 9) {
-        if (lane == 0) {
-            mbar_expect_tx(&bar[B_Q], (uint32_t)(tiles * M::halves * G * R * 128));
-            for (int x = 0; x < tiles; ++x)
-                for (int h = 0; h < M::halves; ++h)
-                    tma_load_3d(sm + x * M::tile + h * kHalf, &qmap, 64 * h, hk * G, r0 + x * R, &bar[B_Q]);
-            int i = 0;
-            const int n = 2 * (j1 - j0);   // K and V tiles in turn
-            for (; i < n; ++i) {
-                const int st = i % NS;
-                if (i >= NS && !mbar_wait(&bar[B_EMPTY + st], (uint32_t)((i / NS - 1) & 1), s_abort)) break;
-                mbar_expect_tx(&bar[B_FULL + st], (uint32_t)M::tile);
-                for (int h = 0; h < M::halves; ++h)
-                    tma_load_3d(sm + M::ring + st * M::tile + h * kHalf, i & 1 ? &vmap : &kmap, 64 * h, hk,
-                                s0 + (j0 + i / 2) * BK, &bar[B_FULL + st]);
+        // ---- loads
+        int i = 0, q = 0;
+        bool ok = true;
+        for (; ok && find(q, &job, &hk); ++q) {
+            const Keys ks(job, R, A.window);
+            const int tiles = ks.to[1] ? 2 : 1;
+            if (lane == 0) {
+                if (q > 0) ok = mbar_wait_soon(&bar[B_QFREE], (uint32_t)((q - 1) & 1), s_abort);
+                if (ok) {
+                    mbar_expect_tx(&bar[B_Q], (uint32_t)(tiles * M::halves * G * R * 128));
+                    for (int x = 0; x < tiles; ++x)
+                        for (int h = 0; h < M::halves; ++h)
+                            tma_load_3d(sm + x * M::tile + h * kHalf, &qmap, 64 * h, hk * G, job.r0 + x * R, &bar[B_Q]);
+                    const int n = i + 2 * (ks.j1 - ks.j0);   // K and V tiles in turn
+                    for (int j = ks.j0; i < n; ++i) {
+                        if (i >= NS && !mbar_wait_soon(&bar[B_EMPTY + i % NS], (uint32_t)((i / NS - 1) & 1), s_abort)) break;
+                        uint64_t* b = &bar[B_FULL + i % NS];
+                        mbar_expect_tx(b, (uint32_t)M::tile);
+                        for (int h = 0; h < M::halves; ++h)
+                            tma_load_3d(sm + M::ring + stage(i) + h * kHalf, i & 1 ? &vmap : &kmap, 64 * h, hk, job.s0 + j * BK, b);
+                        j += i & 1;
+                    }
+                    ok = i == n;
+                }
             }
-            if (i < n) *s_abort = 1;
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        }
+        if (lane == 0) {
+            if (!ok) *s_abort = 1;
             // copies in flight land before the CTA's shared memory can go
-            mbar_wait_bounded(&bar[B_Q], 0);
+            if (q > 0) mbar_wait_bounded(&bar[B_Q], (uint32_t)((q - 1) & 1));
             for (int k = i > NS ? i - NS : 0; k < i; ++k) mbar_wait_bounded(&bar[B_FULL + k % NS], (uint32_t)((k / NS) & 1));
         }
+        __syncwarp();
     } else if (warp == 8) {
-        if (lane == 0) {
-            const uint64_t q0 = sw128_desc(sm), k0 = sw128_desc(sm + M::ring);
-            const uint64_t v0 = sw128_mn_desc(sm + M::ring, kHalf);
-            auto stage = [&](int i) { return (uint64_t)((i % NS) * M::tile >> 4); };
-            auto full = [&](int i) {
-                const bool ok = mbar_wait(&bar[B_FULL + i % NS], (uint32_t)((i / NS) & 1), s_abort);
-                tc_fence_after();
-                return ok;
-            };
-            auto scores = [&](int x, int j) {   // S_x = Q_x K_j^T
-                const uint64_t a = q0 + (uint64_t)(x * M::tile >> 4), b = k0 + stage(2 * (j - j0));
+        // ---- products; the warp stays together: uniform operands, one lane issues
+        const uint32_t who = elect_one();
+        const uint64_t kd = sw128_desc(sm + M::ring), vd = sw128_mn_desc(sm + M::ring, kHalf);
+        const uint64_t qd[2] = {sw128_desc(sm), sw128_desc(sm + M::tile)};
+        auto scores = [&](int x, uint64_t b) {   // S_x = Q_x K^T
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t o = (uint64_t)(((k / 4) * kHalf + (k % 4) * 32) >> 4);
-                    umma_f16_ss(tmem + 128 * x, a + o, b + o, kDescS, k > 0);
-                }
-                umma_commit(&bar[B_S + x]);
-            };
-            auto active = [&](int x, int j) { return j >= first[x] && j < end[x]; };
-            int n[2] = {0, 0};   // weight tiles taken
-            bool ok = mbar_wait(&bar[B_Q], 0, s_abort) && full(0);
-            if (ok) {
-                for (int x = 0; x < 2; ++x)
-                    if (active(x, j0)) scores(x, j0);
-                umma_commit(&bar[B_EMPTY + 0]);
+            for (int k = 0; k < D / 16; ++k) {
+                const uint64_t o = (uint64_t)(((k / 4) * kHalf + (k % 4) * 32) >> 4);
+                umma_f16_ss(tmem + 128 * x, qd[x] + o, b + o, kDescS, k > 0, who);
             }
-            for (int j = j0; j < j1 && ok; ++j) {
-                const bool more = j + 1 < j1;
-                const int iv = 2 * (j - j0) + 1;
-                if (more) ok = full(iv + 1);
-                ok = ok && full(iv);
-                for (int x = 0; x < 2 && ok; ++x) {
-                    if (active(x, j)) {
-                        const uint64_t b = v0 + stage(iv);
-                        for (int h = 0; h < 2 && ok; ++h) {   // 64 keys as soon as their weights are there
-                            ok = mbar_wait(&bar[B_P + 2 * x + h], (uint32_t)(n[x] & 1), s_abort);
-                            if (!ok) break;
+            umma_commit_by(&bar[B_S + x], who);
+        };
+        bool ok = true;
+        int i = 0;
+        uint32_t clean = 0;          // phases of the two places
+        uint32_t seen[2] = {0, 0};   // tiles of weights taken, over all jobs
+        for (int q = 0; ok && find(q, &job, &hk); ++q) {
+            const Keys ks(job, R, A.window);
+            ok = mbar_wait_soon(&bar[B_Q], (uint32_t)(q & 1), s_abort) && full(i);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                if (ks.active(x, ks.j0)) scores(x, kd + (uint64_t)(stage(i) >> 4));
+            umma_commit_by(&bar[B_EMPTY + i % NS], who);
+            if (ks.j0 + 1 == ks.j1) umma_commit_by(&bar[B_QFREE], who);
+            ++i;
+            uint32_t fresh[2] = {1, 1};
+            for (int j = ks.j0; j < ks.j1; ++j, i += 2) {   // V_j in ring place i, K_{j+1} in the next
+                const bool more = j + 1 < ks.j1;
+                ok = full(i) && (!more || full(i + 1));
+                if (ks.any_masked(j)) {
+                    const int z = (i >> 1) & 1;   // which of the ring's two V places
+                    ok = ok && mbar_wait_soon(&bar[B_CLEAN + z], clean >> z & 1, s_abort);
+                    clean ^= 1u << z;
+                }
+                const uint64_t v = vd + (uint64_t)(stage(i) >> 4), kn = kd + (uint64_t)(stage(i + 1) >> 4);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (ks.active(x, j)) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {   // O_x += P_x V_j, 64 keys as soon as their weights are there
+                            ok = ok && mbar_wait_soon(&bar[B_P + 2 * x + h], seen[x] & 1, s_abort);
+                            if (!__all_sync(0xffffffffu, ok)) break;
                             tc_fence_after();
 #pragma unroll
                             for (int k = 4 * h; k < 4 * h + 4; ++k)
-                                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, b + (uint64_t)(k * 16 * 128 >> 4), kDescO,
-                                            n[x] > 0 || k > 0);
+                                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, v + (uint64_t)(k * 16 * 128 >> 4), kDescO,
+                                            !fresh[x] || k > 0, who);
                         }
-                        if (!ok) break;
-                        ++n[x];
-                        if (j + 1 == end[x]) umma_commit(&bar[B_O + x]);
+                        ++seen[x];
+                        fresh[x] = 0;
+                        if (j + 1 == ks.to[x]) umma_commit_by(&bar[B_O + x], who);
                     }
-                    if (more && active(x, j + 1)) scores(x, j + 1);
+                    if (more && ks.active(x, j + 1)) scores(x, kn);
                 }
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                umma_commit(&bar[B_EMPTY + iv % NS]);
-                if (more) umma_commit(&bar[B_EMPTY + (iv + 1) % NS]);
+                umma_commit_by(&bar[B_EMPTY + i % NS], who);
+                if (more) {
+                    umma_commit_by(&bar[B_EMPTY + (i + 1) % NS], who);
+                    if (j + 2 == ks.j1) umma_commit_by(&bar[B_QFREE], who);   // the job's last scores
+                }
             }
-            if (!ok) *s_abort = 1;
-            umma_commit(&bar[B_DRAIN]);
-            mbar_wait_bounded(&bar[B_DRAIN], 0);
+            --i;   // the last V had no K behind it
         }
+        if (!ok) *s_abort = 1;
+        // the MMAs issued so far read shared memory and write tensor memory: they end before either is freed
+        umma_commit_by(&bar[B_DRAIN], who);
+        mbar_wait_bounded(&bar[B_DRAIN], 0);
+        __syncwarp();
+    } else if (warp >= 10) {
+        // ---- values that are not finite
+        bool ok = true;
+        int i = 0;
+        for (int q = 0; ok && find(q, &job, &hk); ++q) {
+            const Keys ks(job, R, A.window);
+            for (int j = ks.j0; j < ks.j1 && ok; ++j) {
+                // every V place in its turn, and released by these warps too: a phase passed over could be taken for another
+                const int place = i + 2 * (j - ks.j0) + 1;
+                ok = full(place);
+                if (!ok) break;
+                if (ks.any_masked(j)) {
+                    uint4* t = reinterpret_cast<uint4*>(sm + M::ring + stage(place));
+                    bool odd = false;
+#pragma unroll 4
+                    for (int e = threadIdx.x - 320; e < M::tile / 16; e += 64) {
+                        uint4 w = t[e];
+                        if (not_finite2<E>(w.x) | not_finite2<E>(w.y) | not_finite2<E>(w.z) | not_finite2<E>(w.w)) {
+                            uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+                            for (int k = 0; k < 4; ++k) u[k] &= ~((not_finite2<E>(u[k]) >> 15) * 0xFFFFu);
+                            t[e] = w;
+                            odd = true;
+                        }
+                    }
+                    if (odd) s_odd[q & 3] = q + 1;
+                    fence_async_smem();
+                    mbar_arrive(&bar[B_CLEAN + ((place >> 1) & 1)]);
+                }
+                mbar_arrive(&bar[B_EMPTY + place % NS]);
+            }
+            i += 2 * (ks.j1 - ks.j0);
+        }
+        if (!ok) *s_abort = 1;
         __syncwarp();
     } else {
+        // ---- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int x = warp >> 2, row = threadIdx.x & 127;   // MMA row = tensor-memory lane
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + 128 * x + lanes, to = tmem + 256 + 128 * x + lanes;
-        const int lo = r0 + x * R - s0, hi = min(lo + R, s1 - s0) - 1;
+        bool ok = true;
+        uint32_t n = 0, outs = 0;   // score tiles and outputs taken, over all jobs
+        for (int q = 0; ok && find(q, &job, &hk); ++q) {
+        const Keys ks(job, R, A.window);
+        const int from = x ? ks.from[1] : ks.from[0], upto = x ? ks.to[1] : ks.to[0];
+        const int lo = x ? ks.lo[1] : ks.lo[0], hi = x ? ks.hi[1] : ks.hi[0];
         const int i = lo + row / G;                          // this row's position in the sequence
         const bool live = row < R * G && i <= hi;
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;
-        for (int j = first[x]; j < end[x]; ++j) {
+        for (int j = from; j < upto; ++j, ++n) {
             const int kb = j * BK;
             const bool masked = kb + BK - 1 > lo || (A.window > 0 && kb <= hi - A.window);
-            if (masked) {
-                // values that a row does not see must not reach it as 0 x inf: the tile's
-                // values that are not finite become 0, and the rows that see them get them at the end
-                const int iv = 2 * (j - j0) + 1;
-                ok = mbar_wait(&bar[B_FULL + iv % NS], (uint32_t)((iv / NS) & 1), s_abort);
-                if (!ok) break;
-                uint4* t = reinterpret_cast<uint4*>(sm + M::ring + (iv % NS) * M::tile);
-                bool odd = false;
-                for (int e = row; e < M::tile / 16; e += 128) {
-                    uint4 w = t[e];
-                    if (not_finite2<E>(w.x) | not_finite2<E>(w.y) | not_finite2<E>(w.z) | not_finite2<E>(w.w)) {
-                        uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t b = not_finite2<E>(u[k]);
-                            u[k] &= ~((b >> 15) * 0xFFFFu);
-                        }
-                        t[e] = w;
-                        odd = true;
-                    }
-                }
-                if (odd) *s_odd = 1;
-                fence_async_smem();
-            }
-            ok = mbar_wait(&bar[B_S + x], (uint32_t)((j - first[x]) & 1), s_abort);
+            ok = mbar_wait_soon(&bar[B_S + x], n & 1, s_abort);
             if (!ok) break;
             tc_fence_after();
             float s[4][32];
@@ -335,39 +402,13 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     for (int e = 0; e < 32; ++e)
                         if (32 * c + e > top || 32 * c + e <= bottom) s[c][e] = -INFINITY;
             }
-            float mm[8];   // eight chains of three-operand maxima
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mm[e] = fmaxf(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1]);
-#pragma unroll
-            for (int u = 2; u < 16; u += 2)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) mm[e] = fmaxf(fmaxf(mm[e], s[e / 2][16 * (e % 2) + u]), s[e / 2][16 * (e % 2) + u + 1]);
-            const float mx = fmaxf(fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])), fmaxf(fmaxf(mm[4], mm[5]), fmaxf(mm[6], mm[7])));
-            if (j == first[x]) {
-                m = mx;
-            } else {
-                const bool raise = (mx - m) * A.c > kRaise;   // also from -inf
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float f = raise ? ex2((m - mx) * A.c) : 1.0f;
-                    if (raise) m = mx;
-                    l *= f;
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        int o[16];
-                        uint32_t u[16];
-                        tmem_ld16(to + 16 * c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__int_as_float(o[e]) * f);
-                        tmem_st16(to + 16 * c, u);
-                    }
-                }
-            }
-            const float2 c2 = make_float2(A.c, A.c), mc2 = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m * A.c, -m * A.c);
-            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t u[32];
+            // Weights of the first 64 keys against the reference as it is, their maximum beside them: the exponentials
+            // and the maxima are different pipes. Where the reference has to rise (and at the first tile) they are done again.
+            float2 sum0, sum1;
+            uint32_t u[32];
+            auto weights = [&](int h) {
+                const float mc = m == -INFINITY ? 0.0f : -m * A.c;
+                const float2 c2 = make_float2(A.c, A.c), mc2 = make_float2(mc, mc);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                     float2 y = fma2(make_float2(s[2 * h + e / 16][2 * e % 32], s[2 * h + e / 16][2 * e % 32 + 1]), c2, mc2);
@@ -377,49 +418,87 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     else sum0 = add2(sum0, y);
                     u[e] = pack2<E>(y.x, y.y);
                 }
+            };
+            auto hand_over = [&](int h) {
                 tmem_st32(ts + 32 * h, u);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&bar[B_P + 2 * x + h]);
+            };
+            for (bool checked = false;;) {
+                sum0 = sum1 = make_float2(0.0f, 0.0f);
+                weights(0);
+                if (checked) break;
+                float mm[8];   // eight chains; a NaN comes through and makes the row's reference NaN
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mm[e] = max3(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1], s[e / 2][16 * (e % 2) + 2]);
+#pragma unroll
+                for (int k = 3; k < 15; k += 2)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mm[e] = max3(mm[e], s[e / 2][16 * (e % 2) + k], s[e / 2][16 * (e % 2) + k + 1]);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
+                const float mx = max3(max3(mm[0], mm[2], mm[4]), mm[6], mm[6]);
+                const bool raise = mx != -INFINITY && !((mx - m) * A.c <= kRaise);   // from -inf, and to NaN, too
+                if (!__any_sync(0xffffffffu, raise)) break;
+                const float f = raise ? ex2((m - mx) * A.c) : 1.0f;
+                if (raise) m = mx;
+                l *= f;
+                if (j > from) {
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        int o[16];
+                        uint32_t w[16];
+                        tmem_ld16(to + 16 * c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__int_as_float(o[e]) * f);
+                        tmem_st16(to + 16 * c, w);
+                    }
+                }
+                checked = true;
             }
+            hand_over(0);
+            weights(1);
+            hand_over(1);
             sum0 = add2(sum0, sum1);
             l += sum0.x + sum0.y;
         }
-        if (ok && end[x]) {
-            ok = mbar_wait(&bar[B_O + x], 0, s_abort);
-            tc_fence_after();
-        }
-        if (!ok) *s_abort = 1;
-        asm volatile("bar.sync 1, 256;" ::: "memory");       // both tiles' finds
-        const bool odd = *s_odd != 0;
-        if (ok && end[x]) {
-            const float inv = 1.0f / l;
-            E* dst = static_cast<E*>(A.out) + (int64_t)(s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D;
-            const E* v = static_cast<const E*>(A.v) + (int64_t)s0 * A.ldkv + (int64_t)hk * D;
+        if (!ok || !upto) continue;
+        ok = mbar_wait_soon(&bar[B_O + x], outs & 1, s_abort);
+        ++outs;
+        if (!ok) break;
+        tc_fence_after();
+        const bool odd = s_odd[q & 3] == q + 1;
+        const float inv = 1.0f / l;
+        E* dst = static_cast<E*>(A.out) + (int64_t)(job.s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D;
+        const E* v = static_cast<const E*>(A.v) + (int64_t)job.s0 * A.ldkv + (int64_t)hk * D;
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                float o[32];
-                tmem_ld32(to + 32 * c, o);
-                tmem_ld_wait();
-                if (live) {
+        for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32(to + 32 * c, o);
+            tmem_ld_wait();
+            if (live) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] *= inv;
-                    if (odd) {
-                        for (int k = A.window > 0 ? max(0, i - A.window + 1) : 0; k <= i; ++k)
+                for (int e = 0; e < 32; ++e) o[e] *= inv;
+                if (odd) {
+                    for (int k = A.window > 0 ? max(0, i - A.window + 1) : 0; k <= i; ++k)
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float y = to_f32<E>(v[k * A.ldkv + 32 * c + e]);
-                                if (!(fabsf(y) < INFINITY)) o[e] += y;
-                            }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(dst + 32 * c + e) =
-                            make_uint4(pack2<E>(o[e], o[e + 1]), pack2<E>(o[e + 2], o[e + 3]), pack2<E>(o[e + 4], o[e + 5]),
-                                       pack2<E>(o[e + 6], o[e + 7]));
+                        for (int e = 0; e < 32; ++e) {
+                            const float y = to_f32<E>(v[k * A.ldkv + 32 * c + e]);
+                            if (!(fabsf(y) < INFINITY)) o[e] += y;
+                        }
                 }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    *reinterpret_cast<uint4*>(dst + 32 * c + e) =
+                        make_uint4(pack2<E>(o[e], o[e + 1]), pack2<E>(o[e + 2], o[e + 3]), pack2<E>(o[e + 4], o[e + 5]),
+                                   pack2<E>(o[e + 6], o[e + 7]));
             }
         }
+        tc_fence_before();   // O is read before the next job's first weights are handed over
+        }
+        if (!ok) *s_abort = 1;
         tc_fence_before();
     }
     __syncthreads();
@@ -480,8 +559,8 @@ cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void*
     constexpr float kLog2e = 1.4426950408889634f;
     pk::Args a{cu, B, n_rows, HKV, G, R, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
                window, out, ldo, v, ldkv};
-    const int64_t tiles = n_rows / (2 * R) + std::min<int64_t>(B, n_rows);
-    return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)(tiles * HKV)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
+    const int64_t jobs = (n_rows / (2 * R) + std::min<int64_t>(B, n_rows)) * HKV;
+    return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)std::min<int64_t>(jobs, 148)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
                       km, vm, a);
 }
 

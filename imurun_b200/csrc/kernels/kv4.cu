@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     for (int j = 0; j < n; ++j) {
         if ((j & 15) == 16 - kSlots) ids_next = look_up((j & ~15) + 16);
         const uint32_t parity = (uint32_t)(j / kSlots) & 1u;
-        ok = ok && (mbar_try_wait(&bar[j % kSlots], parity) || mbar_wait_bounded(&bar[j % kSlots], parity));
+        ok = ok && mbar_wait_soon(&bar[j % kSlots], parity, nullptr);
         __syncwarp();
         const uint8_t* rec0 = ring + (j % kSlots) * 2 * R::bytes;
         // ---- scores of keys row and row + 8 (0, 1 and 2, 3) of both pages, heads 2 t, 2 t + 1, in log2 units
