@@ -41,30 +41,31 @@
 namespace fb {
 namespace pk {
 
-constexpr int BK = 128, NS = 4;          // keys a tile, ring stages
+constexpr int BK = 128, NS = 2;          // keys a tile, ring places of a V and a K tile
 constexpr int kHalf = 128 * 128;         // 128 rows x 64 values of 16 bits: one SW128 box
 constexpr int kSoft = 256, kThreads = kSoft + 128;
 constexpr float kRaise = 8.0f;
 
-enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + 2, B_P = B_S + 2, B_O = B_P + 4,
+enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + NS, B_P = B_S + 2, B_O = B_P + 4,
        B_DRAIN = B_O + 2, B_COUNT };
 
 template <int D>
 struct Smem {
     static constexpr int halves = (D + 63) / 64;
     static constexpr int tile = halves * kHalf;            // one Q, K or V tile
-    static constexpr int ring = 2 * tile, bar = ring + NS * tile;
+    static constexpr int place = 2 * tile;                 // V_j and, behind it, K_{j+1}
+    static constexpr int ring = 2 * tile, bar = ring + NS * place;
     static constexpr int bytes = bar + 8 * B_COUNT + 64 + 1024;
 };
 
 struct Job {
     int s0, s1, r0;   // the sequence's rows, the first row of the job's tiles
 };
-// Key tiles [from[x], to[x]) of a job's tile x, counted from the sequence's start; `masked` where some row of it does not see
-// some key of the tile.
+// Key tiles [from[x], to[x]) of a job's tile x, counted from the sequence's start; `masked` where some row of the job does not
+// see some key of the tile.
 struct Keys {
-    int lo[2], hi[2], from[2], to[2], j0, j1, window;
-    __device__ __forceinline__ Keys(const Job& job, int R, int w) : window(w) {
+    int lo[2], hi[2], from[2], to[2], j0, j1, upper, lower;
+    __device__ __forceinline__ Keys(const Job& job, int R, int w) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             lo[x] = job.r0 + x * R - job.s0;
@@ -74,12 +75,12 @@ struct Keys {
         }
         j0 = from[0];
         j1 = max(to[0], to[1]);
+        upper = (lo[0] + 1) / BK;                                     // from here on keys past the first row
+        const int out = (to[1] ? hi[1] : hi[0]) - w;
+        lower = w > 0 && out >= 0 ? out / BK : -1;                    // up to here keys before the last row's window
     }
     __device__ __forceinline__ bool active(int x, int j) const { return j >= from[x] && j < to[x]; }
-    __device__ __forceinline__ bool masked(int x, int j) const {
-        return j * BK + BK - 1 > lo[x] || (window > 0 && j * BK <= hi[x] - window);
-    }
-    __device__ __forceinline__ bool any_masked(int j) const { return (active(0, j) && masked(0, j)) || (active(1, j) && masked(1, j)); }
+    __device__ __forceinline__ bool masked(int j) const { return j >= upper || j <= lower; }
 };
 
 // Job `tile`: sequences in order, each from its last (longest) job to its 32 sequences at a time, one a lane. s1 = 0 past the last one.
@@ -135,6 +136,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
     return *reinterpret_cast<float2*>(&r);
 }
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// Waits of the roles. A wait that runs out (some 10 ms at least) marks the CTA: every role then goes through its loops without
+// waiting, on whatever lies in shared and tensor memory, and the CTA ends.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n)
+        if ((n & 255) == 0 && (*abort || n >= 1u << 22)) {
+            *abort = 1;
+            break;
+        }
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -165,6 +180,7 @@ struct Args {
     int window;
     void* out;
     int64_t ldo;
+    int wide;       // rows of out on 32-byte boundaries
     const void* v;  // for rows that see values which are not finite
     int64_t ldkv;
 };
@@ -195,8 +211,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         *s_abort = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
         for (int i = 0; i < B_COUNT; ++i) {
-            const bool v_place = i >= B_EMPTY && i < B_CLEAN && (i - B_EMPTY) % 2 == 1;
-            mbar_init(&bar[i], v_place ? 65 : i >= B_P && i < B_O ? 128 : i >= B_CLEAN && i < B_S ? 64 : 1);
+            mbar_init(&bar[i], i >= B_EMPTY && i < B_CLEAN ? 65 : i >= B_CLEAN && i < B_S ? 64 : i >= B_P && i < B_O ? 128 : 1);
         }
         mbar_fence_init();
     }
@@ -209,50 +224,48 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     const uint32_t tmem = *s_tmem;
     // job n of this CTA; false past the last
     auto find = [&](int n, Job* job, int* hk) {
-        const int64_t id = blockIdx.x + (int64_t)n * gridDim.x;
-        *hk = (int)(id % A.HKV);
-        *job = find_job(A.cu, A.B, A.n_rows, (int)min(id / A.HKV, (int64_t)INT_MAX / 2), 2 * R);
-        return job->s1 != 0;
+        const uint32_t id = blockIdx.x + (uint32_t)n * gridDim.x, unit = id / (uint32_t)A.HKV;
+        *hk = (int)(id - unit * A.HKV);
+        *job = find_job(A.cu, A.B, A.n_rows, (int)unit, 2 * R);
+        return job->s1 != 0 && !__any_sync(0xffffffffu, *s_abort);
     };
-    // ring place i (counted over all jobs)
-    auto stage = [&](int i) { return (i % NS) * M::tile; };
-    auto full = [&](int i) { return mbar_wait_soon(&bar[B_FULL + i % NS], (uint32_t)((i / NS) & 1), s_abort); };
+    // ring place i, counted over all jobs; a job of n key tiles takes n + 1: K_0 alone, V_0 with K_1, .., V_{n-1} alone
+    auto v_at = [&](int i) { return (i % NS) * M::place; };
+    auto k_at = [&](int i) { return (i % NS) * M::place + M::tile; };
+    auto full = [&](int i) { wait(&bar[B_FULL + i % NS], (uint32_t)((i / NS) & 1), s_abort); };
 
     if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");   // 256 x 208 + 128 x 80 <= 384 x 168
     Job job;
     int hk;
     if (warp == 9) {
         // ---- loads
-        int i = 0, q = 0;
-        bool ok = true;
-        for (; ok && find(q, &job, &hk); ++q) {
+        int i = 0, loaded = 0;
+        for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
             const int tiles = ks.to[1] ? 2 : 1;
-            if (lane == 0) {
-                if (q > 0) ok = mbar_wait_soon(&bar[B_QFREE], (uint32_t)((q - 1) & 1), s_abort);
-                if (ok) {
-                    mbar_expect_tx(&bar[B_Q], (uint32_t)(tiles * M::halves * G * R * 128));
-                    for (int x = 0; x < tiles; ++x)
-                        for (int h = 0; h < M::halves; ++h)
-                            tma_load_3d(sm + x * M::tile + h * kHalf, &qmap, 64 * h, hk * G, job.r0 + x * R, &bar[B_Q]);
-                    const int n = i + 2 * (ks.j1 - ks.j0);   // K and V tiles in turn
-                    for (int j = ks.j0; i < n; ++i) {
-                        if (i >= NS && !mbar_wait_soon(&bar[B_EMPTY + i % NS], (uint32_t)((i / NS - 1) & 1), s_abort)) break;
-                        uint64_t* b = &bar[B_FULL + i % NS];
-                        mbar_expect_tx(b, (uint32_t)M::tile);
-                        for (int h = 0; h < M::halves; ++h)
-                            tma_load_3d(sm + M::ring + stage(i) + h * kHalf, i & 1 ? &vmap : &kmap, 64 * h, hk, job.s0 + j * BK, b);
-                        j += i & 1;
+            if (lane == 0 && q > 0) wait(&bar[B_QFREE], (uint32_t)((q - 1) & 1), s_abort);
+            if (lane == 0 && !*s_abort) {   // a marked CTA brings nothing more
+                ++loaded;
+                mbar_expect_tx(&bar[B_Q], (uint32_t)(tiles * M::halves * G * R * 128));
+                for (int x = 0; x < tiles; ++x)
+                    for (int h = 0; h < M::halves; ++h)
+                        tma_load_3d(sm + x * M::tile + h * kHalf, &qmap, 64 * h, hk * G, job.r0 + x * R, &bar[B_Q]);
+                for (int j = ks.j0; j <= ks.j1; ++j, ++i) {   // V_{j-1} and K_j
+                    if (i >= NS) wait(&bar[B_EMPTY + i % NS], (uint32_t)((i / NS - 1) & 1), s_abort);
+                    if (*s_abort) break;
+                    uint64_t* b = &bar[B_FULL + i % NS];
+                    mbar_expect_tx(b, (uint32_t)(M::tile * ((j > ks.j0) + (j < ks.j1))));
+                    for (int h = 0; h < M::halves; ++h) {
+                        if (j > ks.j0) tma_load_3d(sm + M::ring + v_at(i) + h * kHalf, &vmap, 64 * h, hk, job.s0 + (j - 1) * BK, b);
+                        if (j < ks.j1) tma_load_3d(sm + M::ring + k_at(i) + h * kHalf, &kmap, 64 * h, hk, job.s0 + j * BK, b);
                     }
-                    ok = i == n;
                 }
             }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            __syncwarp();
         }
         if (lane == 0) {
-            if (!ok) *s_abort = 1;
             // copies in flight land before the CTA's shared memory can go
-            if (q > 0) mbar_wait_bounded(&bar[B_Q], (uint32_t)((q - 1) & 1));
+            if (loaded > 0) mbar_wait_bounded(&bar[B_Q], (uint32_t)((loaded - 1) & 1));
             for (int k = i > NS ? i - NS : 0; k < i; ++k) mbar_wait_bounded(&bar[B_FULL + k % NS], (uint32_t)((k / NS) & 1));
         }
         __syncwarp();
@@ -269,39 +282,37 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
             }
             umma_commit_by(&bar[B_S + x], who);
         };
-        bool ok = true;
         int i = 0;
-        uint32_t clean = 0;          // phases of the two places
+        uint32_t clean = 0;          // phases of the places' barriers
         uint32_t seen[2] = {0, 0};   // tiles of weights taken, over all jobs
-        for (int q = 0; ok && find(q, &job, &hk); ++q) {
+        for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
-            ok = mbar_wait_soon(&bar[B_Q], (uint32_t)(q & 1), s_abort) && full(i);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            wait(&bar[B_Q], (uint32_t)(q & 1), s_abort);
+            full(i);
             tc_fence_after();
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-                if (ks.active(x, ks.j0)) scores(x, kd + (uint64_t)(stage(i) >> 4));
+                if (ks.active(x, ks.j0)) scores(x, kd + (uint64_t)(k_at(i) >> 4));
             umma_commit_by(&bar[B_EMPTY + i % NS], who);
             if (ks.j0 + 1 == ks.j1) umma_commit_by(&bar[B_QFREE], who);
-            ++i;
+            full(++i);
             uint32_t fresh[2] = {1, 1};
-            for (int j = ks.j0; j < ks.j1; ++j, i += 2) {   // V_j in ring place i, K_{j+1} in the next
+            for (int j = ks.j0; j < ks.j1; ++j) {   // V_j and K_{j+1} in place i
                 const bool more = j + 1 < ks.j1;
-                ok = full(i) && (!more || full(i + 1));
-                if (ks.any_masked(j)) {
-                    const int z = (i >> 1) & 1;   // which of the ring's two V places
-                    ok = ok && mbar_wait_soon(&bar[B_CLEAN + z], clean >> z & 1, s_abort);
+                if (ks.masked(j)) {
+                    const int z = i % NS;
+                    wait(&bar[B_CLEAN + z], clean >> z & 1, s_abort);
                     clean ^= 1u << z;
                 }
-                const uint64_t v = vd + (uint64_t)(stage(i) >> 4), kn = kd + (uint64_t)(stage(i + 1) >> 4);
+                const uint64_t v = vd + (uint64_t)(v_at(i) >> 4), kn = kd + (uint64_t)(k_at(i) >> 4);
+                uint64_t* empty = &bar[B_EMPTY + i % NS];
+                ++i;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if (ks.active(x, j)) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {   // O_x += P_x V_j, 64 keys as soon as their weights are there
-                            ok = ok && mbar_wait_soon(&bar[B_P + 2 * x + h], seen[x] & 1, s_abort);
-                            if (!__all_sync(0xffffffffu, ok)) break;
+                            wait(&bar[B_P + 2 * x + h], seen[x] & 1, s_abort);
                             tc_fence_after();
 #pragma unroll
                             for (int k = 4 * h; k < 4 * h + 4; ++k)
@@ -313,35 +324,26 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                         if (j + 1 == ks.to[x]) umma_commit_by(&bar[B_O + x], who);
                     }
                     if (more && ks.active(x, j + 1)) scores(x, kn);
+                    if (more && x == 0) full(i);   // what the next turn reads, looked for while the other tile's weights are formed
                 }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                umma_commit_by(&bar[B_EMPTY + i % NS], who);
-                if (more) {
-                    umma_commit_by(&bar[B_EMPTY + (i + 1) % NS], who);
-                    if (j + 2 == ks.j1) umma_commit_by(&bar[B_QFREE], who);   // the job's last scores
-                }
+                umma_commit_by(empty, who);
+                if (j + 2 == ks.j1) umma_commit_by(&bar[B_QFREE], who);   // the job's last scores
             }
-            --i;   // the last V had no K behind it
         }
-        if (!ok) *s_abort = 1;
         // the MMAs issued so far read shared memory and write tensor memory: they end before either is freed
         umma_commit_by(&bar[B_DRAIN], who);
         mbar_wait_bounded(&bar[B_DRAIN], 0);
         __syncwarp();
     } else if (warp >= 10) {
         // ---- values that are not finite
-        bool ok = true;
         int i = 0;
-        for (int q = 0; ok && find(q, &job, &hk); ++q) {
+        for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
-            for (int j = ks.j0; j < ks.j1 && ok; ++j) {
-                // every V place in its turn, and released by these warps too: a phase passed over could be taken for another
-                const int place = i + 2 * (j - ks.j0) + 1;
-                ok = full(place);
-                if (!ok) break;
-                if (ks.any_masked(j)) {
-                    uint4* t = reinterpret_cast<uint4*>(sm + M::ring + stage(place));
+            for (int j = ks.j0; j <= ks.j1; ++j, ++i) {   // V_{j-1} in place i
+                // every place in its turn, and released by these warps too: a phase passed over could be taken for another
+                full(i);
+                if (j > ks.j0 && ks.masked(j - 1)) {
+                    uint4* t = reinterpret_cast<uint4*>(sm + M::ring + v_at(i));
                     bool odd = false;
 #pragma unroll 4
                     for (int e = threadIdx.x - 320; e < M::tile / 16; e += 64) {
@@ -355,13 +357,11 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     }
                     if (odd) s_odd[q & 3] = q + 1;
                     fence_async_smem();
-                    mbar_arrive(&bar[B_CLEAN + ((place >> 1) & 1)]);
+                    mbar_arrive(&bar[B_CLEAN + i % NS]);
                 }
-                mbar_arrive(&bar[B_EMPTY + place % NS]);
+                mbar_arrive(&bar[B_EMPTY + i % NS]);
             }
-            i += 2 * (ks.j1 - ks.j0);
         }
-        if (!ok) *s_abort = 1;
         __syncwarp();
     } else {
         // ---- softmax
@@ -369,9 +369,8 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         const int x = warp >> 2, row = threadIdx.x & 127;   // MMA row = tensor-memory lane
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + 128 * x + lanes, to = tmem + 256 + 128 * x + lanes;
-        bool ok = true;
         uint32_t n = 0, outs = 0;   // score tiles and outputs taken, over all jobs
-        for (int q = 0; ok && find(q, &job, &hk); ++q) {
+        for (int q = 0; find(q, &job, &hk); ++q) {
         const Keys ks(job, R, A.window);
         const int from = x ? ks.from[1] : ks.from[0], upto = x ? ks.to[1] : ks.to[0];
         const int lo = x ? ks.lo[1] : ks.lo[0], hi = x ? ks.hi[1] : ks.hi[0];
@@ -381,8 +380,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         for (int j = from; j < upto; ++j, ++n) {
             const int kb = j * BK;
             const bool masked = kb + BK - 1 > lo || (A.window > 0 && kb <= hi - A.window);
-            ok = mbar_wait_soon(&bar[B_S + x], n & 1, s_abort);
-            if (!ok) break;
+            wait(&bar[B_S + x], n & 1, s_abort);
             tc_fence_after();
             float s[4][32];
 #pragma unroll
@@ -464,10 +462,9 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
             sum0 = add2(sum0, sum1);
             l += sum0.x + sum0.y;
         }
-        if (!ok || !upto) continue;
-        ok = mbar_wait_soon(&bar[B_O + x], outs & 1, s_abort);
+        if (!upto) continue;
+        wait(&bar[B_O + x], outs & 1, s_abort);
         ++outs;
-        if (!ok) break;
         tc_fence_after();
         const bool odd = s_odd[q & 3] == q + 1;
         const float inv = 1.0f / l;
@@ -489,16 +486,21 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                             if (!(fabsf(y) < INFINITY)) o[e] += y;
                         }
                 }
+                uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                    *reinterpret_cast<uint4*>(dst + 32 * c + e) =
-                        make_uint4(pack2<E>(o[e], o[e + 1]), pack2<E>(o[e + 2], o[e + 3]), pack2<E>(o[e + 4], o[e + 5]),
-                                   pack2<E>(o[e + 6], o[e + 7]));
+                for (int e = 0; e < 16; ++e) w[e] = pack2<E>(o[2 * e], o[2 * e + 1]);
+                if (A.wide) {   // whole sectors
+                    store32(dst + 32 * c, w);
+                    store32(dst + 32 * c + 16, w + 8);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<uint4*>(dst + 32 * c + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+                }
             }
         }
         tc_fence_before();   // O is read before the next job's first weights are handed over
         }
-        if (!ok) *s_abort = 1;
         tc_fence_before();
     }
     __syncthreads();
@@ -558,8 +560,9 @@ cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void*
     }
     constexpr float kLog2e = 1.4426950408889634f;
     pk::Args a{cu, B, n_rows, HKV, G, R, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
-               window, out, ldo, v, ldkv};
+               window, out, ldo, (reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * 2)) % 32 == 0, v, ldkv};
     const int64_t jobs = (n_rows / (2 * R) + std::min<int64_t>(B, n_rows)) * HKV;
+    if (jobs > INT_MAX / 2) return cudaErrorInvalidValue;
     return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)std::min<int64_t>(jobs, 148)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
                       km, vm, a);
 }
