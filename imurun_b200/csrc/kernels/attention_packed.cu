@@ -400,8 +400,6 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     for (int e = 0; e < 32; ++e)
                         if (32 * c + e > top || 32 * c + e <= bottom) s[c][e] = -INFINITY;
             }
-            // Weights of the first 64 keys against the reference as it is, their maximum beside them: the exponentials
-            // and the maxima are different pipes. Where the reference has to rise (and at the first tile) they are done again.
             float2 sum0, sum1;
             uint32_t u[32];
             auto weights = [&](int h) {
@@ -423,27 +421,23 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                 tc_fence_before();
                 mbar_arrive(&bar[B_P + 2 * x + h]);
             };
-            for (bool checked = false;;) {
-                sum0 = sum1 = make_float2(0.0f, 0.0f);
-                weights(0);
-                if (checked) break;
-                float mm[8];   // eight chains; a NaN comes through and makes the row's reference NaN
+            float mm[8];   // eight chains; a NaN comes through and makes the row's reference NaN
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mm[e] = max3(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1], s[e / 2][16 * (e % 2) + 2]);
+            for (int e = 0; e < 8; ++e) mm[e] = max3(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1], s[e / 2][16 * (e % 2) + 2]);
 #pragma unroll
-                for (int k = 3; k < 15; k += 2)
+            for (int k = 3; k < 15; k += 2)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mm[e] = max3(mm[e], s[e / 2][16 * (e % 2) + k], s[e / 2][16 * (e % 2) + k + 1]);
+                for (int e = 0; e < 8; ++e) mm[e] = max3(mm[e], s[e / 2][16 * (e % 2) + k], s[e / 2][16 * (e % 2) + k + 1]);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
-                const float mx = max3(max3(mm[0], mm[2], mm[4]), mm[6], mm[6]);
-                const bool raise = mx != -INFINITY && !((mx - m) * A.c <= kRaise);   // from -inf, and to NaN, too
-                if (!__any_sync(0xffffffffu, raise)) break;
+            for (int e = 0; e < 8; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
+            const float mx = max3(max3(mm[0], mm[2], mm[4]), mm[6], mm[6]);
+            const bool raise = mx != -INFINITY && !((mx - m) * A.c <= kRaise);   // from -inf, and to NaN, too
+            if (__any_sync(0xffffffffu, raise)) {
                 const float f = raise ? ex2((m - mx) * A.c) : 1.0f;
                 if (raise) m = mx;
                 l *= f;
                 if (j > from) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         int o[16];
                         uint32_t w[16];
@@ -454,8 +448,9 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                         tmem_st16(to + 16 * c, w);
                     }
                 }
-                checked = true;
             }
+            sum0 = sum1 = make_float2(0.0f, 0.0f);
+            weights(0);
             hand_over(0);
             weights(1);
             hand_over(1);
@@ -470,7 +465,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         const float inv = 1.0f / l;
         E* dst = static_cast<E*>(A.out) + (int64_t)(job.s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D;
         const E* v = static_cast<const E*>(A.v) + (int64_t)job.s0 * A.ldkv + (int64_t)hk * D;
-#pragma unroll
+#pragma unroll 1   // once a job: little code rather than many instruction fetches
         for (int c = 0; c < D / 32; ++c) {
             float o[32];
             tmem_ld32(to + 32 * c, o);
