@@ -370,7 +370,12 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + 128 * x + lanes, to = tmem + 256 + 128 * x + lanes;
         uint32_t n = 0, outs = 0;   // score tiles and outputs taken, over all jobs
-        for (int q = 0; find(q, &job, &hk); ++q) {
+        Job next;
+        int next_hk;
+        bool some = find(0, &next, &next_hk);
+        for (int q = 0; some; ++q) {
+        job = next;
+        hk = next_hk;
         const Keys ks(job, R, A.window);
         const int from = x ? ks.from[1] : ks.from[0], upto = x ? ks.to[1] : ks.to[0];
         const int lo = x ? ks.lo[1] : ks.lo[0], hi = x ? ks.hi[1] : ks.hi[0];
@@ -457,6 +462,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
             sum0 = add2(sum0, sum1);
             l += sum0.x + sum0.y;
         }
+        some = find(q + 1, &next, &next_hk);   // while the last products run
         if (!upto) continue;
         wait(&bar[B_O + x], outs & 1, s_abort);
         ++outs;

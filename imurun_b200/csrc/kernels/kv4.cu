@@ -10,93 +10,136 @@ namespace fb {
 
 // ================================================================ append
 // CTA y of token x takes the heads hpc y .. hpc (y + 1) - 1 of the token's
-// H + 2 HKV (q, then k, then v); a thread owns 8 consecutive dimensions (one
-// 16-byte load of 16-bit values) and walks over the heads, so the token's
-// cos and sin stay in registers. A group of 32 values is four neighbouring
-// threads: its extremes by two shuffles, its codes one 32-bit word of K or
-// two 16-bit words of V a thread. Rotation and quantisation are in 32 bits
-// with every step rounded by itself (no fused multiply-add), so the codes are
-// those of the plain formula.
-template <class E, class O, int D>
+// H + 2 HKV (q, then k, then v), a warp 32 / (D / 8) heads at a time, a lane 8
+// consecutive dimensions (one 16-byte load of 16-bit values). What bounds it is
+// memory: a lane's loads of U heads are issued before anything else, under the
+// chain of position, page and rotation that the stores wait for, and the cos and
+// sin of its 8 dimensions serve all its heads. The partner of a rotated value is
+// in the same lane (pairs of neighbours) or comes by shuffle (halves, where half
+// the rotated dimensions are whole lanes; else by a second load). A group of 32
+// values is four neighbouring lanes: its extremes by two shuffles, its codes one
+// 32-bit word of K or two 16-bit words of V a lane. Rotation and quantisation are
+// in 32 bits with every step rounded by itself (no fused multiply-add), so the
+// codes are those of the plain formula.
+enum : int { ROPE_PAIRS, ROPE_HALVES, ROPE_ANY };
+
+// 8 values as loaded, and as f32
+template <class E> struct Raw8 { uint4 v[sizeof(E) / 2]; };
+template <class E>
+__device__ __forceinline__ Raw8<E> fetch8(const E* p) {
+    Raw8<E> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
+}
+template <class E>
+__device__ __forceinline__ void unpack8(const Raw8<E>& r, float (&x)[8]) {
+    const E* e = reinterpret_cast<const E*>(r.v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32<E>(e[i]);
+}
+
+template <class E, class O, int D, int ROPE>
 __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_kv4_cache c, const E* q, const E* k,
                                                     const E* v, int64_t ldq, int64_t ldkv, int H, int hpc,
                                                     const int32_t* __restrict__ tok_seq,
-                                                    const int32_t* __restrict__ tok_pos, int rot, int neox,
+                                                    const int32_t* __restrict__ tok_pos, int rot,
                                                     const float* __restrict__ rcos, const float* __restrict__ rsin,
                                                     int n_rope, O* q_out, int64_t ldq_out, O* k_out, O* v_out,
                                                     int64_t ldkv_out) {
     using R = Kv4Rec<D>;
-    constexpr int L = D / 8;   // threads a head
+    constexpr int L = D / 8, HPW = 32 / L;   // lanes a head, heads a warp (D = 96: 8 lanes idle)
+    constexpr int U = sizeof(E) == 4 ? 3 : 5;
     pdl_trigger();
+    const int t = blockIdx.x, HKV = c.n_head_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int d0 = (lane % L) * 8, half = rot / 2;
+    const int h0 = hpc * blockIdx.y, h1 = min(h0 + hpc, H + 2 * HKV), step = (int)blockDim.x / 32 * HPW;
+    const bool busy = lane < HPW * L;
+    auto source = [&](int h) {
+        return h < H ? q + t * ldq + h * D : h < H + HKV ? k + t * ldkv + (h - H) * D : v + t * ldkv + (h - H - HKV) * D;
+    };
     pdl_wait();
-    const int t = blockIdx.x, HKV = c.n_head_kv;
-    const int pos = tok_pos[t];
+    Raw8<E> raw[U];
+    auto fetch = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = from + u * step + warp * HPW + lane / L;
+            if (busy && h < h1) raw[u] = fetch8<E>(source(h) + d0);
+        }
+    };
+    fetch(h0);
+    const int pos = __ldg(tok_pos + t), seq = __ldg(tok_seq + t);
     if (pos < 0) return;   // padding
-    const int seq = tok_seq[t];
     if (seq < 0 || seq >= c.n_seqs || pos >= n_rope) {
         if (c.err && threadIdx.x == 0) atomicExch(c.err, 6);
         return;
     }
-    const int page = kv4_page(c, seq, pos / kKv4Page), row = pos % kKv4Page;
-    if (page < 0) return;
-    const int d0 = (threadIdx.x % L) * 8, half = rot / 2;
-    // cos and sin of this thread's 8 dimensions, and where their partners are
+    // cos and sin of this lane's 8 dimensions; x0 cos - x1 sin for the first of a pair, x1 cos + x0 sin for the second
     float cs[8], sn[8];
-    int other[8];
+    const float *cr = rcos + (size_t)pos * half, *sr = rsin + (size_t)pos * half;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int d = d0 + i;
         cs[i] = 1.0f;
         sn[i] = 0.0f;
-        other[i] = d;
         if (d < rot) {
-            const int pair = neox ? (d < half ? d : d - half) : d / 2;
-            const bool first = neox ? d < half : d % 2 == 0;
-            cs[i] = __ldg(rcos + (size_t)pos * half + pair);
-            sn[i] = __ldg(rsin + (size_t)pos * half + pair);
-            if (first) sn[i] = -sn[i];   // x0 cos - x1 sin, and x1 cos + x0 sin for the second
-            other[i] = neox ? (first ? d + half : d - half) : d ^ 1;
+            const bool first = ROPE == ROPE_PAIRS ? i % 2 == 0 : d < half;
+            const int pair = ROPE == ROPE_PAIRS ? d / 2 : first ? d : d - half;
+            cs[i] = __ldg(cr + pair);
+            sn[i] = first ? -__ldg(sr + pair) : __ldg(sr + pair);
         }
     }
-    const int h1 = min(hpc * ((int)blockIdx.y + 1), H + 2 * HKV), step = blockDim.x / L;
-    // whole warps walk together (the shuffles below): a head past the end repeats nothing but takes part
-    for (int hb = hpc * blockIdx.y; hb < h1; hb += step) {
-        const int h = hb + threadIdx.x / L;
-        const bool live = h < h1;
-        const int kind = !live ? 3 : h < H ? 0 : h < H + HKV ? 1 : 2;
-        const int hk = kind == 1 ? h - H : kind == 2 ? h - H - HKV : 0;
-        const E* src = kind == 0 ? q + t * ldq + h * D : kind == 1 ? k + t * ldkv + hk * D : v + t * ldkv + hk * D;
-        float x[8];
+    const int page = kv4_page(c, seq, pos / kKv4Page), row = pos % kKv4Page;
+    if (page < 0) return;
+    for (int hb = h0; hb < h1; hb += U * step) {
+        if (hb > h0) fetch(hb);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-        if (live) load8(src + d0, x);
-        if (kind < 2 && d0 < rot) {
-            float y[8];
+        for (int u = 0; u < U; ++u) {
+            if (hb + u * step >= h1) break;   // the whole CTA
+            const int h = hb + u * step + warp * HPW + lane / L;
+            const bool live = busy && h < h1;
+            const int kind = !live ? 3 : h < H ? 0 : h < H + HKV ? 1 : 2;
+            const int hk = kind == 1 ? h - H : kind == 2 ? h - H - HKV : 0;
+            float x[8], o[8];
+            if (live) unpack8<E>(raw[u], x);
+            else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+            }
+            if (ROPE == ROPE_PAIRS) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
+            } else if (ROPE == ROPE_HALVES) {
+                const int from = lane + (d0 < half ? half / 8 : d0 < rot ? -(half / 8) : 0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], from);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int d = d0 + i;
+                    o[i] = live && d < rot ? to_f32<E>(source(h)[d < half ? d + half : d - half]) : 0.0f;
+                }
+                __syncwarp();   // every read of the head before any write: the outputs may be the inputs
+            }
+            if (kind < 2) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d0 + i < rot) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(o[i], sn[i]));
+            }
+            if (kind == 0) store8(q_out + t * ldq_out + h * D + d0, x);
+            if (!__any_sync(0xffffffffu, kind == 1 || kind == 2)) continue;
+            float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float o = to_f32<E>(src[other[i]]);
-                y[i] = d0 + i < rot ? __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(o, sn[i])) : x[i];
+                lo = fminf(lo, x[i]);
+                hi = fmaxf(hi, x[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = y[i];
-        }
-        // every read of the head before any write: the outputs may be the inputs
-        if constexpr (32 % L == 0) __syncwarp();
-        else __syncthreads();
-        float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
-        }
-#pragma unroll
-        for (int o = 1; o <= 2; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-        if (kind == 0) {
-            store8(q_out + t * ldq_out + h * D + d0, x);
-        } else if (live) {
+            for (int w = 1; w <= 2; w <<= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, w));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, w));
+            }
+            if (kind != 1 && kind != 2) continue;
             if (!(lo <= hi)) lo = hi = 0.0f;   // nothing but NaN
             const __half lo16 = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
             lo = __half2float(lo16);
@@ -110,16 +153,16 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
                 x[i] = __fadd_rn(lo, __fmul_rn(d, code));
             }
             uint8_t* rec = kv4_record(c, page, hk, R::bytes);
-            const int g = d0 / 32, u = (d0 / 8) % 4;
+            const int g = d0 / 32, n = (d0 / 8) % 4;
             if (kind == 1) {
-                *reinterpret_cast<uint32_t*>(rec + row * R::row + 4 * R::NG * u + 4 * g) = word;
+                *reinterpret_cast<uint32_t*>(rec + row * R::row + 4 * R::NG * n + 4 * g) = word;
             } else {
                 const int turn = ((row >> 1) & 1) * 4;
                 uint8_t* at = rec + R::v + row * R::row + 2 * g;
-                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * u) ^ turn)) = (uint16_t)word;
-                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * u + 1) ^ turn)) = (uint16_t)(word >> 16);
+                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * n) ^ turn)) = (uint16_t)word;
+                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * n + 1) ^ turn)) = (uint16_t)(word >> 16);
             }
-            if (u == 0) {
+            if (n == 0) {
                 __half* sc = reinterpret_cast<__half*>(rec + (kind == 1 ? R::kd : R::vd)) + row * R::GP + g;
                 sc[0] = d16;
                 sc[kKv4Page * R::GP] = lo16;
@@ -718,15 +761,20 @@ struct AppendArgs {
     int64_t ldkv_out;
 };
 
+template <class E, class O, int D, int ROPE>
+static cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t st) {
+    constexpr int HPW = 32 / (D / 8);
+    const int H = a.q ? a.H : 0, heads = H + 2 * a.c.n_head_kv;
+    // few tokens: CTAs of 8 warps with a turn each; many: a token's heads in one CTA, of no more warps than they fill
+    const int warps = std::min(8, (heads + HPW - 1) / HPW), hpc = a.T >= 148 ? heads : warps * HPW;
+    return fbk_launch_early(k_kv4_append<E, O, D, ROPE>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(32 * warps), 0, st, a.c,
+                            (const E*)a.q, (const E*)a.k, (const E*)a.v, a.ldq, a.ldkv, H, hpc, a.tok_seq, a.tok_pos, a.rot,
+                            a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
+}
 template <class E, class O, int D>
 static cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
-    const int H = a.q ? a.H : 0, heads = H + 2 * a.c.n_head_kv;
-    const int threads = D == 96 ? 192 : 256, per = threads / (D / 8);
-    // few tokens: a CTA a run of heads; many: a token's heads in one CTA
-    const int hpc = a.T >= 148 ? heads : per;
-    return fbk_launch_early(k_kv4_append<E, O, D>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(threads), 0, st, a.c,
-                      (const E*)a.q, (const E*)a.k, (const E*)a.v, a.ldq, a.ldkv, H, hpc, a.tok_seq, a.tok_pos, a.rot,
-                      a.neox, a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
+    return !a.neox ? launch_append_as<E, O, D, ROPE_PAIRS>(a, st)
+         : a.rot % 16 == 0 ? launch_append_as<E, O, D, ROPE_HALVES>(a, st) : launch_append_as<E, O, D, ROPE_ANY>(a, st);
 }
 template <class E, class O>
 static cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
