@@ -14,9 +14,12 @@ namespace fb {
 // consecutive dimensions (one 16-byte load of 16-bit values). What bounds it is
 // memory: a lane's loads of U heads are issued before anything else, under the
 // chain of position, page and rotation that the stores wait for, and the cos and
-// sin of its 8 dimensions serve all its heads. The partner of a rotated value is
-// in the same lane (pairs of neighbours) or comes by shuffle (halves, where half
-// the rotated dimensions are whole lanes; else by a second load). A group of 32
+// sin of its 8 dimensions serve all its heads. Where a lane's 8 dimensions are
+// rotated together or not at all, the partner of a value is in the same lane
+// (pairs of neighbours) or comes by shuffle (halves); other rotations load it
+// once more. Beside memory it is instructions: 64 registers keep four CTAs on an
+// SM, and a code is rounded by adding 1.5 2^23, whose low bits are then the code
+// (a multiply-add a code puts them together). A group of 32
 // values is four neighbouring lanes: its extremes by two shuffles, its codes one
 // 32-bit word of K or two 16-bit words of V a lane. Rotation and quantisation are
 // in 32 bits with every step rounded by itself (no fused multiply-add), so the
@@ -39,22 +42,29 @@ __device__ __forceinline__ void unpack8(const Raw8<E>& r, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = to_f32<E>(e[i]);
 }
 
+// The rotation of a lane's 8 dimensions: cos and sin, of 4 pairs or of 8 values (sin with its sign)
+template <int ROPE>
+struct Turn {
+    static constexpr int N = ROPE == ROPE_PAIRS ? 4 : 8;
+    float cs[N], sn[N];
+};
+
 template <class E, class O, int D, int ROPE>
-__global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_kv4_cache c, const E* q, const E* k,
-                                                    const E* v, int64_t ldq, int64_t ldkv, int H, int hpc,
-                                                    const int32_t* __restrict__ tok_seq,
-                                                    const int32_t* __restrict__ tok_pos, int rot,
-                                                    const float* __restrict__ rcos, const float* __restrict__ rsin,
-                                                    int n_rope, O* q_out, int64_t ldq_out, O* k_out, O* v_out,
-                                                    int64_t ldkv_out) {
+__global__ void __launch_bounds__(256, 4) k_kv4_append(const __grid_constant__ fbx_kv4_cache c, const E* q, const E* k,
+                                                       const E* v, int64_t ldq, int64_t ldkv, int H, int hpc,
+                                                       const int32_t* __restrict__ tok_seq,
+                                                       const int32_t* __restrict__ tok_pos, int rot, int neox,
+                                                       const float* __restrict__ rcos, const float* __restrict__ rsin,
+                                                       int n_rope, O* q_out, int64_t ldq_out, O* k_out, O* v_out,
+                                                       int64_t ldkv_out) {
     using R = Kv4Rec<D>;
     constexpr int L = D / 8, HPW = 32 / L;   // lanes a head, heads a warp (D = 96: 8 lanes idle)
-    constexpr int U = sizeof(E) == 4 ? 3 : 5;
+    constexpr int U = sizeof(E) == 4 ? 2 : 5;
     pdl_trigger();
     const int t = blockIdx.x, HKV = c.n_head_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int d0 = (lane % L) * 8, half = rot / 2;
     const int h0 = hpc * blockIdx.y, h1 = min(h0 + hpc, H + 2 * HKV), step = (int)blockDim.x / 32 * HPW;
-    const bool busy = lane < HPW * L;
+    const bool busy = lane < HPW * L, turns = d0 < rot;
     auto source = [&](int h) {
         return h < H ? q + t * ldq + h * D : h < H + HKV ? k + t * ldkv + (h - H) * D : v + t * ldkv + (h - H - HKV) * D;
     };
@@ -74,19 +84,26 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
         if (c.err && threadIdx.x == 0) atomicExch(c.err, 6);
         return;
     }
-    // cos and sin of this lane's 8 dimensions; x0 cos - x1 sin for the first of a pair, x1 cos + x0 sin for the second
-    float cs[8], sn[8];
+    // x0 cos - x1 sin for the first of a pair, x1 cos + x0 sin for the second
+    Turn<ROPE> turn;
     const float *cr = rcos + (size_t)pos * half, *sr = rsin + (size_t)pos * half;
+    if (ROPE == ROPE_ANY) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = d0 + i;
-        cs[i] = 1.0f;
-        sn[i] = 0.0f;
-        if (d < rot) {
-            const bool first = ROPE == ROPE_PAIRS ? i % 2 == 0 : d < half;
-            const int pair = ROPE == ROPE_PAIRS ? d / 2 : first ? d : d - half;
-            cs[i] = __ldg(cr + pair);
-            sn[i] = first ? -__ldg(sr + pair) : __ldg(sr + pair);
+        for (int i = 0; i < Turn<ROPE>::N; ++i) {
+            const int d = d0 + i;
+            const bool first = neox ? d < half : i % 2 == 0;
+            const int pair = neox ? (first ? d : d - half) : d / 2;
+            turn.cs[i] = d < rot ? __ldg(cr + pair) : 1.0f;
+            turn.sn[i] = d < rot ? (first ? -__ldg(sr + pair) : __ldg(sr + pair)) : 0.0f;
+        }
+    } else if (turns) {
+        const int at = ROPE == ROPE_PAIRS ? d0 / 2 : d0 < half ? d0 : d0 - half;
+        const float sign = ROPE == ROPE_HALVES && d0 < half ? -1.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < Turn<ROPE>::N; i += 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(cr + at + i)), b = __ldg(reinterpret_cast<const float4*>(sr + at + i));
+            turn.cs[i] = a.x; turn.cs[i + 1] = a.y; turn.cs[i + 2] = a.z; turn.cs[i + 3] = a.w;
+            turn.sn[i] = sign * b.x; turn.sn[i + 1] = sign * b.y; turn.sn[i + 2] = sign * b.z; turn.sn[i + 3] = sign * b.w;
         }
     }
     const int page = kv4_page(c, seq, pos / kKv4Page), row = pos % kKv4Page;
@@ -99,41 +116,46 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
             const int h = hb + u * step + warp * HPW + lane / L;
             const bool live = busy && h < h1;
             const int kind = !live ? 3 : h < H ? 0 : h < H + HKV ? 1 : 2;
-            const int hk = kind == 1 ? h - H : kind == 2 ? h - H - HKV : 0;
-            float x[8], o[8];
+            float x[8];
             if (live) unpack8<E>(raw[u], x);
             else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = 0.0f;
             }
             if (ROPE == ROPE_PAIRS) {
+                if (kind < 2 && turns) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
-            } else if (ROPE == ROPE_HALVES) {
-                const int from = lane + (d0 < half ? half / 8 : d0 < rot ? -(half / 8) : 0);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], from);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = d0 + i;
-                    o[i] = live && d < rot ? to_f32<E>(source(h)[d < half ? d + half : d - half]) : 0.0f;
+                    for (int i = 0; i < 8; i += 2) {
+                        const float a = x[i], b = x[i + 1], cs = turn.cs[i / 2], sn = turn.sn[i / 2];
+                        x[i] = __fsub_rn(__fmul_rn(a, cs), __fmul_rn(b, sn));
+                        x[i + 1] = __fadd_rn(__fmul_rn(a, sn), __fmul_rn(b, cs));
+                    }
                 }
-                __syncwarp();   // every read of the head before any write: the outputs may be the inputs
-            }
-            if (kind < 2) {
+            } else {
+                float o[8];
+                if (ROPE == ROPE_HALVES) {
+                    const int from = lane + (d0 < half ? half / 8 : turns ? -(half / 8) : 0);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (d0 + i < rot) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(o[i], sn[i]));
+                    for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], from);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int d = d0 + i, p = neox ? (d < half ? d + half : d - half) : d ^ 1;
+                        o[i] = live && d < rot ? to_f32<E>(source(h)[p]) : 0.0f;
+                    }
+                    __syncwarp();   // every read of the head before any write: the outputs may be the inputs
+                }
+                if (kind < 2 && turns) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (ROPE == ROPE_HALVES || d0 + i < rot)
+                            x[i] = __fadd_rn(__fmul_rn(x[i], turn.cs[i % Turn<ROPE>::N]), __fmul_rn(o[i], turn.sn[i % Turn<ROPE>::N]));
+                }
             }
             if (kind == 0) store8(q_out + t * ldq_out + h * D + d0, x);
             if (!__any_sync(0xffffffffu, kind == 1 || kind == 2)) continue;
-            float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                lo = fminf(lo, x[i]);
-                hi = fmaxf(hi, x[i]);
-            }
+            float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+            float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
 #pragma unroll
             for (int w = 1; w <= 2; w <<= 1) {
                 lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, w));
@@ -145,22 +167,31 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
             lo = __half2float(lo16);
             const __half d16 = __float2half_rn(__fmul_rn(__fsub_rn(fminf(fmaxf(hi, -65504.0f), 65504.0f), lo), 1.0f / 15.0f));
             const float d = __half2float(d16), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            constexpr float kRound = 12582912.0f;   // 0x4B400000: 0..15 added to it stand in its low bits, rounded to even
             uint32_t word = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float code = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], lo), inv)), 0.0f), 15.0f);
-                word |= (uint32_t)code << (4 * i);
-                x[i] = __fadd_rn(lo, __fmul_rn(d, code));
+                // clamped first (NaN to 0): the bounds are codes, so the rounding is that of the formula
+                const float code = __fadd_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], lo), inv), 0.0f), 15.0f), kRound);
+                word += __float_as_uint(code) << (4 * i);
+                x[i] = code;
             }
+            constexpr uint32_t kExtra = [] {
+                uint32_t e = 0;
+                for (int i = 0; i < 8; ++i) e += 0x4B400000u << (4 * i);
+                return e;
+            }();
+            word -= kExtra;
+            const int hk = kind == 1 ? h - H : h - H - HKV;
             uint8_t* rec = kv4_record(c, page, hk, R::bytes);
             const int g = d0 / 32, n = (d0 / 8) % 4;
             if (kind == 1) {
                 *reinterpret_cast<uint32_t*>(rec + row * R::row + 4 * R::NG * n + 4 * g) = word;
             } else {
-                const int turn = ((row >> 1) & 1) * 4;
+                const int swap = ((row >> 1) & 1) * 4;
                 uint8_t* at = rec + R::v + row * R::row + 2 * g;
-                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * n) ^ turn)) = (uint16_t)word;
-                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * n + 1) ^ turn)) = (uint16_t)(word >> 16);
+                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * n) ^ swap)) = (uint16_t)word;
+                *reinterpret_cast<uint16_t*>(at + 2 * R::NG * ((2 * n + 1) ^ swap)) = (uint16_t)(word >> 16);
             }
             if (n == 0) {
                 __half* sc = reinterpret_cast<__half*>(rec + (kind == 1 ? R::kd : R::vd)) + row * R::GP + g;
@@ -168,7 +199,11 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __grid_constant__ fbx_
                 sc[kKv4Page * R::GP] = lo16;
             }
             O* told = kind == 1 ? k_out : v_out;
-            if (told) store8(told + t * ldkv_out + hk * D + d0, x);
+            if (told) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(lo, __fmul_rn(d, __fsub_rn(x[i], kRound)));
+                store8(told + t * ldkv_out + hk * D + d0, x);
+            }
         }
     }
 }
@@ -769,12 +804,15 @@ static cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t st) {
     const int warps = std::min(8, (heads + HPW - 1) / HPW), hpc = a.T >= 148 ? heads : warps * HPW;
     return fbk_launch_early(k_kv4_append<E, O, D, ROPE>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(32 * warps), 0, st, a.c,
                             (const E*)a.q, (const E*)a.k, (const E*)a.v, a.ldq, a.ldkv, H, hpc, a.tok_seq, a.tok_pos, a.rot,
-                            a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
+                            a.neox, a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
 }
 template <class E, class O, int D>
 static cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
-    return !a.neox ? launch_append_as<E, O, D, ROPE_PAIRS>(a, st)
-         : a.rot % 16 == 0 ? launch_append_as<E, O, D, ROPE_HALVES>(a, st) : launch_append_as<E, O, D, ROPE_ANY>(a, st);
+    // whole lanes of 8 dimensions, and tables that can be read 16 bytes at a time
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.rcos) | reinterpret_cast<uintptr_t>(a.rsin)) & 15) == 0;
+    return wide && !a.neox && a.rot % 8 == 0 ? launch_append_as<E, O, D, ROPE_PAIRS>(a, st)
+         : wide && a.neox && a.rot % 16 == 0 ? launch_append_as<E, O, D, ROPE_HALVES>(a, st)
+                                             : launch_append_as<E, O, D, ROPE_ANY>(a, st);
 }
 template <class E, class O>
 static cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
