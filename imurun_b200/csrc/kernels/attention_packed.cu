@@ -7,9 +7,9 @@
 // A tile is 128 MMA rows: R = 128 / G consecutive rows of one sequence times the
 // G query heads of one kv head, so grouped heads share a tile whatever G is and
 // short prompts still fill it. A job is two neighbouring tiles (2 R rows), which
-// share every key and value tile. A CTA an SM takes jobs blockIdx, blockIdx +
-// gridDim, ..; every role goes from one job to the next by itself, so loads and
-// scores of the next job run under the last weights and the output of this one.
+// share every key and value tile. A CTA an SM takes its part of the jobs, longest
+// first; every role goes from one job to the next by itself, so loads and scores
+// of the next job run under the last weights and the output of this one.
 // Warps:
 //   0..3, 4..7  softmax of tile 0 and 1, a thread a row: scores from tensor
 //               memory, mask, row maximum, weights in 16 bits back over the
@@ -19,10 +19,11 @@
 //               warps form weights, the tensor core works for the other:
 //               S0 S1 | O0 S0 O1 S1 | O0 S0 O1 S1 ..
 //   9           TMA: Q, then K and V tiles of 128 rows through a ring;
-//   10, 11      tiles of V in which some row does not see some key: values that
+//   10          tiles of V in which some row does not see some key: values that
 //               are not finite are taken out before the product (0 x inf is
 //               NaN) and the job is marked; rows that do see them add them at
-//               the end.
+//               the end;
+//   11          looks up the jobs to come.
 // Tensor memory: S0 S1 (128 columns each, P in their first 64) O0 O1.
 //
 // The reference m_i is raised only when a tile's maximum exceeds it by 2^8 (the
@@ -44,10 +45,11 @@ namespace pk {
 constexpr int BK = 128, NS = 2;          // keys a tile, ring places of a V and a K tile
 constexpr int kHalf = 128 * 128;         // 128 rows x 64 values of 16 bits: one SW128 box
 constexpr int kSoft = 256, kThreads = kSoft + 128;
+constexpr int NJ = 4;                    // jobs looked up ahead
 constexpr float kRaise = 8.0f;
 
 enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + NS, B_P = B_S + 2, B_O = B_P + 4,
-       B_DRAIN = B_O + 2, B_COUNT };
+       B_DRAIN = B_O + 2, B_JOB, B_TAKEN = B_JOB + NJ, B_COUNT = B_TAKEN + NJ };
 
 template <int D>
 struct Smem {
@@ -55,7 +57,7 @@ struct Smem {
     static constexpr int tile = halves * kHalf;            // one Q, K or V tile
     static constexpr int place = 2 * tile;                 // V_j and, behind it, K_{j+1}
     static constexpr int ring = 2 * tile, bar = ring + NS * place;
-    static constexpr int bytes = bar + 8 * B_COUNT + 64 + 1024;
+    static constexpr int bytes = bar + 8 * B_COUNT + 32 + 16 * NJ + 1024;
 };
 
 struct Job {
@@ -83,32 +85,52 @@ struct Keys {
     __device__ __forceinline__ bool masked(int j) const { return j >= upper || j <= lower; }
 };
 
-// Job `tile`: sequences in order, each from its last (longest) job to its 32 sequences at a time, one a lane. s1 = 0 past the last one.
-__device__ __forceinline__ Job find_job(const int32_t* cu, int B, int n_rows, int tile, int rows) {
-    const int lane = threadIdx.x & 31;
-    for (int b = 0; b < B; b += 32) {
-        int a = 0, z = 0;
-        if (b + lane < B) {
-            a = min(max(__ldg(cu + b + lane), 0), n_rows);
-            z = min(max(__ldg(cu + b + lane + 1), a), n_rows);
+// The jobs of all sequences from the longest to the shortest: a sequence of n jobs has one on each of the levels 0 .. n - 1
+// (the level-th from its start, so the higher the longer), and they are counted from the highest level down, level by level,
+// sequence by sequence. Dealt out in turns that go to and fro over the CTAs, they leave every CTA about the same work
+// however the lengths differ. A whole warp looks them up, in ascending order; a lane keeps one of up to 32 sequences.
+struct Finder {
+    const int32_t* cu;
+    int B, n_rows, rows, level, before;   // jobs on the levels above
+    int a, z, n;                          // this lane's sequence, its jobs
+    __device__ __forceinline__ void sequence(int s) {
+        a = z = 0;
+        if (s < B) {
+            a = min(max(__ldg(cu + s), 0), n_rows);
+            z = min(max(__ldg(cu + s + 1), a), n_rows);
         }
-        const int n = (z - a + rows - 1) / rows;
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += up;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, sum > tile);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            const int r = a + (sum - 1 - tile) * rows;   // lane l: tile - (sum - n) counted from its end
-            return {__shfl_sync(0xffffffffu, a, l), __shfl_sync(0xffffffffu, z, l), __shfl_sync(0xffffffffu, r, l)};
-        }
-        tile -= __shfl_sync(0xffffffffu, sum, 31);
+        n = (z - a + rows - 1) / rows;
     }
-    return {0, 0, 0};
-}
+    __device__ __forceinline__ Finder(const int32_t* cu_, int B_, int n_rows_, int rows_) : cu(cu_), B(B_), n_rows(n_rows_), rows(rows_), before(0) {
+        const int lane = threadIdx.x & 31;
+        int most = 0;
+        for (int s = 0; s < B; s += 32) {
+            sequence(s + lane);
+            most = max(most, n);
+        }
+        level = __reduce_max_sync(0xffffffffu, most) - 1;
+    }
+    // Job u (not less than the last one); s1 = 0 past the last.
+    __device__ __forceinline__ Job find(int u) {
+        const int lane = threadIdx.x & 31;
+        for (; level >= 0; --level) {
+            int seen = before;
+            for (int s = 0; s < B; s += 32) {
+                if (B > 32) sequence(s + lane);
+                const unsigned here = __ballot_sync(0xffffffffu, n > level);
+                const int rank = u - seen;   // of the ones here
+                if (rank < __popc(here)) {
+                    const unsigned it = __ballot_sync(0xffffffffu, n > level && __popc(here & ((1u << lane) - 1)) == rank);
+                    const int l = __ffs(it) - 1, s0 = __shfl_sync(0xffffffffu, a, l);
+                    return {s0, __shfl_sync(0xffffffffu, z, l), s0 + level * rows};
+                }
+                seen += __popc(here);
+            }
+            before = seen;
+        }
+        return {0, 0, 0};
+    }
+};
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -150,6 +172,7 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile in
             break;
         }
 }
+__device__ __forceinline__ uint32_t ones(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }   // the low n bits
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -204,6 +227,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + M::bar + 8 * B_COUNT);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
     volatile int* s_odd = s_abort + 1;   // [4] jobs (counted from 1) in which values that are not finite were met
+    volatile int4* s_job = reinterpret_cast<volatile int4*>(s_tmem + 8);   // [NJ] jobs, with the kv head
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = A.R, G = A.G;
     pdl_trigger();
@@ -211,7 +235,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         *s_abort = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
         for (int i = 0; i < B_COUNT; ++i) {
-            mbar_init(&bar[i], i >= B_EMPTY && i < B_CLEAN ? 65 : i >= B_CLEAN && i < B_S ? 64 : i >= B_P && i < B_O ? 128 : 1);
+            mbar_init(&bar[i], i >= B_EMPTY && i < B_CLEAN ? 33 : i >= B_CLEAN && i < B_S ? 32 : i >= B_P && i < B_O ? 128 : i >= B_TAKEN ? 11 : 1);
         }
         mbar_fence_init();
     }
@@ -222,11 +246,14 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
-    // job n of this CTA; false past the last
+    // job n of this CTA, for a whole warp; false past the last
     auto find = [&](int n, Job* job, int* hk) {
-        const uint32_t id = blockIdx.x + (uint32_t)n * gridDim.x, unit = id / (uint32_t)A.HKV;
-        *hk = (int)(id - unit * A.HKV);
-        *job = find_job(A.cu, A.B, A.n_rows, (int)unit, 2 * R);
+        wait(&bar[B_JOB + n % NJ], (uint32_t)(n / NJ) & 1, s_abort);
+        const int4 w = {s_job[n % NJ].x, s_job[n % NJ].y, s_job[n % NJ].z, s_job[n % NJ].w};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[B_TAKEN + n % NJ]);
+        *job = {w.x, w.y, w.z};
+        *hk = w.w;
         return job->s1 != 0 && !__any_sync(0xffffffffu, *s_abort);
     };
     // ring place i, counted over all jobs; a job of n key tiles takes n + 1: K_0 alone, V_0 with K_1, .., V_{n-1} alone
@@ -334,19 +361,37 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         umma_commit_by(&bar[B_DRAIN], who);
         mbar_wait_bounded(&bar[B_DRAIN], 0);
         __syncwarp();
-    } else if (warp >= 10) {
+    } else if (warp == 11) {
+        // ---- what comes next: the others find it in shared memory, instead of each fetching the code that looks it up
+        Finder finder(A.cu, A.B, A.n_rows, 2 * R);
+        for (int n = 0;; ++n) {
+            if (n >= NJ) wait(&bar[B_TAKEN + n % NJ], (uint32_t)(n / NJ - 1) & 1, s_abort);
+            const uint32_t id = (uint32_t)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), unit = id / (uint32_t)A.HKV;
+            job = finder.find((int)unit);
+            if (__any_sync(0xffffffffu, *s_abort)) job.s1 = 0;
+            if (lane == 0) {
+                s_job[n % NJ].x = job.s0;
+                s_job[n % NJ].y = job.s1;
+                s_job[n % NJ].z = job.r0;
+                s_job[n % NJ].w = (int)(id - unit * A.HKV);
+                mbar_arrive(&bar[B_JOB + n % NJ]);
+            }
+            if (job.s1 == 0) break;
+        }
+        __syncwarp();
+    } else if (warp == 10) {
         // ---- values that are not finite
         int i = 0;
         for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
             for (int j = ks.j0; j <= ks.j1; ++j, ++i) {   // V_{j-1} in place i
-                // every place in its turn, and released by these warps too: a phase passed over could be taken for another
+                // every place in its turn, and released by this warp too: a phase passed over could be taken for another
                 full(i);
                 if (j > ks.j0 && ks.masked(j - 1)) {
                     uint4* t = reinterpret_cast<uint4*>(sm + M::ring + v_at(i));
                     bool odd = false;
-#pragma unroll 4
-                    for (int e = threadIdx.x - 320; e < M::tile / 16; e += 64) {
+#pragma unroll 8
+                    for (int e = lane; e < M::tile / 16; e += 32) {
                         uint4 w = t[e];
                         if (not_finite2<E>(w.x) | not_finite2<E>(w.y) | not_finite2<E>(w.z) | not_finite2<E>(w.w)) {
                             uint32_t* u = reinterpret_cast<uint32_t*>(&w);
@@ -400,10 +445,12 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
             if (masked) {
                 const int top = i - kb, bottom = A.window > 0 ? top - A.window : -1;   // keys bottom < e <= top are seen
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t seen = ones(top + 1 - 32 * c) & ~ones(bottom + 1 - 32 * c);
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        if (32 * c + e > top || 32 * c + e <= bottom) s[c][e] = -INFINITY;
+                        if (!(seen >> e & 1)) s[c][e] = -INFINITY;
+                }
             }
             float2 sum0, sum1;
             uint32_t u[32];
