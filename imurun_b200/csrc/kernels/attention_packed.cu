@@ -56,7 +56,7 @@ struct Smem {
     static constexpr int halves = (D + 63) / 64;
     static constexpr int tile = halves * kHalf;            // one Q, K or V tile
     static constexpr int place = 2 * tile;                 // V_j and, behind it, K_{j+1}
-    static constexpr int ring = 2 * tile, bar = ring + NS * place;
+    static constexpr int ring = 2 * tile, out = ring + NS * place, bar = out + 8 * 4096;   // out: 32 rows x 128 bytes a warp
     static constexpr int bytes = bar + 8 * B_COUNT + 32 + 16 * NJ + 1024;
 };
 
@@ -158,11 +158,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
     return *reinterpret_cast<float2*>(&r);
 }
-__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
 // Waits of the roles. A wait that runs out (some 10 ms at least) marks the CTA: every role then goes through its loops without
 // waiting, on whatever lies in shared and tensor memory, and the CTA ends.
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -195,6 +190,19 @@ template <class E> __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
     else return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
 }
 
+// two values of a type
+template <class E> struct Pair;
+template <> struct Pair<__half> {
+    using type = __half2;
+    static __device__ __forceinline__ type of(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+    static __device__ __forceinline__ type zero() { return of(0); }
+};
+template <> struct Pair<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    static __device__ __forceinline__ type of(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ type zero() { return of(0); }
+};
+
 struct Args {
     const int32_t* cu;
     int B, n_rows, HKV, G, R;
@@ -203,7 +211,6 @@ struct Args {
     int window;
     void* out;
     int64_t ldo;
-    int wide;       // rows of out on 32-byte boundaries
     const void* v;  // for rows that see values which are not finite
     int64_t ldkv;
 };
@@ -388,19 +395,30 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                 // every place in its turn, and released by this warp too: a phase passed over could be taken for another
                 full(i);
                 if (j > ks.j0 && ks.masked(j - 1)) {
+                    // 0 x each of them, summed: NaN where one is not finite
                     uint4* t = reinterpret_cast<uint4*>(sm + M::ring + v_at(i));
-                    bool odd = false;
+                    typename Pair<E>::type acc[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[k] = Pair<E>::zero();
 #pragma unroll 8
                     for (int e = lane; e < M::tile / 16; e += 32) {
-                        uint4 w = t[e];
-                        if (not_finite2<E>(w.x) | not_finite2<E>(w.y) | not_finite2<E>(w.z) | not_finite2<E>(w.w)) {
+                        const uint4 w = t[e];
+                        acc[0] = __hfma2(Pair<E>::of(w.x), Pair<E>::zero(), acc[0]);
+                        acc[1] = __hfma2(Pair<E>::of(w.y), Pair<E>::zero(), acc[1]);
+                        acc[2] = __hfma2(Pair<E>::of(w.z), Pair<E>::zero(), acc[2]);
+                        acc[3] = __hfma2(Pair<E>::of(w.w), Pair<E>::zero(), acc[3]);
+                    }
+                    const auto all = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
+                    if (!__hbeq2(all, all)) {
+#pragma unroll 1
+                        for (int e = lane; e < M::tile / 16; e += 32) {
+                            uint4 w = t[e];
                             uint32_t* u = reinterpret_cast<uint32_t*>(&w);
                             for (int k = 0; k < 4; ++k) u[k] &= ~((not_finite2<E>(u[k]) >> 15) * 0xFFFFu);
                             t[e] = w;
-                            odd = true;
                         }
+                        s_odd[q & 3] = q + 1;
                     }
-                    if (odd) s_odd[q & 3] = q + 1;
                     fence_async_smem();
                     mbar_arrive(&bar[B_CLEAN + i % NS]);
                 }
@@ -516,36 +534,42 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         tc_fence_after();
         const bool odd = s_odd[q & 3] == q + 1;
         const float inv = 1.0f / l;
-        E* dst = static_cast<E*>(A.out) + (int64_t)(job.s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D;
+        // 64 columns of the warp's 32 rows at a time by way of shared memory, so that a store instruction writes whole lines
+        const uint64_t dst = live ? reinterpret_cast<uint64_t>(static_cast<E*>(A.out) + (int64_t)(job.s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D) : 0;
         const E* v = static_cast<const E*>(A.v) + (int64_t)job.s0 * A.ldkv + (int64_t)hk * D;
-#pragma unroll 1   // once a job: little code rather than many instruction fetches
-        for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tmem_ld32(to + 32 * c, o);
-            tmem_ld_wait();
-            if (live) {
+        uint8_t* stage = sm + M::out + (threadIdx.x >> 5) * 4096;
+#pragma unroll 1   // run once a job: little code rather than many instruction fetches
+        for (int c = 0; c < D; c += 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (c + 32 * h >= D) break;
+                float o[32];
+                tmem_ld32(to + c + 32 * h, o);
+                tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] *= inv;
-                if (odd) {
+                if (odd && live) {
                     for (int k = A.window > 0 ? max(0, i - A.window + 1) : 0; k <= i; ++k)
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            const float y = to_f32<E>(v[k * A.ldkv + 32 * c + e]);
+                            const float y = to_f32<E>(v[k * A.ldkv + c + 32 * h + e]);
                             if (!(fabsf(y) < INFINITY)) o[e] += y;
                         }
                 }
-                uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = pack2<E>(o[2 * e], o[2 * e + 1]);
-                if (A.wide) {   // whole sectors
-                    store32(dst + 32 * c, w);
-                    store32(dst + 32 * c + 16, w + 8);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<uint4*>(dst + 32 * c + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
-                }
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * h + e) ^ (lane & 7)) << 4)) =
+                        make_uint4(pack2<E>(o[8 * e], o[8 * e + 1]), pack2<E>(o[8 * e + 2], o[8 * e + 3]),
+                                   pack2<E>(o[8 * e + 4], o[8 * e + 5]), pack2<E>(o[8 * e + 6], o[8 * e + 7]));
             }
+            __syncwarp();
+#pragma unroll
+            for (int r = lane >> 3; r < 32; r += 4) {   // 8 lanes a row
+                const uint64_t at = __shfl_sync(0xffffffffu, dst, r);
+                const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                if (at && c + 8 * (lane & 7) < D) *reinterpret_cast<uint4*>(at + 2 * c + 16 * (lane & 7)) = w;
+            }
+            __syncwarp();
         }
         tc_fence_before();   // O is read before the next job's first weights are handed over
         }
@@ -608,7 +632,7 @@ cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void*
     }
     constexpr float kLog2e = 1.4426950408889634f;
     pk::Args a{cu, B, n_rows, HKV, G, R, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
-               window, out, ldo, (reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * 2)) % 32 == 0, v, ldkv};
+               window, out, ldo, v, ldkv};
     const int64_t jobs = (n_rows / (2 * R) + std::min<int64_t>(B, n_rows)) * HKV;
     if (jobs > INT_MAX / 2) return cudaErrorInvalidValue;
     return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)std::min<int64_t>(jobs, 148)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
