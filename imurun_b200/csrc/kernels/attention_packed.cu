@@ -635,7 +635,7 @@ cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void*
                window, out, ldo, v, ldkv};
     const int64_t jobs = (n_rows / (2 * R) + std::min<int64_t>(B, n_rows)) * HKV;
     if (jobs > INT_MAX / 2) return cudaErrorInvalidValue;
-    return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)std::min<int64_t>(jobs, 148)), dim3(pk::kThreads), (size_t)M::bytes, st, qm,
+    return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)std::min<int64_t>(jobs, 148)), dim3(pk::kThreads), (size_t)M::bytes, st, 1, qm,
                       km, vm, a);
 }
 

@@ -1,5 +1,7 @@
 // kv4.cu — the paged cache held in 4 bits: append with RoPE, and attention of
 // single tokens over it.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -247,6 +249,7 @@ __global__ void __launch_bounds__(256, 4) k_kv4_append(const __grid_constant__ f
 // be the larger part of the error; for bf16, whose own step is 8 times as
 // wide, p is rounded first and codes stay 0..15.
 constexpr int kAtWarps = 8, kSlots = 2;
+constexpr int kMaxCluster = 8;
 constexpr float kNoRef = -1e30f;   // before the first key: finite, so that a key outside (-inf) weighs 0 against it
 
 // key of row r of the 16-row operand tiles
@@ -333,7 +336,8 @@ struct AtArgs {
     int window;
     void* out;
     int64_t ldo;
-    float* part;   // [token][kv head and run of 8 heads][split]: ref[8], sum[8], O[8][D]; null: one split, straight to out
+    float* part;   // [token][kv head and run of 8 heads][split]: ref[8], sum[8], O[8][D], for the join; null: the splits are
+                   // one cluster, which joins them through its shared memory
 };
 
 template <int D>
@@ -347,7 +351,8 @@ struct AtSmem {
     static constexpr int bytes = bar + 8 * kAtWarps * kSlots;
     // at the end, over the rings: [warps][8] ref, [warps][8] sum, [warps][8][D + 4] O
     static constexpr int ml = 0, o = kAtWarps * 8 * 8;
-    static_assert(o + kAtWarps * 8 * (D + 4) * 4 <= q, "merge area");
+    static constexpr int part = o + kAtWarps * 8 * (D + 4) * 4;   // and of the CTA, as AtArgs::part
+    static_assert(part + (16 + 8 * D) * 4 <= q, "merge area");
 };
 
 // how the weights of an element type go into the products with V (see above)
@@ -685,7 +690,8 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         }
     }
     __syncthreads();
-    float* part = A.part ? A.part + ((size_t)(tok * gridDim.y + blockIdx.y) * S + blockIdx.x) * (16 + 8 * D) : nullptr;
+    float* part = reinterpret_cast<float*>(sm + M::part);
+    if (A.part) part = A.part + ((size_t)(tok * gridDim.y + blockIdx.y) * S + blockIdx.x) * (16 + 8 * D);
     for (int i = threadIdx.x; i < gn * (D / 4); i += 32 * kAtWarps) {
         const int h = i / (D / 4), d = i % (D / 4) * 4;
         float top = -INFINITY, l = 0.0f;
@@ -702,7 +708,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             x.z = fmaf(f, y.z, x.z);
             x.w = fmaf(f, y.w, x.w);
         }
-        if (part) {
+        if (A.part || S > 1) {
             if (d == 0) {
                 part[h] = top;
                 part[8 + h] = l;
@@ -713,6 +719,36 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             store4(static_cast<E*>(A.out) + tok * A.ldo + (int64_t)(hk * G + g0 + h) * D + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
         }
     }
+    if (A.part || S == 1) return;
+    // ---- one cluster: every CTA joins its part of the outputs
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = threadIdx.x + 32 * kAtWarps * blockIdx.x; i < gn * (D / 4); i += 32 * kAtWarps * S) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float tops[kMaxCluster], top = -INFINITY, l = 0.0f;
+        float4 y[kMaxCluster], x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int s = 0; s < kMaxCluster; ++s) {
+            const float* p = cluster.map_shared_rank(part, s < S ? s : 0);
+            tops[s] = s < S ? p[h] : -INFINITY;
+            y[s] = *reinterpret_cast<const float4*>(p + 16 + h * D + d);
+            top = fmaxf(top, tops[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < kMaxCluster; ++s) {
+            if (s >= S) break;
+            const float f = at_ex2(tops[s] - top);
+            l = fmaf(f, cluster.map_shared_rank(part, s)[8 + h], l);
+            x.x = fmaf(f, y[s].x, x.x);
+            x.y = fmaf(f, y[s].y, x.y);
+            x.z = fmaf(f, y[s].z, x.z);
+            x.w = fmaf(f, y[s].w, x.w);
+        }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // NaN stays NaN
+        store4(static_cast<E*>(A.out) + tok * A.ldo + (int64_t)(hk * G + g0 + h) * D + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    }
+    cluster.sync();   // nobody's shared memory goes while it is read
 }
 
 // The splits of one (token, query head) joined: out = sum_s 2^(ref_s - top) O_s / sum_s 2^(ref_s - top) sum_s.
@@ -802,7 +838,7 @@ static cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t st) {
     const int H = a.q ? a.H : 0, heads = H + 2 * a.c.n_head_kv;
     // few tokens: CTAs of 8 warps with a turn each; many: a token's heads in one CTA, of no more warps than they fill
     const int warps = std::min(8, (heads + HPW - 1) / HPW), hpc = a.T >= 148 ? heads : warps * HPW;
-    return fbk_launch_early(k_kv4_append<E, O, D, ROPE>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(32 * warps), 0, st, a.c,
+    return fbk_launch_early(k_kv4_append<E, O, D, ROPE>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(32 * warps), 0, st, 1, a.c,
                             (const E*)a.q, (const E*)a.k, (const E*)a.v, a.ldq, a.ldkv, H, hpc, a.tok_seq, a.tok_pos, a.rot,
                             a.neox, a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
 }
@@ -825,11 +861,17 @@ static cudaError_t append_o(const AppendArgs& a, int out_type, cudaStream_t st) 
          : out_type == T_F16 ? append_d<E, __half>(a, st) : append_d<E, __nv_bfloat16>(a, st);
 }
 
-// CTAs a token and kv head: as many as two an SM give, each warp of them with a step or more
+// CTAs a token and kv head: as many as two an SM give, each warp of them with a step or more. Up to eight are one cluster (2,
+// 4 or 8 of them) and one launch; more leave partial results for a second one.
 static int at_splits(int T, int H, int HKV, int max_keys) {
+    constexpr int64_t kRoom = 2 * 148;
     const int64_t pairs = (int64_t)T * HKV * ((H / HKV + 7) / 8);
     const int pages = (max_keys - 1) / kKv4Page + 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * 148 / pairs, (pages + 2 * kAtWarps - 1) / (2 * kAtWarps)));
+    const int S = (int)std::max<int64_t>(1, std::min<int64_t>(kRoom / pairs, (pages + 2 * kAtWarps - 1) / (2 * kAtWarps)));
+    if (S > kMaxCluster) return S;
+    int c = 1;
+    while (c < S) c *= 2;
+    return c > S && pairs * c > kRoom ? c / 2 : c;
 }
 
 template <class E, int D>
@@ -845,9 +887,10 @@ static cudaError_t launch_kv4_attention(const AtArgs& a, int T, int S, cudaStrea
         __atomic_fetch_or(&set, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
     }
     const int HKV = a.c.n_head_kv;
-    e = fbk_launch_early(k_kv4_attention<E, D>, dim3(S, HKV * ((a.H / HKV + 7) / 8), T), dim3(32 * kAtWarps), (size_t)M::bytes, st, a);
+    const dim3 grid(S, HKV * ((a.H / HKV + 7) / 8), T);
+    e = fbk_launch_early(k_kv4_attention<E, D>, grid, dim3(32 * kAtWarps), (size_t)M::bytes, st, a.part ? 1 : S, a);
     if (e != cudaSuccess || !a.part) return e;
-    return fbk_launch_early(k_kv4_join<E, D>, dim3(a.H, T), dim3(32 * kJoinWarps), 0, st, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
+    return fbk_launch_early(k_kv4_join<E, D>, dim3(a.H, T), dim3(32 * kJoinWarps), 0, st, 1, (const float*)a.part, S, a.H, HKV, a.tok_pos, (E*)a.out, a.ldo);
 }
 template <class E>
 static cudaError_t kv4_attention_d(const AtArgs& a, int T, int S, cudaStream_t st) {
@@ -871,7 +914,7 @@ extern "C" int fbk_kv4_append(const fbx_kv4_cache& c, int type, const void* q, c
 
 extern "C" size_t fbk_kv4_attention_workspace(int T, int H, int HKV, int D, int max_keys) {
     const int S = at_splits(T, H, HKV, max_keys);
-    return S > 1 ? (size_t)T * HKV * ((H / HKV + 7) / 8) * S * (16 + 8 * D) * sizeof(float) : 0;
+    return S > kMaxCluster ? (size_t)T * HKV * ((H / HKV + 7) / 8) * S * (16 + 8 * D) * sizeof(float) : 0;
 }
 
 extern "C" int fbk_kv4_attention(const fbx_kv4_cache& c, int type, const void* q, int64_t ldq, int T, int H,
@@ -880,7 +923,7 @@ extern "C" int fbk_kv4_attention(const fbx_kv4_cache& c, int type, const void* q
     // a window bounds the keys too (it may begin inside a page); never more splits than the workspace was sized for
     const int keys = window > 0 ? (int)std::min<int64_t>(max_keys, (int64_t)window + kKv4Page) : max_keys;
     const int S = at_splits(T, H, c.n_head_kv, keys);
-    const AtArgs a{c, q, ldq, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, S > 1 ? (float*)ws : nullptr};
+    const AtArgs a{c, q, ldq, H, tok_seq, tok_pos, scale, softcap, window, out, ldo, S > kMaxCluster ? (float*)ws : nullptr};
     return (int)(type == T_F32 ? kv4_attention_d<float>(a, T, S, st)
                : type == T_F16 ? kv4_attention_d<__half>(a, T, S, st) : kv4_attention_d<__nv_bfloat16>(a, T, S, st));
 }

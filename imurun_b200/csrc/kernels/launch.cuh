@@ -34,20 +34,30 @@ static inline cudaError_t fbk_launch(void (*kern)(KArgs...), dim3 grid, dim3 blo
 
 // The same, with programmatic dependent launch also where no engine has turned
 // it on (entry points on device buffers; FISH_NO_PDL=1 turns it off). The
-// kernel keeps the rule above whatever runs before it on the stream.
+// kernel keeps the rule above whatever runs before it on the stream. cluster:
+// CTAs of a cluster, along x.
 template <class... KArgs, class... Args>
 static inline cudaError_t fbk_launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                                           Args&&... args) {
+                                           int cluster, Args&&... args) {
     static const bool off = getenv("FISH_NO_PDL") && atoi(getenv("FISH_NO_PDL"));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (!off) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = off ? 0 : 1;
+    cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
