@@ -379,9 +379,14 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     if (lane < kSlots) mbar_init(&bar[lane], 2);
     mbar_fence_init();
     pdl_wait();
-    const int pos = A.tok_pos[tok];
+    // everything that depends on nothing else at once: the token's place and this warp's query head
+    const int pos = __ldg(A.tok_pos + tok), seq = __ldg(A.tok_seq + tok);
+    static_assert(kAtWarps == 8, "a warp a query head");
+    float x[NG];
+#pragma unroll
+    for (int e = 0; e < NG; ++e)
+        x[e] = warp < gn ? to_f32<E>(static_cast<const E*>(A.q)[tok * A.ldq + (int64_t)(hk * G + g0 + warp) * D + 32 * e + lane]) : 0.0f;
     if (pos < 0) return;   // padding
-    const int seq = A.tok_seq[tok];
     const bool known = seq >= 0 && seq < c.n_seqs;
     if (!known && c.err && threadIdx.x == 0) atomicExch(c.err, 6);
 
@@ -413,40 +418,41 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     };
     for (int j = 0; j < kSlots && j < n; ++j) issue(j, ids);
 
-    // the queries: a warp brings head g0 + w to at most 2 in size, as f16 parts, dimensions 32 e + 8 t + n in the order
+    // the queries: warp w brings head g0 + w to at most 2 in size, as f16 parts, dimensions 32 e + 8 t + n in the order
     // (0, 4), (1, 5), (2, 6), (3, 7) of n that a lane's operands have
     constexpr int QS = AtSmem<D>::q_row;
-    for (int w = warp; w < 8; w += kAtWarps) {
-        float x[NG], top = 0.0f;
+    {
+        float top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < NG; ++e) {
-            x[e] = w < gn ? to_f32<E>(static_cast<const E*>(A.q)[tok * A.ldq + (int64_t)(hk * G + g0 + w) * D + 32 * e + lane]) : 0.0f;
-            top = fmaxf(top, fabsf(x[e]));
-        }
+        for (int e = 0; e < NG; ++e) top = fmaxf(top, fabsf(x[e]));
         top = warp_max(top);
         int ex = (int)(__float_as_uint(top) >> 23) - 127;
         if (ex == 128 || top == 0.0f) ex = 0;
         ex = min(max(ex, -120), 120);
         const float down = __int_as_float((127 - ex) << 23);
-        __half* sq = reinterpret_cast<__half*>(sm + M::q) + w * QS + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
-        __half* ss = reinterpret_cast<__half*>(sm + M::qs);
+        __half* sq = reinterpret_cast<__half*>(sm + M::q) + warp * QS + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
+        __half* ss = reinterpret_cast<__half*>(sm + M::qs) + warp * 4;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
-            const float y = x[e] * down;
-            const float z = SUB && lane % 2 == 0 ? 16.0f * y : y;   // a code of an even dimension is 2^-4 less
+            sum[e] = x[e] * down;
+            const float z = SUB && lane % 2 == 0 ? 16.0f * sum[e] : sum[e];   // a code of an even dimension is 2^-4 less
             const __half hi = __float2half_rn(z);
             sq[32 * e] = hi;
             if (PL == 2) sq[8 * QS + 32 * e] = __float2half_rn(z - __half2float(hi));
-            const float sum = warp_sum(y);
-            if (lane == 0) {
-                const __half h = __float2half_rn(sum);
-                ss[w * 4 + e] = h;
-                ss[32 + w * 4 + e] = __float2half_rn(sum - __half2float(h));
-            }
         }
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+            for (int e = 0; e < NG; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], w);
         if (lane == 0) {
-            for (int e = NG; e < 4; ++e) ss[w * 4 + e] = ss[32 + w * 4 + e] = __float2half_rn(0.0f);
-            reinterpret_cast<float*>(sm + M::ex)[w] = __int_as_float((127 + ex) << 23);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const __half h = __float2half_rn(sum[e]);
+                ss[e] = h;
+                ss[32 + e] = __float2half_rn(sum[e] - __half2float(h));
+            }
+            reinterpret_cast<float*>(sm + M::ex)[warp] = __int_as_float((127 + ex) << 23);
         }
     }
     __syncthreads();
