@@ -605,3 +605,169 @@ def test_calls_allocate_nothing_and_refuse_foreign_memory(env):
     assert torch.cuda.mem_get_info()[0] == free
     assert call(addr) == -1   # a host array
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ larger calls
+
+def filled(env, lens, HKV, D, seed, spread=1.0):
+    """A cache filled by fbx_kv4_append without rotation, and the values that it holds, K, V and V's d [rows][HKV][D] f64."""
+    lib, torch, _ = env
+    c = Cache(env, lens, HKV, D, seed=seed)
+    torch.manual_seed(seed)
+    seq = np.concatenate([np.full(n, s) for s, n in enumerate(lens)])
+    pos = np.concatenate([np.arange(n) for n in lens])
+    x = torch.randn((len(seq), 2 * HKV * D), device="cuda") * spread
+    x[:, HKV * D:] += 0.25
+    cos, sin = (dev(torch, a) for a in tables(max(lens), 2))
+    k, v = (torch.empty((len(seq), HKV * D), device="cuda") for _ in range(2))
+    dseq, dpos = dev(torch, seq.astype(np.int32)), dev(torch, pos.astype(np.int32))
+    ld = x.shape[1]
+    assert lib.fbx_kv4_append(c.handle, 0, None, x.data_ptr(), x.data_ptr() + 4 * HKV * D, 0, ld, len(seq), 0, dseq.data_ptr(),
+                              dpos.data_ptr(), 0, 0, cos.data_ptr(), sin.data_ptr(), max(lens), 0, None, 0, k.data_ptr(),
+                              v.data_ptr(), HKV * D, None) == 0
+    torch.cuda.synchronize()
+    y = x[:, HKV * D:].view(-1, HKV, D // 32, 32)
+    d = ((y.amax(-1) - y.amin(-1)) / 15 + 1e-3).double().repeat_interleave(32, -1)   # no less than the d that is stored
+    return c, k.view(-1, HKV, D).double(), v.view(-1, HKV, D).double(), d, np.concatenate([[0], np.cumsum(lens)])
+
+
+@pytest.mark.parametrize("t,H,HKV,D,lens,window", [
+    ("bf16", 8, 1, 128, [6001, 2900, 17], 0),          # more than eight splits: a second launch joins them
+    ("f32", 24, 2, 64, [1000] * 19 + [3], 0),          # heads in two runs of eight, clusters
+    ("f16", 4, 4, 96, [700, 260, 130, 513], 0),
+    ("f16", 16, 8, 128, [300, 40, 2000, 5], 64),
+    ("f32", 9, 1, 128, [4000], 2500),
+    ("bf16", 6, 2, 128, list(range(1, 180)), 0),       # many tokens, one CTA each
+])
+def test_attention_over_long_caches(env, t, H, HKV, D, lens, window):
+    lib, torch, _ = env
+    c, k, v, d, at = filled(env, lens, HKV, D, seed=H + D)
+    T, G, scale = len(lens), H // HKV, 1.3 / np.sqrt(D)
+    torch.manual_seed(1)
+    q = torch.randn((T, H * D), device="cuda").to(dtype(torch, t))
+    out = attention(env, c, t, q, H, list(range(T)), [n - 1 for n in lens], max(lens), scale, 0.0, window)
+    assert int(c.err) == 0
+    for s, n in enumerate(lens):
+        a = max(0, n - window) if window else 0
+        rows = slice(at[s] + a, at[s] + n)
+        x = q[s].view(HKV, G, D).double()
+        kk, vv, dd = (y[rows].transpose(0, 1) for y in (k, v, d))
+        w = torch.softmax(x @ kk.transpose(1, 2) * scale, -1)
+        want, mean, coarse = (z.reshape(H, D).cpu().numpy() for z in (w @ vv, w @ vv.abs(), w @ dd))
+        ext = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(H).cpu().numpy() * scale
+        near(host(out[s]).reshape(H, D), want, (mean, ext, coarse), t)
+
+
+def test_attention_tokens_of_one_sequence(env):
+    """Several tokens of a sequence in one call, as a draft's verification has them: each sees its own past, and each row
+    has the bits that it has alone with the same bound."""
+    lib, torch, _ = env
+    H, HKV, D, n = 8, 2, 128, 333
+    c, k, v, d, _ = filled(env, [n], HKV, D, seed=3)
+    q = torch.randn((6, H * D), device="cuda")
+    pos = [n - 1, 100, n - 1, 0, 15, 16]
+    out = attention(env, c, "f32", q, H, [0] * 6, pos, n, 0.1)
+    for i, p in enumerate(pos):
+        x = q[i].view(HKV, 4, D).double()
+        kk, vv, dd = (y[:p + 1].transpose(0, 1) for y in (k, v, d))
+        w = torch.softmax(x @ kk.transpose(1, 2) * 0.1, -1)
+        want, mean, coarse = (z.reshape(H, D).cpu().numpy() for z in (w @ vv, w @ vv.abs(), w @ dd))
+        ext = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(H).cpu().numpy() * 0.1
+        near(host(out[i]).reshape(H, D), want, (mean, ext, coarse), "f32")
+    again = attention(env, c, "f32", q, H, [0] * 6, pos, n, 0.1)
+    assert torch.equal(out, again)
+
+
+def test_attention_keeps_nan_queries(env):
+    """A NaN or infinite query gives NaN in its own head and nowhere else."""
+    lib, torch, _ = env
+    H, HKV, D = 8, 2, 64
+    c, *_ = filled(env, [200], HKV, D, seed=4)
+    for t in ("f32", "f16", "bf16"):
+        q = torch.randn((1, H * D), device="cuda").to(dtype(torch, t))
+        clean = attention(env, c, t, q, H, [0], [199], 200, 0.1)
+        q[0, 2 * D + 5], q[0, 7 * D] = float("nan"), float("inf")
+        out = attention(env, c, t, q, H, [0], [199], 200, 0.1).view(H, D)
+        assert bool(torch.isnan(out[2]).all()) and bool(torch.isnan(out[7]).all())
+        keep = [0, 1, 3, 4, 5, 6]
+        assert torch.equal(out[keep], clean.view(H, D)[keep])
+
+
+def packed64(torch, q, k, v, lens, H, HKV, D, scale, softcap, window):
+    """packed_reference on the device, for longer sequences."""
+    G, at = H // HKV, 0
+    want, mean = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    ext = torch.zeros((len(q), H), dtype=torch.float64, device="cuda")
+    for n in lens:
+        if not n:
+            continue
+        x, kk, vv = (y[at:at + n].double().view(n, -1, D).transpose(0, 1) for y in (q, k, v))
+        kk, vv = kk.repeat_interleave(G, 0), vv.repeat_interleave(G, 0)
+        s = x @ kk.transpose(1, 2) * scale
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        i = torch.arange(n, device="cuda")
+        off = i[None, :] > i[:, None]
+        if window:
+            off |= i[None, :] <= i[:, None] - window
+        w = torch.softmax(s.masked_fill(off, -float("inf")), -1)
+        want[at:at + n] = (w @ vv).transpose(0, 1).reshape(n, -1)
+        mean[at:at + n] = (w @ vv.abs()).transpose(0, 1).reshape(n, -1)
+        ext[at:at + n] = ((x.abs() @ kk.abs().transpose(1, 2)).masked_fill(off, 0).amax(-1) * scale).T
+        at += n
+    return want.cpu().numpy(), mean.cpu().numpy(), ext.cpu().numpy()
+
+
+def many(seed, count, low, high):
+    r = np.random.default_rng(seed)
+    return [int(n) for n in r.integers(low, high, count)]
+
+
+@pytest.mark.parametrize("t,lens,H,HKV,D,softcap,window", [
+    ("bf16", many(1, 40, 0, 700), 16, 4, 128, 0.0, 0),       # several jobs a CTA
+    ("f16", many(2, 100, 0, 90), 5, 1, 64, 0.0, 0),          # more sequences than a warp has lanes
+    ("f16", [0] * 50 + [333] + [0] * 40 + [1, 129], 28, 4, 96, 0.0, 0),
+    ("bf16", [150, 3], 128, 1, 64, 0.0, 0),                  # the widest group: a row a tile
+    ("f16", [40, 130], 50, 1, 128, 0.0, 0),
+    ("bf16", [5000], 2, 1, 128, 0.0, 300),
+    ("f16", many(3, 9, 100, 1500), 6, 2, 64, 15.0, 500),
+    ("bf16", [3001, 17], 7, 1, 128, 0.0, 0),
+])
+def test_packed_many_jobs(env, t, lens, H, HKV, D, softcap, window):
+    lib, torch, _ = env
+    torch.manual_seed(sum(lens))
+    N = sum(lens)
+    q, k, v = (torch.randn((N, h * D), device="cuda").to(dtype(torch, t)) for h in (H, HKV, HKV))
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    scale = 1.5 / np.sqrt(D)
+    out = packed(env, t, q, k, v, cu, H, HKV, D, scale, softcap, window)
+    check_packed(host(out), *packed64(torch, q, k, v, lens, H, HKV, D, scale, softcap, window), H, D, t, softcap, N)
+    assert torch.equal(out, packed(env, t, q, k, v, cu, H, HKV, D, scale, softcap, window))
+
+
+def test_packed_rising_scores(env):
+    """Scores that grow by far more than the reference's slack from tile to tile: the accumulator is rescaled all the way."""
+    lib, torch, _ = env
+    H, HKV, D, N = 4, 2, 128, 1400
+    torch.manual_seed(5)
+    q = torch.ones((N, H * D), device="cuda").bfloat16()
+    k = (torch.randn((N, HKV * D), device="cuda") * 0.05 + torch.arange(N, device="cuda")[:, None] * 0.01).bfloat16()
+    v = torch.randn((N, HKV * D), device="cuda").bfloat16()
+    cu = dev(torch, np.array([0, N], np.int32))
+    for scale in (0.05, 1.0):
+        out = packed(env, "bf16", q, k, v, cu, H, HKV, D, scale)
+        check_packed(host(out), *packed64(torch, q, k, v, [N], H, HKV, D, scale, 0.0, 0), H, D, "bf16", 0.0, N)
+
+
+def test_packed_rows_past_32_bits(env):
+    """Rows so wide that their byte offsets pass 32 bits."""
+    lib, torch, _ = env
+    H, HKV, D, N, ld = 2, 1, 128, 300, 1 << 23   # 16 MiB a row
+    torch.manual_seed(6)
+    wide = torch.empty((N, ld), dtype=torch.float16, device="cuda")
+    wide[:, :4 * D] = torch.randn((N, 4 * D), device="cuda").half()
+    q, k, v = wide[:, :H * D], wide[:, H * D:3 * D], wide[:, 3 * D:4 * D]
+    out = torch.empty((N, ld), dtype=torch.float16, device="cuda")[:, :H * D]
+    cu = dev(torch, np.array([0, 170, N], np.int32))
+    packed(env, "f16", q, k, v, cu, H, HKV, D, 0.1, out=out)
+    check_packed(host(out), *packed64(torch, q, k, v, [170, 130], H, HKV, D, 0.1, 0.0, 0), H, D, "f16", 0.0, N)
