@@ -16,19 +16,41 @@
 //               scores' columns; at the end the rows of out;
 //   8           the MMAs: S_x = Q_x K_j^T (both from shared memory), then
 //               O_x += P_x V_j with P_x from tensor memory. While one tile's
-//               warps form weights, the tensor core works for the other:
-//               S0 S1 | O0 S0 O1 S1 | O0 S0 O1 S1 ..
-//   9           TMA: Q, then K and V tiles of 128 rows through a ring;
+//               warps form weights, the tensor core works for the other;
+//   9           TMA: Q, then K and V tiles of BK rows through a ring;
 //   10          tiles of V in which some row does not see some key: values that
 //               are not finite are taken out before the product (0 x inf is
 //               NaN) and the job is marked; rows that do see them add them at
 //               the end;
 //   11          looks up the jobs to come.
-// Tensor memory: S0 S1 (128 columns each, P in their first 64) O0 O1.
+// Tensor memory: S0 S1 (128 columns each), O0 O1. Key tiles have 128 rows or 64.
+// With 128 a tile's scores take its 128 columns, P the first 64 of them, and the
+// scores of the next keys wait for the product: S0 S1 | O0 S0 O1 S1 | O0 S0 ..
+// With 64 there are two places, so scores are ahead of the weights by one tile
+// and less is computed beyond the diagonal; but a product of 64 columns takes
+// the tensor core longer than half of one of 128, and each step has its fixed
+// part. Measured with D = 64, 96, 128 (us, tiles of 64 against 128): 64 prompts of
+// 0-300 rows 27 - 31, 33 - 35, 33 - 37; 16 of 600-1000 96 - 94, 113 - 117,
+// 117 - 127; 16 of 100-2047 174 - 168, 205 - 204, 215 - 223; one of 8192
+// 213 - 191, 236 - 211, 270 - 225. So the mean length decides, at 10 D rows. Where
+// the jobs are no more than the SMs the longest one is all the time, and 128 it is:
+// one prompt of 512 rows 18 - 17, 20 - 18, 20.5 - 19.5 (those with cold caches).
 //
 // The reference m_i is raised only when a tile's maximum exceeds it by 2^8 (the
 // weights stay below 256, exact in both types' range), so the accumulator is
 // rescaled a few times a row, not once a tile.
+//
+// What bounds it: long prompts the tensor core under the power limit. One of
+// 16384 rows, 64 heads in 8 groups, D = 128: 3.84 ms, 1.15 PFLOP/s; the same
+// kernel without its softmax takes 3.14 ms, which is the rate of a large matrix
+// product over as long a time. The tensor core is fed 1140 cycles a tile and 128
+// keys where 1024 would do (shared memory gives the scores' two operands at just
+// its rate) and waits 340 for weights. Shorter prompts: the change from job to
+// job, some 9000 cycles of 26000 at 1000 rows (weights and output of the first
+// and last tiles, which nothing else covers), and 5 us for launch and first loads.
+// Tried and slower: a warpgroup of its own for the output (286 us against 247 at
+// 16 of 100-2047 rows), two threads a row (251), weights handed over in four
+// parts, part of the exponentials on the FMA pipe, two warps that issue MMAs.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -42,22 +64,22 @@
 namespace fb {
 namespace pk {
 
-constexpr int BK = 128, NS = 2;          // keys a tile, ring places of a V and a K tile
 constexpr int kHalf = 128 * 128;         // 128 rows x 64 values of 16 bits: one SW128 box
 constexpr int kSoft = 256, kThreads = kSoft + 128;
 constexpr int NJ = 4;                    // jobs looked up ahead
 constexpr float kRaise = 8.0f;
 
-enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + NS, B_P = B_S + 2, B_O = B_P + 4,
-       B_DRAIN = B_O + 2, B_JOB, B_TAKEN = B_JOB + NJ, B_COUNT = B_TAKEN + NJ };
-
-template <int D>
+// BK keys a tile, NB = 128 / BK places of a tile's scores in tensor memory, NS ring places of a V and a K tile
+template <int D, int BK>
 struct Smem {
+    static constexpr int NB = 128 / BK, NS = 2 * NB, half = BK * 128;
     static constexpr int halves = (D + 63) / 64;
-    static constexpr int tile = halves * kHalf;            // one Q, K or V tile
-    static constexpr int place = 2 * tile;                 // V_j and, behind it, K_{j+1}
-    static constexpr int ring = 2 * tile, out = ring + NS * place, bar = out + 8 * 4096;   // out: 32 rows x 128 bytes a warp
-    static constexpr int bytes = bar + 8 * B_COUNT + 32 + 16 * NJ + 1024;
+    static constexpr int qtile = halves * kHalf, tile = halves * half;   // one Q tile; one K or V tile
+    static constexpr int place = 2 * tile;                 // V_j and, behind it, K_{j+NB}
+    static constexpr int ring = 2 * qtile, out = ring + NS * place, bar = out + 8 * 4096;   // out: 32 rows x 128 bytes a warp
+    enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + NS, B_P = B_S + 4, B_O = B_P + 4,
+           B_END = B_O + 2, B_DRAIN = B_END + 2, B_JOB, B_TAKEN = B_JOB + NJ, B_COUNT = B_TAKEN + NJ };
+    static constexpr int bytes = bar + 8 * B_COUNT + 48 + 16 * NJ + 1024;
 };
 
 struct Job {
@@ -65,6 +87,7 @@ struct Job {
 };
 // Key tiles [from[x], to[x]) of a job's tile x, counted from the sequence's start; `masked` where some row of the job does not
 // see some key of the tile.
+template <int BK>
 struct Keys {
     int lo[2], hi[2], from[2], to[2], j0, j1, upper, lower;
     __device__ __forceinline__ Keys(const Job& job, int R, int w) {
@@ -88,10 +111,15 @@ struct Keys {
 // The jobs of all sequences from the longest to the shortest: a sequence of n jobs has one on each of the levels 0 .. n - 1
 // (the level-th from its start, so the higher the longer), and they are counted from the highest level down, level by level,
 // sequence by sequence. Dealt out in turns that go to and fro over the CTAs, they leave every CTA about the same work
-// however the lengths differ. A whole warp looks them up, in ascending order; a lane keeps one of up to 32 sequences.
+// however the lengths differ. A whole warp looks them up, in ascending order; a lane keeps one of up to 32 sequences. Past
+// kLevels sequences every level would cost a look at all of them: then jobs are counted sequence by sequence, which passes
+// over the sequences once. Measured, by levels and one by one: one prompt of 16384 rows and 200 of 20 587 - 671 to 767 us by
+// their order; 260 of 0-300 67 - 71, 1000 of 0-100 139 - 79, 20000 of one row 24900 - 850.
+constexpr int kLevels = 256;
 struct Finder {
     const int32_t* cu;
-    int B, n_rows, rows, level, before;   // jobs on the levels above
+    int B, n_rows, rows, level, before;   // jobs on the levels above, or of the sequences before
+    int first;                            // without levels: the sequence of lane 0
     int a, z, n;                          // this lane's sequence, its jobs
     __device__ __forceinline__ void sequence(int s) {
         a = z = 0;
@@ -101,8 +129,13 @@ struct Finder {
         }
         n = (z - a + rows - 1) / rows;
     }
-    __device__ __forceinline__ Finder(const int32_t* cu_, int B_, int n_rows_, int rows_) : cu(cu_), B(B_), n_rows(n_rows_), rows(rows_), before(0) {
+    __device__ __forceinline__ Finder(const int32_t* cu_, int B_, int n_rows_, int rows_)
+        : cu(cu_), B(B_), n_rows(n_rows_), rows(rows_), level(-1), before(0), first(0) {
         const int lane = threadIdx.x & 31;
+        if (B > kLevels) {
+            sequence(lane);
+            return;
+        }
         int most = 0;
         for (int s = 0; s < B; s += 32) {
             sequence(s + lane);
@@ -110,9 +143,32 @@ struct Finder {
         }
         level = __reduce_max_sync(0xffffffffu, most) - 1;
     }
+    __device__ __forceinline__ Job of(int l, int at) const {   // job `at` of lane l's sequence
+        const int s0 = __shfl_sync(0xffffffffu, a, l);
+        return {s0, __shfl_sync(0xffffffffu, z, l), s0 + at * rows};
+    }
     // Job u (not less than the last one); s1 = 0 past the last.
     __device__ __forceinline__ Job find(int u) {
         const int lane = threadIdx.x & 31;
+        if (B > kLevels) {
+            while (first < B) {
+                int up = n;   // jobs up to this lane's
+#pragma unroll
+                for (int w = 1; w < 32; w <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, up, w);
+                    if (lane >= w) up += o;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, u - before < up);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    return of(l, u - before - __shfl_sync(0xffffffffu, up - n, l));
+                }
+                before += __shfl_sync(0xffffffffu, up, 31);
+                first += 32;
+                sequence(first + lane);
+            }
+            return {0, 0, 0};
+        }
         for (; level >= 0; --level) {
             int seen = before;
             for (int s = 0; s < B; s += 32) {
@@ -121,8 +177,7 @@ struct Finder {
                 const int rank = u - seen;   // of the ones here
                 if (rank < __popc(here)) {
                     const unsigned it = __ballot_sync(0xffffffffu, n > level && __popc(here & ((1u << lane) - 1)) == rank);
-                    const int l = __ffs(it) - 1, s0 = __shfl_sync(0xffffffffu, a, l);
-                    return {s0, __shfl_sync(0xffffffffu, z, l), s0 + level * rows};
+                    return of(__ffs(it) - 1, level);
                 }
                 seen += __popc(here);
             }
@@ -217,13 +272,17 @@ struct Args {
 
 }  // namespace pk
 
-template <class E, int D, bool CAP>
+template <class E, int D, int BK, bool CAP>
 __global__ void __launch_bounds__(pk::kThreads, 1)
     k_attention_packed(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const pk::Args A) {
     using namespace pk;
     using namespace tc;
-    using M = Smem<D>;
+    using M = Smem<D, BK>;
+    using Keys = pk::Keys<BK>;
+    constexpr int NB = M::NB, NS = M::NS, NH = BK / 64;   // NH: parts in which weights are handed over
+    constexpr int B_Q = M::B_Q, B_QFREE = M::B_QFREE, B_FULL = M::B_FULL, B_EMPTY = M::B_EMPTY, B_CLEAN = M::B_CLEAN, B_S = M::B_S,
+                  B_P = M::B_P, B_O = M::B_O, B_END = M::B_END, B_DRAIN = M::B_DRAIN, B_JOB = M::B_JOB, B_TAKEN = M::B_TAKEN;
     constexpr bool kBf16 = std::is_same<E, __nv_bfloat16>::value;
     // instruction descriptors: f32 accumulator, A and B of type E, M = 128; B of the second transposed (MN-major)
     constexpr uint32_t kType = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);
@@ -231,17 +290,17 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + M::bar);
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + M::bar + 8 * B_COUNT);
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + M::bar + 8 * M::B_COUNT);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-    volatile int* s_odd = s_abort + 1;   // [4] jobs (counted from 1) in which values that are not finite were met
-    volatile int4* s_job = reinterpret_cast<volatile int4*>(s_tmem + 8);   // [NJ] jobs, with the kv head
+    volatile int* s_odd = s_abort + 1;   // [2 NJ] jobs (counted from 1) in which values that are not finite were met
+    volatile int4* s_job = reinterpret_cast<volatile int4*>(s_tmem + 12);   // [NJ] jobs, with the kv head
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = A.R, G = A.G;
     pdl_trigger();
     if (threadIdx.x == kSoft) {
         *s_abort = 0;
-        for (int i = 0; i < 4; ++i) s_odd[i] = 0;
-        for (int i = 0; i < B_COUNT; ++i) {
+        for (int i = 0; i < 2 * NJ; ++i) s_odd[i] = 0;
+        for (int i = 0; i < M::B_COUNT; ++i) {
             mbar_init(&bar[i], i >= B_EMPTY && i < B_CLEAN ? 33 : i >= B_CLEAN && i < B_S ? 32 : i >= B_P && i < B_O ? 128 : i >= B_TAKEN ? 11 : 1);
         }
         mbar_fence_init();
@@ -263,12 +322,12 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         *hk = w.w;
         return job->s1 != 0 && !__any_sync(0xffffffffu, *s_abort);
     };
-    // ring place i, counted over all jobs; a job of n key tiles takes n + 1: K_0 alone, V_0 with K_1, .., V_{n-1} alone
+    // ring place i, counted over all jobs; a job of n key tiles takes n + NB: K_0 (and K_1), V_0 with K_NB, .., V_{n-1}
     auto v_at = [&](int i) { return (i % NS) * M::place; };
     auto k_at = [&](int i) { return (i % NS) * M::place + M::tile; };
     auto full = [&](int i) { wait(&bar[B_FULL + i % NS], (uint32_t)((i / NS) & 1), s_abort); };
 
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");   // 256 x 208 + 128 x 80 <= 384 x 168
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");   // 256 x 208 + 128 x 88 = 384 x 168
     Job job;
     int hk;
     if (warp == 9) {
@@ -283,15 +342,15 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                 mbar_expect_tx(&bar[B_Q], (uint32_t)(tiles * M::halves * G * R * 128));
                 for (int x = 0; x < tiles; ++x)
                     for (int h = 0; h < M::halves; ++h)
-                        tma_load_3d(sm + x * M::tile + h * kHalf, &qmap, 64 * h, hk * G, job.r0 + x * R, &bar[B_Q]);
-                for (int j = ks.j0; j <= ks.j1; ++j, ++i) {   // V_{j-1} and K_j
+                        tma_load_3d(sm + x * M::qtile + h * kHalf, &qmap, 64 * h, hk * G, job.r0 + x * R, &bar[B_Q]);
+                for (int j = ks.j0; j < ks.j1 + NB; ++j, ++i) {   // V_{j-NB} and K_j
                     if (i >= NS) wait(&bar[B_EMPTY + i % NS], (uint32_t)((i / NS - 1) & 1), s_abort);
                     if (*s_abort) break;
                     uint64_t* b = &bar[B_FULL + i % NS];
-                    mbar_expect_tx(b, (uint32_t)(M::tile * ((j > ks.j0) + (j < ks.j1))));
+                    mbar_expect_tx(b, (uint32_t)(M::tile * ((j >= ks.j0 + NB) + (j < ks.j1))));
                     for (int h = 0; h < M::halves; ++h) {
-                        if (j > ks.j0) tma_load_3d(sm + M::ring + v_at(i) + h * kHalf, &vmap, 64 * h, hk, job.s0 + (j - 1) * BK, b);
-                        if (j < ks.j1) tma_load_3d(sm + M::ring + k_at(i) + h * kHalf, &kmap, 64 * h, hk, job.s0 + j * BK, b);
+                        if (j >= ks.j0 + NB) tma_load_3d(sm + M::ring + v_at(i) + h * M::half, &vmap, 64 * h, hk, job.s0 + (j - NB) * BK, b);
+                        if (j < ks.j1) tma_load_3d(sm + M::ring + k_at(i) + h * M::half, &kmap, 64 * h, hk, job.s0 + j * BK, b);
                     }
                 }
             }
@@ -306,62 +365,69 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     } else if (warp == 8) {
         // ---- products; the warp stays together: uniform operands, one lane issues
         const uint32_t who = elect_one();
-        const uint64_t kd = sw128_desc(sm + M::ring), vd = sw128_mn_desc(sm + M::ring, kHalf);
-        const uint64_t qd[2] = {sw128_desc(sm), sw128_desc(sm + M::tile)};
-        auto scores = [&](int x, uint64_t b) {   // S_x = Q_x K^T
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint64_t o = (uint64_t)(((k / 4) * kHalf + (k % 4) * 32) >> 4);
-                umma_f16_ss(tmem + 128 * x, qd[x] + o, b + o, kDescS, k > 0, who);
-            }
-            umma_commit_by(&bar[B_S + x], who);
-        };
+        // the K-major descriptor of Q_0, to which the others are steps, and the MN-major one of the first V
+        const uint64_t qd = sw128_desc(sm), vd = sw128_mn_desc(sm + M::ring, M::half);
         int i = 0;
-        uint32_t clean = 0;          // phases of the places' barriers
-        uint32_t seen[2] = {0, 0};   // tiles of weights taken, over all jobs
+        uint32_t clean = 0;            // phases of the places' barriers
+        uint32_t given[2] = {0, 0};    // score tiles, over all jobs; they take the places of S_x in turn
+        uint32_t seen[2] = {0, 0};     // tiles of weights taken
+        auto scores = [&](int x, uint64_t b) {   // S_x = Q_x K^T
+            const uint32_t to = given[x]++ % NB;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                umma_f16_ss(tmem + 128 * x + 64 * to, qd + (uint64_t)((x * M::qtile + (k / 4) * kHalf + (k % 4) * 32) >> 4),
+                            b + (uint64_t)(((k / 4) * M::half + (k % 4) * 32) >> 4), kDescS, k > 0, who);
+            umma_commit_by(&bar[B_S + 2 * x + to], who);
+        };
         for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
             wait(&bar[B_Q], (uint32_t)(q & 1), s_abort);
-            full(i);
-            tc_fence_after();
+#pragma unroll 1
+            for (int j = ks.j0; j < ks.j0 + NB; ++j) {
+                full(i);
+                tc_fence_after();
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-                if (ks.active(x, ks.j0)) scores(x, kd + (uint64_t)(k_at(i) >> 4));
-            umma_commit_by(&bar[B_EMPTY + i % NS], who);
-            if (ks.j0 + 1 == ks.j1) umma_commit_by(&bar[B_QFREE], who);
-            full(++i);
+                for (int x = 0; x < 2; ++x)
+                    if (ks.active(x, j)) scores(x, qd + (uint64_t)((M::ring + k_at(i)) >> 4));
+                umma_commit_by(&bar[B_EMPTY + i % NS], who);
+                ++i;
+            }
+            if (ks.j0 + NB >= ks.j1) umma_commit_by(&bar[B_QFREE], who);
+            full(i);
             uint32_t fresh[2] = {1, 1};
-            for (int j = ks.j0; j < ks.j1; ++j) {   // V_j and K_{j+1} in place i
+            for (int j = ks.j0; j < ks.j1; ++j) {   // V_j and K_{j+NB} in place i
                 const bool more = j + 1 < ks.j1;
                 if (ks.masked(j)) {
                     const int z = i % NS;
                     wait(&bar[B_CLEAN + z], clean >> z & 1, s_abort);
                     clean ^= 1u << z;
                 }
-                const uint64_t v = vd + (uint64_t)(v_at(i) >> 4), kn = kd + (uint64_t)(k_at(i) >> 4);
+                const uint64_t v = vd + (uint64_t)(v_at(i) >> 4), kn = qd + (uint64_t)((M::ring + k_at(i)) >> 4);
                 uint64_t* empty = &bar[B_EMPTY + i % NS];
                 ++i;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    if (ks.active(x, j)) {
+                    if (ks.active(x, j)) {   // O_x += P_x V_j
+                        const uint32_t at = seen[x] % NB;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {   // O_x += P_x V_j, 64 keys as soon as their weights are there
-                            wait(&bar[B_P + 2 * x + h], seen[x] & 1, s_abort);
+                        for (int h = 0; h < NH; ++h) {   // 64 keys as soon as their weights are there
+                            wait(&bar[B_P + 2 * x + at + h], seen[x] / NB & 1, s_abort);
                             tc_fence_after();
 #pragma unroll
                             for (int k = 4 * h; k < 4 * h + 4; ++k)
-                                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, v + (uint64_t)(k * 16 * 128 >> 4), kDescO,
+                                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 64 * at + 8 * k, v + (uint64_t)(k * 16 * 128 >> 4), kDescO,
                                             !fresh[x] || k > 0, who);
                         }
                         ++seen[x];
                         fresh[x] = 0;
-                        if (j + 1 == ks.to[x]) umma_commit_by(&bar[B_O + x], who);
+                        if (NB > 1) umma_commit_by(&bar[B_O + x], who);
+                        if (j + 1 == ks.to[x]) umma_commit_by(&bar[B_END + x], who);
                     }
-                    if (more && ks.active(x, j + 1)) scores(x, kn);
+                    if (ks.active(x, j + NB)) scores(x, kn);
                     if (more && x == 0) full(i);   // what the next turn reads, looked for while the other tile's weights are formed
                 }
                 umma_commit_by(empty, who);
-                if (j + 2 == ks.j1) umma_commit_by(&bar[B_QFREE], who);   // the job's last scores
+                if (j + NB + 1 == ks.j1) umma_commit_by(&bar[B_QFREE], who);   // the job's last scores
             }
         }
         // the MMAs issued so far read shared memory and write tensor memory: they end before either is freed
@@ -391,10 +457,10 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         int i = 0;
         for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
-            for (int j = ks.j0; j <= ks.j1; ++j, ++i) {   // V_{j-1} in place i
+            for (int j = ks.j0; j < ks.j1 + NB; ++j, ++i) {   // V_{j-NB} in place i
                 // every place in its turn, and released by this warp too: a phase passed over could be taken for another
                 full(i);
-                if (j > ks.j0 && ks.masked(j - 1)) {
+                if (j >= ks.j0 + NB && ks.masked(j - NB)) {
                     // 0 x each of them, summed: NaN where one is not finite
                     uint4* t = reinterpret_cast<uint4*>(sm + M::ring + v_at(i));
                     typename Pair<E>::type acc[4];
@@ -417,7 +483,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                             for (int k = 0; k < 4; ++k) u[k] &= ~((not_finite2<E>(u[k]) >> 15) * 0xFFFFu);
                             t[e] = w;
                         }
-                        s_odd[q & 3] = q + 1;
+                        s_odd[q % (2 * NJ)] = q + 1;
                     }
                     fence_async_smem();
                     mbar_arrive(&bar[B_CLEAN + i % NS]);
@@ -448,65 +514,50 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         for (int j = from; j < upto; ++j, ++n) {
             const int kb = j * BK;
             const bool masked = kb + BK - 1 > lo || (A.window > 0 && kb <= hi - A.window);
-            wait(&bar[B_S + x], n & 1, s_abort);
+            const uint32_t at = n % NB, tn = ts + 64 * at;
+            wait(&bar[B_S + 2 * x + at], n / NB & 1, s_abort);
             tc_fence_after();
-            float s[4][32];
+            float s[BK / 32][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+            for (int c = 0; c < BK / 32; ++c) tmem_ld32(tn + 32 * c, s[c]);
             tmem_ld_wait();
             if (CAP) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < BK / 32; ++c)
 #pragma unroll
                     for (int e = 0; e < 32; ++e) s[c][e] = fmaf(-2.0f, rcp(ex2(s[c][e] * A.pre) + 1.0f), 1.0f);   // tanh
             }
             if (masked) {
                 const int top = i - kb, bottom = A.window > 0 ? top - A.window : -1;   // keys bottom < e <= top are seen
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < BK / 32; ++c) {
                     const uint32_t seen = ones(top + 1 - 32 * c) & ~ones(bottom + 1 - 32 * c);
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (!(seen >> e & 1)) s[c][e] = -INFINITY;
                 }
             }
-            float2 sum0, sum1;
-            uint32_t u[32];
-            auto weights = [&](int h) {
-                const float mc = m == -INFINITY ? 0.0f : -m * A.c;
-                const float2 c2 = make_float2(A.c, A.c), mc2 = make_float2(mc, mc);
+            constexpr int C = BK / 16;
+            float mm[C];   // chains; a NaN comes through and makes the row's reference NaN
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float2 y = fma2(make_float2(s[2 * h + e / 16][2 * e % 32], s[2 * h + e / 16][2 * e % 32 + 1]), c2, mc2);
-                    y.x = ex2(y.x);
-                    y.y = ex2(y.y);
-                    if (e & 1) sum1 = add2(sum1, y);
-                    else sum0 = add2(sum0, y);
-                    u[e] = pack2<E>(y.x, y.y);
-                }
-            };
-            auto hand_over = [&](int h) {
-                tmem_st32(ts + 32 * h, u);
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(&bar[B_P + 2 * x + h]);
-            };
-            float mm[8];   // eight chains; a NaN comes through and makes the row's reference NaN
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mm[e] = max3(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1], s[e / 2][16 * (e % 2) + 2]);
+            for (int e = 0; e < C; ++e) mm[e] = max3(s[e / 2][16 * (e % 2)], s[e / 2][16 * (e % 2) + 1], s[e / 2][16 * (e % 2) + 2]);
 #pragma unroll
             for (int k = 3; k < 15; k += 2)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mm[e] = max3(mm[e], s[e / 2][16 * (e % 2) + k], s[e / 2][16 * (e % 2) + k + 1]);
+                for (int e = 0; e < C; ++e) mm[e] = max3(mm[e], s[e / 2][16 * (e % 2) + k], s[e / 2][16 * (e % 2) + k + 1]);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
-            const float mx = max3(max3(mm[0], mm[2], mm[4]), mm[6], mm[6]);
+            for (int e = 0; e < C; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
+            const float mx = max3(mm[0], mm[2], C > 4 ? max3(mm[C - 4], mm[C - 2], mm[C - 2]) : mm[0]);
             const bool raise = mx != -INFINITY && !((mx - m) * A.c <= kRaise);   // from -inf, and to NaN, too
             if (__any_sync(0xffffffffu, raise)) {
                 const float f = raise ? ex2((m - mx) * A.c) : 1.0f;
                 if (raise) m = mx;
                 l *= f;
                 if (j > from) {
+                    if (NB > 1) {   // the product before; the one before that, as with one place the last, ended before these scores
+                        wait(&bar[B_O + x], (n - 1) & 1, s_abort);
+                        tc_fence_after();
+                    }
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         int o[16];
@@ -519,21 +570,38 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     }
                 }
             }
-            sum0 = sum1 = make_float2(0.0f, 0.0f);
-            weights(0);
-            hand_over(0);
-            weights(1);
-            hand_over(1);
+            const float mc = m == -INFINITY ? 0.0f : -m * A.c;
+            const float2 c2 = make_float2(A.c, A.c), mc2 = make_float2(mc, mc);
+            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+#pragma unroll
+            for (int c = 0; c < BK / 32; ++c) {
+                uint32_t u[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float2 y = fma2(make_float2(s[c][2 * e], s[c][2 * e + 1]), c2, mc2);
+                    y.x = ex2(y.x);
+                    y.y = ex2(y.y);
+                    if (e & 1) sum1 = add2(sum1, y);
+                    else sum0 = add2(sum0, y);
+                    u[e] = pack2<E>(y.x, y.y);
+                }
+                tmem_st16(tn + 16 * c, u);
+                if (c % 2) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&bar[B_P + 2 * x + at + c / 2]);
+                }
+            }
             sum0 = add2(sum0, sum1);
             l += sum0.x + sum0.y;
         }
         some = find(q + 1, &next, &next_hk);   // while the last products run
         if (!upto) continue;
-        wait(&bar[B_O + x], outs & 1, s_abort);
+        wait(&bar[B_END + x], outs & 1, s_abort);
         ++outs;
         tc_fence_after();
-        const bool odd = s_odd[q & 3] == q + 1;
-        const float inv = 1.0f / l;
+        const bool odd = s_odd[q % (2 * NJ)] == q + 1;
+        const float inv = *s_abort ? NAN : 1.0f / l;   // nobody takes what a wait that ran out left for an answer
         // 64 columns of the warp's 32 rows at a time by way of shared memory, so that a store instruction writes whole lines
         const uint64_t dst = live ? reinterpret_cast<uint64_t>(static_cast<E*>(A.out) + (int64_t)(job.s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D) : 0;
         const E* v = static_cast<const E*>(A.v) + (int64_t)job.s0 * A.ldkv + (int64_t)hk * D;
@@ -610,32 +678,38 @@ bool make_map(CUtensorMap* m, const void* p, int D, int heads, int n, int64_t ld
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class E, int D, bool CAP>
+constexpr int kSMs = 148;
+// as many jobs as there can be
+int64_t most_jobs(int n_rows, int B, int H, int HKV) {
+    return (n_rows / (2 * (128 / (H / HKV))) + std::min<int64_t>(B, n_rows)) * HKV;
+}
+
+template <class E, int D, int BK, bool CAP>
 cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv, int n_rows,
                           const int32_t* cu, int B, int H, int HKV, float scale, float softcap, int window, void* out,
                           int64_t ldo, cudaStream_t st) {
-    using M = pk::Smem<D>;
+    using M = pk::Smem<D, BK>;
     const int G = H / HKV, R = 128 / G;
     CUtensorMap qm, km, vm;
     if (!encode_ready()) return cudaErrorNotSupported;
-    if (!make_map<E>(&qm, q, D, H, n_rows, ldq, G, R) || !make_map<E>(&km, k, D, HKV, n_rows, ldkv, 1, pk::BK) ||
-        !make_map<E>(&vm, v, D, HKV, n_rows, ldkv, 1, pk::BK))
+    if (!make_map<E>(&qm, q, D, H, n_rows, ldq, G, R) || !make_map<E>(&km, k, D, HKV, n_rows, ldkv, 1, BK) ||
+        !make_map<E>(&vm, v, D, HKV, n_rows, ldkv, 1, BK))
         return cudaErrorInvalidValue;
     static uint64_t set = 0;   // one bit a device; setting it twice does no harm
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!(__atomic_load_n(&set, __ATOMIC_RELAXED) >> (dev & 63) & 1)) {
-        e = cudaFuncSetAttribute(k_attention_packed<E, D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::bytes);
+        e = cudaFuncSetAttribute(k_attention_packed<E, D, BK, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::bytes);
         if (e != cudaSuccess) return e;
         __atomic_fetch_or(&set, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
     }
     constexpr float kLog2e = 1.4426950408889634f;
     pk::Args a{cu, B, n_rows, HKV, G, R, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
                window, out, ldo, v, ldkv};
-    const int64_t jobs = (n_rows / (2 * R) + std::min<int64_t>(B, n_rows)) * HKV;
+    const int64_t jobs = most_jobs(n_rows, B, H, HKV);
     if (jobs > INT_MAX / 2) return cudaErrorInvalidValue;
-    return fbk_launch_early(k_attention_packed<E, D, CAP>, dim3((unsigned)std::min<int64_t>(jobs, 148)), dim3(pk::kThreads), (size_t)M::bytes, st, 1, qm,
+    return fbk_launch_early(k_attention_packed<E, D, BK, CAP>, dim3((unsigned)std::min<int64_t>(jobs, kSMs)), dim3(pk::kThreads), (size_t)M::bytes, st, 1, qm,
                       km, vm, a);
 }
 
@@ -647,11 +721,14 @@ using namespace fb;
 extern "C" int fbk_attention_packed(int type, const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
                                     int n_rows, const int32_t* cu, int B, int H, int HKV, int D, float scale,
                                     float softcap, int window, void* out, int64_t ldo, cudaStream_t st) {
-#define GO(E, DD)                                                                                                           \
-    (int)(softcap > 0.0f                                                                                                    \
-              ? launch_packed<E, DD, true>(q, ldq, k, v, ldkv, n_rows, cu, B, H, HKV, scale, softcap, window, out, ldo, st) \
-              : launch_packed<E, DD, false>(q, ldq, k, v, ldkv, n_rows, cu, B, H, HKV, scale, softcap, window, out, ldo, st))
-    if (type == T_F16) return D == 128 ? GO(__half, 128) : D == 96 ? GO(__half, 96) : GO(__half, 64);
-    return D == 128 ? GO(__nv_bfloat16, 128) : D == 96 ? GO(__nv_bfloat16, 96) : GO(__nv_bfloat16, 64);
+    const bool many = most_jobs(n_rows, B, H, HKV) > kSMs;
+#define GO(E, D, BK, CAP) \
+    (int)launch_packed<E, D, BK, CAP>(q, ldq, k, v, ldkv, n_rows, cu, B, H, HKV, scale, softcap, window, out, ldo, st)
+#define GO_CAP(E, D, BK) (softcap > 0.0f ? GO(E, D, BK, true) : GO(E, D, BK, false))
+#define GO_TILE(E, D) (many && n_rows < (int64_t)10 * D * B ? GO_CAP(E, D, 64) : GO_CAP(E, D, 128))
+    if (type == T_F16) return D == 128 ? GO_TILE(__half, 128) : D == 96 ? GO_TILE(__half, 96) : GO_TILE(__half, 64);
+    return D == 128 ? GO_TILE(__nv_bfloat16, 128) : D == 96 ? GO_TILE(__nv_bfloat16, 96) : GO_TILE(__nv_bfloat16, 64);
+#undef GO_TILE
+#undef GO_CAP
 #undef GO
 }
