@@ -15,7 +15,11 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t type_bytes(int type) { return type == T_F32 ? 4 : type == T_F16 || type == T_BF16 ? 2 : 0; }
-constexpr float kMost = 1e30f;   // scale and soft cap: no infinity
+constexpr float kMost = 1e30f;
+// what scores are multiplied by stays finite
+bool scale_ok(float scale, float softcap) {
+    return scale > 0.0f && scale <= kMost && (softcap == 0.0f || (softcap > 0.0f && softcap <= kMost && scale / softcap <= kMost && 1.0f / softcap <= kMost));
+}
 bool head_dim_ok(int D) { return D == 64 || D == 96 || D == 128; }
 
 // a row stride that holds `width` values and keeps rows on 16-byte boundaries
@@ -63,7 +67,9 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* c, int type, const void* q, con
                             int64_t ldkv, int T, int H, const int32_t* tok_seq, const int32_t* tok_pos, int rot, int neox,
                             const float* rope_cos, const float* rope_sin, int n_rope, int out_type, void* q_out,
                             int64_t ldq_out, void* k_out, void* v_out, int64_t ldkv_out, void* stream) {
-    if (!cache_ok(c) || !type_bytes(type) || !type_bytes(out_type) || T < 0 || !k || !v || !tok_seq || !tok_pos) return -1;
+    if (!cache_ok(c) || !type_bytes(type) || !type_bytes(out_type) || T < 0) return -1;
+    if (T == 0) return 0;
+    if (!k || !v || !tok_seq || !tok_pos) return -1;
     const int D = c->head_dim, HKV = c->n_head_kv;
     if ((q == nullptr) != (q_out == nullptr)) return -1;
     if (rot < 0 || rot > D || rot % 2 || n_rope <= 0 || (rot > 0 && (!rope_cos || !rope_sin))) return -1;
@@ -76,7 +82,6 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* c, int type, const void* q, con
     // in place means the same rows
     if (q && q == q_out && (type != out_type || ldq != ldq_out)) return -1;
     if ((k == k_out || v == v_out) && (type != out_type || ldkv != ldkv_out)) return -1;
-    if (T == 0) return 0;
     const int rc = on_device({c->pool, c->page_table, q, k, tok_pos, rope_cos, q_out, k_out});
     if (rc) return rc;
     return fbk_kv4_append(*c, type, q, k, v, ldq, ldkv, T, H, tok_seq, tok_pos, rot, neox ? 1 : 0, rope_cos, rope_sin, n_rope,
@@ -91,12 +96,13 @@ FISH_API size_t fbx_kv4_attention_workspace(int T, int H, int n_head_kv, int hea
 FISH_API int fbx_kv4_attention(const fbx_kv4_cache* c, int type, const void* q, int64_t ldq, int T, int H,
                                const int32_t* tok_seq, const int32_t* tok_pos, int max_keys, float scale, float softcap,
                                int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!cache_ok(c) || !type_bytes(type) || T < 0 || T > 65535 || !q || !out || !tok_seq || !tok_pos || max_keys <= 0) return -1;
+    if (!cache_ok(c) || !type_bytes(type) || T < 0 || T > 65535 || max_keys <= 0) return -1;
+    if (T == 0) return 0;
+    if (!q || !out || !tok_seq || !tok_pos) return -1;
     const int D = c->head_dim, HKV = c->n_head_kv;
-    if (H <= 0 || H > 65535 || H % HKV || !(softcap >= 0.0f) || softcap > kMost || !(scale > 0.0f) || scale > kMost || window < 0) return -1;
+    if (H <= 0 || H > 65535 || H % HKV || !scale_ok(scale, softcap) || window < 0) return -1;
     if (!stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldo, (int64_t)H * D, type)) return -1;
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
-    if (T == 0) return 0;
     const size_t need = fbk_kv4_attention_workspace(T, H, HKV, D, max_keys);
     if (need && (!workspace || workspace_bytes < need)) return -1;
     const int rc = on_device({c->pool, c->page_table, q, tok_pos, out, need ? workspace : nullptr});
@@ -108,16 +114,15 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* c, int type, const void* q, 
 FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
                                   int n_rows, const int32_t* cu_seqlens, int n_seqs, int H, int HKV, int D, float scale,
                                   float softcap, int window, void* out, int64_t ldo, void* stream) {
-    if ((type != T_F16 && type != T_BF16) || !q || !k || !v || !out || !cu_seqlens || n_rows < 0 || n_seqs <= 0 ||
-        n_seqs > (1 << 20) || n_rows > (1 << 30))
-        return -1;
-    if (!head_dim_ok(D) || HKV <= 0 || H <= 0 || H % HKV || H > 65535 || H / HKV > 128 || !(softcap >= 0.0f) || softcap > kMost || !(scale > 0.0f) || scale > kMost || window < 0)
+    if ((type != T_F16 && type != T_BF16) || n_rows < 0 || n_seqs <= 0 || n_seqs > (1 << 20) || n_rows > (1 << 30)) return -1;
+    if (n_rows == 0) return 0;
+    if (!q || !k || !v || !out || !cu_seqlens) return -1;
+    if (!head_dim_ok(D) || HKV <= 0 || H <= 0 || H % HKV || H > 65535 || H / HKV > 128 || !scale_ok(scale, softcap) || window < 0)
         return -1;
     if (!stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldkv, (int64_t)HKV * D, type) ||
         !stride_ok(ldo, (int64_t)H * D, type))
         return -1;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return -1;
-    if (n_rows == 0) return 0;
     const int rc = on_device({q, k, cu_seqlens, out});
     if (rc) return rc;
     return fbk_attention_packed(type, q, ldq, k, v, ldkv, n_rows, cu_seqlens, n_seqs, H, HKV, D, scale, softcap, window, out,

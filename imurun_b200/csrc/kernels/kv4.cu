@@ -465,13 +465,11 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     // and of sum_g lo sum(q_g): the sums' high parts against k = 0..3, their low parts against k = 4..7
     const uint32_t qsb = *reinterpret_cast<const uint32_t*>(sm + M::qs + (t >> 1) * 64 + g * 8 + (t & 1) * 4);
     constexpr float kLog2e = 1.4426950408889634f;
-    float cs[2], csc[2];   // log2 units of the heads 2 t, 2 t + 1, and of the code products
+    float cs[2];   // log2 units of the heads 2 t, 2 t + 1
     const bool cap = A.softcap > 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
         cs[i] = A.scale * reinterpret_cast<const float*>(sm + M::ex)[2 * t + i] * (cap ? 1.0f / A.softcap : kLog2e);
-        csc[i] = cs[i] * kCode;
-    }
     float ref[2] = {kNoRef, kNoRef}, sum[2] = {0.0f, 0.0f};
     int top_e = 0;                          // E
     __half2 down_e = __float2half2_rn(0.0f), limit_e = down_e;   // 2^-E, 2^(E + 1); a limit of 0 is passed by the first page
@@ -532,7 +530,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 s[h][3] = e ? fmaf(db, x[3], s[h][3]) : db * x[3];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[h][i] = fmaf(s[h][i], csc[i & 1], sl[i] * cs[i & 1]);
+            for (int i = 0; i < 4; ++i) s[h][i] = fmaf(s[h][i], kCode, sl[i]) * cs[i & 1];
             words<GP / 2>(rec + R::vd + row * GP * 2, v0[h]);
             words<GP / 2>(rec + R::vd + (row + 8) * GP * 2, v1[h]);
             words<GP / 2>(rec + R::vlo + row * GP * 2, u0[h]);

@@ -61,18 +61,6 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 
 // 8 consecutive values at a 16-byte boundary
 template <class E>
-__device__ __forceinline__ void load8(const E* p, float (&x)[8]) {
-    if constexpr (sizeof(E) == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        uint4 raw = *reinterpret_cast<const uint4*>(p);
-        const E* e = reinterpret_cast<const E*>(&raw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<E>(e[i]);
-    }
-}
-template <class E>
 __device__ __forceinline__ void store8(E* p, const float (&x)[8]) {
     if constexpr (sizeof(E) == 4) {
         *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);

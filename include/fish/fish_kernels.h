@@ -128,7 +128,10 @@ FISH_API int fbx_attention_static(const float* q, const void* k, const void* v, 
  * for it; they allocate nothing, so they can be captured into a graph from the
  * first call on. They return 0, -1 for arguments that cannot be right
  * (including a buffer that is not memory of the current device, and an address
- * or row stride that is not a multiple of 16 bytes), or a positive CUDA error.
+ * or row stride that is not a multiple of 16 bytes), or a positive CUDA error;
+ * of k and v, of tok_seq and tok_pos, of the two tables and of k_out and v_out
+ * one is looked at, and the other has to lie in memory of the same kind. With
+ * no tokens or rows nothing is done, and buffers may be NULL.
  * `type` is an element type: 0 F32, 1 F16, 30 BF16 (ggml's ids). Row strides
  * (ld..) are in elements. No counterpart in the reference, whose cache is f32
  * (model/fish/include/fish/model.h:279-280) and whose attention takes one
@@ -182,7 +185,8 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* cache, int type, const void* q,
 /* Attention of T query tokens over the cache: token t (rotated queries q, H
  * heads in groups of H / n_head_kv) sees the positions 0..tok_pos[t] of its
  * sequence, or the last `window` of them (0: all); scores are scale * q.k
- * (scale > 0), then with softcap > 0 softcap * tanh(score / softcap). out has q's type;
+ * (scale > 0), then with softcap > 0 softcap * tanh(score / softcap); scale,
+ * 1 / softcap and scale / softcap are at most 1e30. out has q's type;
  * rows of padding tokens (negative tok_pos) stay as they were, and a token
  * that sees nothing that can be read gets zeros. max_keys, an upper bound on
  * tok_pos + 1, sizes the split of long contexts (any value gives the right
@@ -203,7 +207,9 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
  * its sequence up to itself, or with window > 0 the last `window` of them. scale
  * and softcap as above. Nothing in rows that a query does not see reaches its
  * output, infinities and NaN included. Rows of out outside every sequence
- * stay as they were. */
+ * stay as they were. The kernel's waits for its own copies and products are
+ * bounded (some 10 ms each): if one ran out, rows of out would be NaN or stay
+ * as they were. */
 FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
                                   int n_rows, const int32_t* cu_seqlens, int n_seqs, int H, int HKV, int D, float scale,
                                   float softcap, int window, void* out, int64_t ldo, void* stream);

@@ -732,6 +732,8 @@ def many(seed, count, low, high):
     ("bf16", [5000], 2, 1, 128, 0.0, 300),
     ("f16", many(3, 9, 100, 1500), 6, 2, 64, 15.0, 500),
     ("bf16", [3001, 17], 7, 1, 128, 0.0, 0),
+    ("bf16", many(4, 1000, 0, 60), 4, 2, 64, 0.0, 0),         # so many sequences that they are taken one by one
+    ("f16", [0] * 700 + [400] + many(5, 300, 0, 4) + [0] * 100, 3, 1, 128, 0.0, 0),
 ])
 def test_packed_many_jobs(env, t, lens, H, HKV, D, softcap, window):
     lib, torch, _ = env
@@ -771,3 +773,14 @@ def test_packed_rows_past_32_bits(env):
     cu = dev(torch, np.array([0, 170, N], np.int32))
     packed(env, "f16", q, k, v, cu, H, HKV, D, 0.1, out=out)
     check_packed(host(out), *packed64(torch, q, k, v, [170, 130], H, HKV, D, 0.1, 0.0, 0), H, D, "f16", 0.0, N)
+
+
+def test_attention_of_huge_queries(env):
+    """f32 queries near the top of their range: scores are finite, and so is the result."""
+    lib, torch, _ = env
+    H, HKV, D = 2, 1, 64
+    c, *_ = filled(env, [40], HKV, D, seed=9)
+    q = torch.randn((1, H * D), device="cuda")
+    base = attention(env, c, "f32", q, H, [0], [39], 40, 2.0**-3)
+    out = attention(env, c, "f32", q * 2.0**118, H, [0], [39], 40, 2.0**-121)
+    assert torch.equal(out, base)   # powers of two only

@@ -129,3 +129,14 @@ def test_format_holds_every_value_once(D):
         assert np.array_equal(got.astype(np.float32), plain.values(codes, d, lo))
         # half a code of the group's range, and the rounding of lo and d to f16
         assert (np.abs(got - want).reshape(16, -1, 32) <= 0.5 * d[..., None].astype(np.float64) + 2e-2).all()
+
+
+def test_empty_calls_need_no_buffers(lib):
+    assert append(lib, T=0, k=None, v=None, q=None, q_out=None, seq=None, pos=None) == 0
+    assert attend(lib, T=0, q=None, out=None, seq=None, pos=None) == 0
+    assert packed(lib, rows=0, q=None, k=None, v=None, out=None) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(softcap=1e-31), dict(scale=1e20, softcap=1e-15), dict(scale=2e30), dict(softcap=2e30)])
+def test_scales_that_could_overflow_are_refused(lib, bad):
+    assert attend(lib, **bad) == -1 and packed(lib, **bad) == -1
