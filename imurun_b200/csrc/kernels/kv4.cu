@@ -243,11 +243,13 @@ __global__ void __launch_bounds__(256, 4) k_kv4_append(const __grid_constant__ f
 // d 2^-E <= 2 the products stay in f16's range whatever the values' size is.
 //
 // Roundings: 16-bit queries are exact in one f16 part (scaled by a power of
-// two), f32 ones go in as two, and so do their weights p d (2^-22). For f16
-// outputs p d is rounded once and meets codes of -8..7 (8 sum(p d) is taken off
-// by one more MMA a group, and lo + 8 d stands for lo), else the rounding would
-// be the larger part of the error; for bf16, whose own step is 8 times as
-// wide, p is rounded first and codes stay 0..15.
+// two), f32 ones go in as two, and so do their weights p d (2^-22), which meet
+// codes of -8..7 with lo + 8 d in lo's place: sums that are all of one sign, and
+// of which lo takes most away again, would leave the adder's truncation several
+// times as large in the result. For f16 outputs p d is rounded once and meets
+// codes of -8..7 too (8 sum(p d) is taken off by one more MMA a group), else the
+// rounding would be the larger part of the error; for bf16, whose own step is 8
+// times as wide, p is rounded first and codes stay 0..15.
 constexpr int kAtWarps = 8, kSlots = 2;
 constexpr int kMaxCluster = 8;
 constexpr float kNoRef = -1e30f;   // before the first key: finite, so that a key outside (-inf) weighs 0 against it
@@ -280,8 +282,9 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cas
 
 // The 8 codes of w as f16, r[n] = (code n, code n + 4). Sub: as the subnormals
 // that they are where they lie, 2^-24 for even n and 2^-20 for odd; else as
-// they are (dropped into the mantissa of 1024 or of 64, which is taken off exactly).
-template <bool Sub>
+// they are, less Mid (dropped into the mantissa of 1024 or of 64, which is taken
+// off exactly together with Mid).
+template <bool Sub, int Mid = 0>
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
     if (Sub) {
         const uint32_t u = w >> 8;
@@ -290,7 +293,7 @@ __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
         r[2] = u & 0x000F000Fu;
         r[3] = u & 0x00F000F0u;
     } else {
-        const __half2 k1024 = bits_h2(0x64006400u), k64 = bits_h2(0x54005400u);
+        const __half2 k1024 = bits_h2(0x64006400u + Mid * 0x00010001u), k64 = bits_h2(0x54005400u + Mid * 0x00100010u);
         const uint32_t u = w >> 8;
         r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), k1024));
         r[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | 0x54005400u), k64));
@@ -624,15 +627,15 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 const __half2 n0 = __hmul2(bits_h2(v0[h][e / 2]), down_e), n1 = __hmul2(bits_h2(v1[h][e / 2]), down_e);   // d 2^-E
                 float la = e & 1 ? half_at<1>(u0[h][e / 2]) : half_at<0>(u0[h][e / 2]);
                 float lb = e & 1 ? half_at<1>(u1[h][e / 2]) : half_at<0>(u1[h][e / 2]);
-                if (W == W_MID) {
+                if (W != W_HALF) {
                     la = fmaf(8.0f, e & 1 ? half_at<1>(v0[h][e / 2]) : half_at<0>(v0[h][e / 2]), la);
                     lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[h][e / 2]) : half_at<0>(v1[h][e / 2]), lb);
                 }
                 olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
                 olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
                 uint32_t ra[4], rc[4];
-                codes8<SUB>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
-                codes8<SUB>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+                codes8<SUB, W == W_PAIR ? 8 : 0>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
+                codes8<SUB, W == W_PAIR ? 8 : 0>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
                 __half2 hi0, hi1;
                 float x[4];
                 if (W == W_HALF) {
