@@ -19,13 +19,19 @@ namespace fb {
 // sin of its 8 dimensions serve all its heads. Where a lane's 8 dimensions are
 // rotated together or not at all, the partner of a value is in the same lane
 // (pairs of neighbours) or comes by shuffle (halves); other rotations load it
-// once more. Beside memory it is instructions: 64 registers keep four CTAs on an
-// SM, and a code is rounded by adding 1.5 2^23, whose low bits are then the code
-// (a multiply-add a code puts them together). A group of 32
-// values is four neighbouring lanes: its extremes by two shuffles, its codes one
-// 32-bit word of K or two 16-bit words of V a lane. Rotation and quantisation are
-// in 32 bits with every step rounded by itself (no fused multiply-add), so the
-// codes are those of the plain formula.
+// once more. Beside memory it is instructions and the loads in flight: 64
+// registers (50 where a warp has no more than three turns of 16-bit heads) keep
+// four (five) CTAs on an SM, the warps of a CTA have equal turns, and a code is
+// rounded by adding 1.5 2^23, whose low bits are then the code (a multiply-add a
+// code puts them together). A group of 32 values is four neighbouring lanes: its
+// extremes by two shuffles, its codes one 32-bit word of K or two 16-bit words
+// of V a lane. Rotation and quantisation are in 32 bits with every step rounded
+// by itself (no fused multiply-add), so the codes are those of the plain formula.
+// Measured, 16384 bf16 tokens with 64 + 2 x 8 heads of 128: 158 us, 4.4 TB/s; 8192
+// with 28 + 2 x 4 f16 heads 45 us (65 with eight warps of unequal turns and five
+// heads a lane), rotated by halves 51; one token 2.3 us in a graph. A token's
+// heads in several CTAs of three turns instead of one of five: 87 us against 80
+// at 8192 tokens.
 enum : int { ROPE_PAIRS, ROPE_HALVES, ROPE_ANY };
 
 // 8 values as loaded, and as f32
@@ -51,8 +57,9 @@ struct Turn {
     float cs[N], sn[N];
 };
 
-template <class E, class O, int D, int ROPE>
-__global__ void __launch_bounds__(256, 4) k_kv4_append(const __grid_constant__ fbx_kv4_cache c, const E* q, const E* k,
+// FEW: a warp has at most three turns, all of them fetched at once
+template <class E, class O, int D, int ROPE, bool FEW>
+__global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_constant__ fbx_kv4_cache c, const E* q, const E* k,
                                                        const E* v, int64_t ldq, int64_t ldkv, int H, int hpc,
                                                        const int32_t* __restrict__ tok_seq,
                                                        const int32_t* __restrict__ tok_pos, int rot, int neox,
@@ -61,7 +68,7 @@ __global__ void __launch_bounds__(256, 4) k_kv4_append(const __grid_constant__ f
                                                        int64_t ldkv_out) {
     using R = Kv4Rec<D>;
     constexpr int L = D / 8, HPW = 32 / L;   // lanes a head, heads a warp (D = 96: 8 lanes idle)
-    constexpr int U = sizeof(E) == 4 ? 2 : 5;
+    constexpr int U = sizeof(E) == 4 ? 2 : FEW ? 3 : 5;
     pdl_trigger();
     const int t = blockIdx.x, HKV = c.n_head_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int d0 = (lane % L) * 8, half = rot / 2;
@@ -843,9 +850,13 @@ template <class E, class O, int D, int ROPE>
 static cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t st) {
     constexpr int HPW = 32 / (D / 8);
     const int H = a.q ? a.H : 0, heads = H + 2 * a.c.n_head_kv;
-    // few tokens: CTAs of 8 warps with a turn each; many: a token's heads in one CTA, of no more warps than they fill
-    const int warps = std::min(8, (heads + HPW - 1) / HPW), hpc = a.T >= 148 ? heads : warps * HPW;
-    return fbk_launch_early(k_kv4_append<E, O, D, ROPE>, dim3(a.T, (heads + hpc - 1) / hpc), dim3(32 * warps), 0, st, 1, a.c,
+    // few tokens: CTAs of 8 warps with a turn each; many: a token's heads in one CTA, of as many warps as have equal turns
+    const int groups = (heads + HPW - 1) / HPW, turns = (groups + 7) / 8;
+    const bool many = a.T >= 148;
+    const int warps = many ? (groups + turns - 1) / turns : std::min(8, groups), hpc = many ? heads : warps * HPW;
+    const bool few = sizeof(E) == 2 && turns <= 3;
+    auto kern = few ? k_kv4_append<E, O, D, ROPE, sizeof(E) == 2> : k_kv4_append<E, O, D, ROPE, false>;
+    return fbk_launch_early(kern, dim3(a.T, (heads + hpc - 1) / hpc), dim3(32 * warps), 0, st, 1, a.c,
                             (const E*)a.q, (const E*)a.k, (const E*)a.v, a.ldq, a.ldkv, H, hpc, a.tok_seq, a.tok_pos, a.rot,
                             a.neox, a.rcos, a.rsin, a.n_rope, (O*)a.q_out, a.ldq_out, (O*)a.k_out, (O*)a.v_out, a.ldkv_out);
 }
