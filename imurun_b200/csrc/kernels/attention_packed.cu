@@ -197,6 +197,12 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// tanh(x) of y = 2 log2(e) x: 1 - 2 / (2^y + 1), whose error of 2^-23 is too much of a small x (a large cap); there the series
+__device__ __forceinline__ float tanh2(float y) {
+    const float x = y * 0.34657359f, x2 = x * x;   // ln(2) / 2
+    const float t = fmaf(-2.0f, rcp(ex2(y) + 1.0f), 1.0f), small = x * fmaf(x2, fmaf(x2, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
+    return fabsf(x) < 0.05f ? small : t;
+}
 // two f32 operations an instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     unsigned long long r;
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < BK / 32; ++c)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) s[c][e] = fmaf(-2.0f, rcp(ex2(s[c][e] * A.pre) + 1.0f), 1.0f);   // tanh
+                    for (int e = 0; e < 32; ++e) s[c][e] = tanh2(s[c][e] * A.pre);
             }
             if (masked) {
                 const int top = i - kb, bottom = A.window > 0 ? top - A.window : -1;   // keys bottom < e <= top are seen

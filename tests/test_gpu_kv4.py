@@ -784,3 +784,77 @@ def test_attention_of_huge_queries(env):
     base = attention(env, c, "f32", q, H, [0], [39], 40, 2.0**-3)
     out = attention(env, c, "f32", q * 2.0**118, H, [0], [39], 40, 2.0**-121)
     assert torch.equal(out, base)   # powers of two only
+
+
+@pytest.mark.parametrize("cap", [1e3, 1e6, 1e12])
+def test_packed_caps_far_above_the_scores(env, cap):
+    """A cap's rounding goes by the score, not by the cap: the tolerance is that of calls without one."""
+    lib, torch, _ = env
+    torch.manual_seed(11)
+    H, HKV, D, lens = 4, 2, 64, [300, 65]
+    N = sum(lens)
+    q, k, v = (torch.randn((N, h * D), device="cuda").half() for h in (H, HKV, HKV))
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    scale = 1.0 / np.sqrt(D)
+    out = packed(env, "f16", q, k, v, cu, H, HKV, D, scale, cap)
+    ref = packed64(torch, q, k, v, lens, H, HKV, D, scale, cap, 0)
+    check_packed(host(out), *ref, H, D, "f16", 0.0, N)
+
+
+def test_calls_side_by_side(env):
+    """Calls of all three operators on two streams at once, each with a workspace and outputs of its own, leave what they
+    leave alone."""
+    lib, torch, _ = env
+    H, HKV, D, n = 8, 2, 128, 4000
+    c, *_ = filled(env, [n, n], HKV, D, seed=21)
+    torch.manual_seed(21)
+    lens = [700, 33, 0, 1200]
+    N = sum(lens)
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    qp, kp, vp = (torch.randn((N, h * D), device="cuda").half() for h in (H, HKV, HKV))
+    qt = [torch.randn((1, H * D), device="cuda").half() for _ in range(2)]
+    seq, pos = [dev(torch, np.array([s], np.int32)) for s in range(2)], dev(torch, np.array([n - 1], np.int32))
+    size = lib.fbx_kv4_attention_workspace(1, H, HKV, D, n)
+    assert size > 0
+    ws = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def go(i, st, op, tok):
+        assert lib.fbx_attention_packed(1, qp.data_ptr(), H * D, kp.data_ptr(), vp.data_ptr(), HKV * D, N, cu.data_ptr(), 4, H,
+                                        HKV, D, 0.1, 0.0, 0, op.data_ptr(), H * D, st) == 0
+        for _ in range(3):
+            assert lib.fbx_kv4_attention(c.handle, 1, qt[i].data_ptr(), H * D, 1, H, seq[i].data_ptr(), pos.data_ptr(), n, 0.1,
+                                         0.0, 0, tok.data_ptr(), H * D, ws[i].data_ptr(), size, st) == 0
+
+    want = [(torch.zeros_like(qp), torch.zeros_like(qt[0])) for _ in range(2)]
+    for i in range(2):
+        go(i, None, *want[i])
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [(torch.zeros_like(qp), torch.zeros_like(qt[0])) for _ in range(2)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            go(i, streams[i].cuda_stream, *got[i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1])
+    assert int(c.err) == 0
+
+
+def test_sequences_share_pages(env):
+    """Two sequences whose tables name the same pages for a common prefix see the same keys there."""
+    lib, torch, _ = env
+    H, HKV, D = 4, 2, 96
+    c, k, v, d, at = filled(env, [160, 160], HKV, D, seed=31)
+    c.dtable[1, :8] = c.dtable[0, :8]
+    q = torch.randn((1, H * D), device="cuda").expand(2, -1).contiguous()
+    out = attention(env, c, "f32", q, H, [0, 1], [127, 127], 160, 0.1)
+    assert torch.equal(out[0], out[1])
+    out = attention(env, c, "f32", q, H, [0, 1], [159, 159], 160, 0.1)
+    for s in range(2):
+        rows = torch.cat([torch.arange(128), torch.arange(128, 160) + int(at[s])]).cuda()
+        x, kk, vv, dd = q[s].view(HKV, 2, D).double(), *(y[rows].transpose(0, 1) for y in (k, v, d))
+        w = torch.softmax(x @ kk.transpose(1, 2) * 0.1, -1)
+        want, mean, coarse = (z.reshape(H, D).cpu().numpy() for z in (w @ vv, w @ vv.abs(), w @ dd))
+        ext = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(H).cpu().numpy() * 0.1
+        near(host(out[s]).reshape(H, D), want, (mean, ext, coarse), "f32")
