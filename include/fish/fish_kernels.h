@@ -207,10 +207,11 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
  * its sequence up to itself, or with window > 0 the last `window` of them. scale
  * and softcap as above. Nothing in rows that a query does not see reaches its
  * output, infinities and NaN included. Weights are up to 2^8 before the
- * division, so sums stay finite for values of v up to 10^36 / n_rows. Rows of out outside every sequence
- * stay as they were. The kernel's waits for its own copies and products are
- * bounded (some 10 ms each): if one ran out, rows of out would be NaN or stay
- * as they were. */
+ * division, so sums stay finite for values of v up to 10^36 / n_rows. The
+ * tiles, and with them the last bits of a row, go by the batch's lengths. Rows
+ * of out outside every sequence stay as they were. The kernel's waits for its
+ * own copies and products are bounded (some 10 ms each): if one ran out, rows
+ * of out would be NaN or stay as they were. */
 FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
                                   int n_rows, const int32_t* cu_seqlens, int n_seqs, int H, int HKV, int D, float scale,
                                   float softcap, int window, void* out, int64_t ldo, void* stream);

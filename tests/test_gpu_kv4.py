@@ -858,3 +858,30 @@ def test_sequences_share_pages(env):
         want, mean, coarse = (z.reshape(H, D).cpu().numpy() for z in (w @ vv, w @ vv.abs(), w @ dd))
         ext = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(H).cpu().numpy() * 0.1
         near(host(out[s]).reshape(H, D), want, (mean, ext, coarse), "f32")
+
+
+@pytest.mark.parametrize("t,H,HKV,D,softcap,window", [("f16", 4, 4, 64, 0.0, 100), ("bf16", 4, 2, 96, 6.0, 0), ("f16", 8, 2, 128, 20.0, 65),
+                                                      ("bf16", 12, 4, 128, 0.0, 64), ("f16", 10, 5, 96, 0.0, 1)])
+def test_packed_many_short_prompts(env, t, H, HKV, D, softcap, window):
+    """Batches of many short prompts, which take smaller key tiles: windows, caps, and values that are not finite."""
+    lib, torch, _ = env
+    torch.manual_seed(D + H)
+    lens = many(6, 90, 0, 330) + [64, 65, 128, 1]
+    N = sum(lens)
+    q, k, v = (torch.randn((N, h * D), device="cuda").to(dtype(torch, t)) for h in (H, HKV, HKV))
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    scale = 1.3 / np.sqrt(D)
+    clean = packed(env, t, q, k, v, cu, H, HKV, D, scale, softcap, window)
+    check_packed(host(clean), *packed64(torch, q, k, v, lens, H, HKV, D, scale, softcap, window), H, D, t, softcap, N)
+    ends = np.cumsum(lens)
+    vv = v.clone()
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    for i, what in ((3, np.inf), (17, np.nan), (40, -np.inf), (91, np.inf)):
+        n = lens[i]
+        row = int(ends[i]) - n + n // 2
+        vv[row, D - 1] = what          # kv head 0, its last dimension
+        last = min(int(ends[i]), row + window) if window else int(ends[i])
+        for h in range(H // HKV):
+            hit[row:last, h * D + D - 1] = True
+    out = packed(env, t, q, k, vv, cu, H, HKV, D, scale, softcap, window)
+    assert torch.equal(out[~hit], clean[~hit]) and not bool(torch.isfinite(out[hit]).any())
