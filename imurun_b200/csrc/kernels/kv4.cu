@@ -555,6 +555,12 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             words<GP / 2>(rec + R::vlo + row * GP * 2, u0[h]);
             words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1[h]);
             if (NG == 3) v0[h][1] &= 0xFFFFu, v1[h][1] &= 0xFFFFu;
+            // a d below 0 has codes of 0 only (f16 rounded the group's minimum up past its maximum): it counts as 0
+#pragma unroll
+            for (int e = 0; e < GP / 2; ++e) {
+                v0[h][e] = h2_bits(__hmax2_nan(bits_h2(v0[h][e]), bits_h2(0u)));
+                v1[h][e] = h2_bits(__hmax2_nan(bits_h2(v1[h][e]), bits_h2(0u)));
+            }
         }
         if (cap) {
 #pragma unroll

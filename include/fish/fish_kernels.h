@@ -140,10 +140,11 @@ FISH_API int fbx_attention_static(const float* q, const void* k, const void* v, 
  * Format of the cache. The values of one position and kv head are cut into
  * groups of 32 dimensions; a group stores lo = f16(min), d = f16((max - lo) *
  * (1/15)) and per value the code rint((x - lo) * (1 / d)) clamped to 0..15 (0
- * where d = 0), every step rounded to f32, and stands for lo + d * code. min
+ * where d is not positive; it is negative where f16 rounds the minimum up past
+ * the maximum), every step rounded to f32, and stands for lo + d * code. min
  * and max are clamped to the f16 range first, and a NaN counts as nothing in
- * them and takes code 0. A page holds 16 positions; the caller places each layer at an offset inside it, and there a
- * kv head has one record of fbx_kv4_layer_bytes(1, D) bytes: K codes
+ * them and takes code 0. A page holds 16 positions; the caller places each layer
+ * at an offset inside it, and there a kv head has one record of fbx_kv4_layer_bytes(1, D) bytes: K codes
  * [16][D/2], K d [16][GP], K lo [16][GP], then the same three for V, GP =
  * D/32 rounded up to even. In a row of codes, with NG = D/32, K dimension
  * 32 g + 8 t + n sits in byte 4 NG t + 4 g + n/2 and V dimension

@@ -885,3 +885,51 @@ def test_packed_many_short_prompts(env, t, H, HKV, D, softcap, window):
             hit[row:last, h * D + D - 1] = True
     out = packed(env, t, q, k, vv, cu, H, HKV, D, scale, softcap, window)
     assert torch.equal(out[~hit], clean[~hit]) and not bool(torch.isfinite(out[hit]).any())
+
+
+# ------------------------------------------------------------------ values and scores at the edges
+
+
+def appended(env, k, v):
+    """One sequence's rows k, v [n][HKV][D] f32 appended without rotation: the cache, and what it holds, K, V and V's step (0
+    where the stored d is not positive, whose codes are 0) in 64 bits."""
+    lib, torch, _ = env
+    n, HKV, D = k.shape
+    c = Cache(env, [n], HKV, D, seed=n)
+    x = dev(torch, np.concatenate([k.reshape(n, -1), v.reshape(n, -1)], 1).astype(np.float32))
+    cos, sin = (dev(torch, a) for a in tables(n, 2))
+    where = [dev(torch, a.astype(np.int32)) for a in (np.zeros(n), np.arange(n))]
+    assert lib.fbx_kv4_append(c.handle, 0, None, x.data_ptr(), x.data_ptr() + 4 * HKV * D, 0, 2 * HKV * D, n, 0,
+                              where[0].data_ptr(), where[1].data_ptr(), 0, 0, cos.data_ptr(), sin.data_ptr(), n, 0, None, 0, None,
+                              None, 0, None) == 0
+    torch.cuda.synchronize()
+    held = [plain.values(*plain.quantise(y)).astype(np.float64) for y in (k, v)]
+    step = np.maximum(plain.quantise(v)[1].astype(np.float64), 0.0).repeat(32, -1)
+    return c, *held, step
+
+
+def expect(q, k, v, step, H, scale, softcap=0.0):
+    """plain.attend of one token's heads q [H][D] over all keys [n][HKV][D]: the result, mean, ext and coarse, heads first."""
+    G = H // k.shape[1]
+    parts = [plain.attend(q[h:h + 1], k[:, h // G], v[:, h // G], [len(k) - 1], scale, softcap, 0, step[:, h // G]) for h in range(H)]
+    return [np.concatenate(x) for x in zip(*parts)]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [300.13, 1000.3, -300.07, 40.03, 65000.1, 1e-3, -2.0 ** -20 * 1.3])
+def test_attention_over_groups_of_one_value(env, t, value):
+    """A group of equal values that f16 does not hold: where f16 rounds the minimum up, the stored d is negative, all codes
+    are 0, and the group stands for its lo. In every group, and beside groups of other sizes."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(17)
+    H, HKV, D, n = 8, 2, 128, 300
+    k, v = (rng.standard_normal((n, HKV, D)).astype(np.float32) for _ in range(2))
+    v[:, 0] = value
+    v[:, 1, 32:64] = value
+    v[n // 2:, 1, 96:] = value
+    v[:, 1, 64:96] *= 1e-3
+    c, kk, vv, step = appended(env, k, v)
+    q = dev(torch, rng.standard_normal((1, H * D)).astype(np.float32), t)
+    out = host(attention(env, c, t, q, H, [0], [n - 1], n, 0.1)).reshape(H, D)
+    want, *size = expect(host(q).reshape(H, D).astype(np.float64), kk, vv, step, H, 0.1)
+    near(out, want, size, t)
