@@ -245,18 +245,24 @@ __global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_co
 // which want more, take normal operands at four more instructions a word. Two
 // pages a step share the waits and checks. And no maximum is formed over a
 // page: the weights' reference is raised only when some lane's weight passes
-// 2^14, the common exponent 2^E of V's scales only when some d passes 2^(E + 1);
-// both rescale what was summed, a few times a context. With p <= 2^14 and
-// d 2^-E <= 2 the products stay in f16's range whatever the values' size is.
+// 2^kHigh, the exponent 2^E of a group's V scales only when some d passes
+// 2^(E + 1); both rescale what was summed, a few times a context. With p <= 2^7
+// and d 2^(7 - E) <= 2^8 the products stay in f16's range whatever the values'
+// size is, and d keeps all its bits down to 2^-20 of its group's largest.
 //
-// Roundings: 16-bit queries are exact in one f16 part (scaled by a power of
-// two), f32 ones go in as two, and so do their weights p d (2^-22), which meet
-// codes of -8..7 with lo + 8 d in lo's place: sums that are all of one sign, and
-// of which lo takes most away again, would leave the adder's truncation several
-// times as large in the result. For f16 outputs p d is rounded once and meets
-// codes of -8..7 too (8 sum(p d) is taken off by one more MMA a group), else the
-// rounding would be the larger part of the error; for bf16, whose own step is 8
-// times as wide, p is rounded first and codes stay 0..15.
+// Roundings: 16-bit queries go in as one f16 part, scaled by a power of two (a
+// value that is less than 2^-25 of its head's largest counts as nothing), f32
+// ones as two (2^-22, and 2^-25 of the head's largest). Weights p d of f32 calls
+// are three bf16 parts (2^-24, in f32's range, so groups and keys of any size
+// lie beside one another without an exponent). They meet codes of -8..7 with
+// lo + 8 d in lo's place: sums that are all of one sign, and of which lo takes
+// most away again, would leave the adder's truncation several times as large in
+// the result. For f16 outputs p d is rounded once and meets codes of -8..7 too
+// (8 sum(p d) is taken off by one more MMA a group), else the rounding would be
+// the larger part of the error; for bf16, whose own step is 8 times as wide, p
+// is rounded first and codes stay 0..15. In both a p d below 2^-14 of 2^(E - 7),
+// and a p below 2^-14, is held to 2^-25 of that, where a warp's largest p is 2 or
+// more.
 //
 // Measured at D = 128: 32 tokens of 4097-5100 bf16 keys, 64 heads in 8 groups,
 // 46 us, 4.1 TB/s; 64 of 2049-2180 f16 keys, 28 heads in 4 groups, 26 us, 3.3
@@ -283,6 +289,11 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -294,13 +305,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t b2_bits(__nv_bfloat162 b) { return *reinterpret_cast<uint32_t*>(&b); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
 // The 8 codes of w as f16, r[n] = (code n, code n + 4). Sub: as the subnormals
 // that they are where they lie, 2^-24 for even n and 2^-20 for odd; else as
-// they are, less Mid (dropped into the mantissa of 1024 or of 64, which is taken
-// off exactly together with Mid).
-template <bool Sub, int Mid = 0>
+// they are (dropped into the mantissa of 1024 or of 64, which is taken off
+// exactly).
+template <bool Sub>
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
     if (Sub) {
         const uint32_t u = w >> 8;
@@ -309,12 +321,21 @@ __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
         r[2] = u & 0x000F000Fu;
         r[3] = u & 0x00F000F0u;
     } else {
-        const __half2 k1024 = bits_h2(0x64006400u + Mid * 0x00010001u), k64 = bits_h2(0x54005400u + Mid * 0x00100010u);
+        const __half2 k1024 = bits_h2(0x64006400u), k64 = bits_h2(0x54005400u);
         const uint32_t u = w >> 8;
         r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), k1024));
         r[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | 0x54005400u), k64));
         r[2] = h2_bits(__hsub2(bits_h2((u & 0x000F000Fu) | 0x64006400u), k1024));
         r[3] = h2_bits(__hsub2(bits_h2((u & 0x00F000F0u) | 0x54005400u), k64));
+    }
+}
+// The same less 8, as bf16 (dropped into the mantissa of 128, which is taken off exactly together with the 8).
+__device__ __forceinline__ void codes8_mid(uint32_t w, uint32_t (&r)[4]) {
+    const uint32_t k136 = 0x43084308u;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const uint32_t u = (w >> 4 * n & 0x000F000Fu) | 0x43004300u;
+        r[n] = b2_bits(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&k136)));
     }
 }
 template <int I>   // half I of a pair as f32
@@ -344,6 +365,9 @@ __device__ __forceinline__ void halves(const uint8_t* p, uint32_t (&w)[(NG + 1) 
         words<NG / 2>(p, w);
     }
 }
+
+// a / b of powers of two
+__device__ __forceinline__ float over2(float a, float b) { return __int_as_float((127 << 23) + __float_as_int(a) - __float_as_int(b)); }
 
 struct AtArgs {
     fbx_kv4_cache c;
@@ -375,8 +399,8 @@ struct AtSmem {
 };
 
 // how the weights of an element type go into the products with V (see above)
-enum : int { W_PAIR, W_MID, W_HALF };
-template <class E> struct AtWeights { static constexpr int mode = W_PAIR; };
+enum : int { W_PARTS, W_MID, W_HALF };
+template <class E> struct AtWeights { static constexpr int mode = W_PARTS; };
 template <> struct AtWeights<__half> { static constexpr int mode = W_MID; };
 template <> struct AtWeights<__nv_bfloat16> { static constexpr int mode = W_HALF; };
 
@@ -385,7 +409,9 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     using R = Kv4Rec<D>;
     using M = AtSmem<D>;
     constexpr int NG = R::NG, GP = R::GP, PL = sizeof(E) == 4 ? 2 : 1, W = AtWeights<E>::mode;
-    constexpr bool SUB = W != W_PAIR;
+    constexpr bool SUB = W != W_PARTS;
+    // a weight passes 2^kHigh: the reference becomes the largest score less kTo
+    constexpr float kHigh = SUB ? 7.0f : 14.0f, kTo = SUB ? 1.0f : 8.0f;
     constexpr float kCode = SUB ? 1048576.0f : 1.0f;   // a code over its operand
     extern __shared__ __align__(128) uint8_t sm[];
     const fbx_kv4_cache& c = A.c;
@@ -490,17 +516,19 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     for (int i = 0; i < 2; ++i)
         cs[i] = A.scale * reinterpret_cast<const float*>(sm + M::ex)[2 * t + i] * (cap ? 1.0f / A.softcap : kLog2e);
     float ref[2] = {kNoRef, kNoRef}, sum[2] = {0.0f, 0.0f};
-    int top_e = 0;                          // E
-    __half2 down_e = __float2half2_rn(0.0f), limit_e = down_e;   // 2^-E, 2^(E + 1); a limit of 0 is passed by the first page
-    // O^T 2^-E / kCode: dims 32 e + 4 g + 2 u (accumulators 0, 1) and the next (2, 3), heads 2 t + (0, 1)
-    float o[NG][2][4], olo[NG][2], mid[W == W_MID ? NG : 1][4];
+    __half2 down_e[GP / 2];   // 2^(7 - E) of the groups 2 e, 2 e + 1, E from -8 on
+#pragma unroll
+    for (int e = 0; e < GP / 2; ++e) down_e[e] = bits_h2(0x78007800u);   // 2^15
+    // O^T 2^(7 - E) / kCode (O^T for f32 calls): dims 32 e + 4 g + 2 u (accumulators 0, 1) and the next (2, 3), heads 2 t + (0, 1)
+    // mid: -8 sum(p d) 2^(7 - E) / (16 kCode) of the groups 2 e (accumulators 0, 1) and 2 e + 1 (2, 3)
+    float o[NG][2][4], olo[NG][2], mid[GP / 2][4];
 #pragma unroll
     for (int e = 0; e < NG; ++e) {
         olo[e][0] = olo[e][1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             o[e][0][i] = o[e][1][i] = 0.0f;
-            if (W == W_MID) mid[e][i] = 0.0f;
+            if (W == W_MID) mid[e / 2][i] = 0.0f;
         }
     }
     const int row = kv4_key(g);   // and row + 8
@@ -555,12 +583,6 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             words<GP / 2>(rec + R::vlo + row * GP * 2, u0[h]);
             words<GP / 2>(rec + R::vlo + (row + 8) * GP * 2, u1[h]);
             if (NG == 3) v0[h][1] &= 0xFFFFu, v1[h][1] &= 0xFFFFu;
-            // a d below 0 has codes of 0 only (f16 rounded the group's minimum up past its maximum): it counts as 0
-#pragma unroll
-            for (int e = 0; e < GP / 2; ++e) {
-                v0[h][e] = h2_bits(__hmax2_nan(bits_h2(v0[h][e]), bits_h2(0u)));
-                v1[h][e] = h2_bits(__hmax2_nan(bits_h2(v1[h][e]), bits_h2(0u)));
-            }
         }
         if (cap) {
 #pragma unroll
@@ -585,50 +607,82 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 }
             }
         }
-        // ---- the references, raised when a weight passes 2^14 or a scale 2^(E + 1)
-        __half2 dm = __hmax2(__hmax2(bits_h2(v0[0][0]), bits_h2(v1[0][0])), __hmax2(bits_h2(v0[1][0]), bits_h2(v1[1][0])));
+        // ---- the references, raised when a weight passes 2^kHigh or a d passes 2^(E + 1)
+        __half2 dm[GP / 2];
+        bool wide = false;
+        if (SUB) {
 #pragma unroll
-        for (int e = 1; e < GP / 2; ++e)
-            dm = __hmax2(dm, __hmax2(__hmax2(bits_h2(v0[0][e]), bits_h2(v1[0][e])), __hmax2(bits_h2(v0[1][e]), bits_h2(v1[1][e]))));
-        const float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
-        const float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
-        const bool wide = !__hble2(dm, limit_e), high = fmaxf(mx0 - ref[0], mx1 - ref[1]) > 14.0f;
-        if (__any_sync(0xffffffffu, wide || high)) {
-            float mx[2] = {mx0, mx1}, dtop = fmaxf(__low2float(dm), __high2float(dm));
-#pragma unroll
-            for (int w = 4; w <= 16; w <<= 1) {
-                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
-                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
-                dtop = fmaxf(dtop, __shfl_xor_sync(0xffffffffu, dtop, w));
-            }
-            const int e_new = max((int)(__float_as_uint(fmaxf(dtop, 0.0f)) >> 23) - 127, -15);   // d < 2^(e_new + 1)
-            float f_e = 1.0f;
-            if (limit_e.x == __half(0.0f) || e_new > top_e) {
-                f_e = limit_e.x == __half(0.0f) ? 1.0f : __int_as_float((127 + top_e - e_new) << 23);
-                top_e = e_new;
-                down_e = __float2half2_rn(__int_as_float((127 - e_new) << 23));
-                limit_e = __float2half2_rn(__int_as_float((128 + e_new) << 23));
-            }
-            float f[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float to = mx[i] - ref[i] > 14.0f ? mx[i] - 8.0f : ref[i];
-                f[i] = to == ref[i] ? 1.0f : at_ex2(ref[i] - to);
-                ref[i] = to;
-                sum[i] *= f[i];
-            }
-#pragma unroll
-            for (int e = 0; e < NG; ++e) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[e][0][i] *= f[i & 1] * f_e;
-                    o[e][1][i] *= f[i & 1] * f_e;
-                    if (W == W_MID) mid[e][i] *= f[i & 1] * f_e;
-                }
-                olo[e][0] *= f[0];
-                olo[e][1] *= f[1];
+            for (int e = 0; e < GP / 2; ++e) {
+                dm[e] = __hmax2(__hmax2(bits_h2(v0[0][e]), bits_h2(v1[0][e])), __hmax2(bits_h2(v0[1][e]), bits_h2(v1[1][e])));
+                wide |= !__hble2(__hmul2(dm[e], down_e[e]), bits_h2(0x5C005C00u));   // 2^8
             }
         }
+        const float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+        const float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+        const bool high = fmaxf(mx0 - ref[0], mx1 - ref[1]) > kHigh;
+        if (__any_sync(0xffffffffu, wide || high)) {
+            if (SUB && __any_sync(0xffffffffu, wide)) {
+#pragma unroll
+                for (int e2 = 0; e2 < GP / 2; ++e2) {
+#pragma unroll
+                    for (int w = 4; w <= 16; w <<= 1) dm[e2] = __hmax2(dm[e2], bits_h2(__shfl_xor_sync(0xffffffffu, h2_bits(dm[e2]), w)));
+                    float down[2] = {__low2float(down_e[e2]), __high2float(down_e[e2])};
+                    const float d[2] = {__low2float(dm[e2]), __high2float(dm[e2])};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = 2 * e2 + i;
+                        if (e >= NG || !(d[i] * down[i] > 256.0f)) continue;
+                        // d < 2^E, so that the ones to come seldom raise E again
+                        const int E = (int)(__float_as_uint(d[i]) >> 23) - 127 + 1;
+                        const float to = __int_as_float((127 + 7 - E) << 23), f = over2(to, down[i]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            o[e][0][k] *= f;
+                            o[e][1][k] *= f;
+                        }
+                        if (W == W_MID) mid[e2][2 * i] *= f, mid[e2][2 * i + 1] *= f;
+                        down[i] = to;
+                    }
+                    down_e[e2] = __floats2half2_rn(down[0], down[1]);
+                }
+            }
+            if (__any_sync(0xffffffffu, high)) {
+                float mx[2] = {mx0, mx1}, f[2];
+#pragma unroll
+                for (int w = 4; w <= 16; w <<= 1) {
+                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
+                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float to = mx[i] - ref[i] > kHigh ? mx[i] - kTo : ref[i];
+                    f[i] = to == ref[i] ? 1.0f : at_ex2(ref[i] - to);
+                    ref[i] = to;
+                    sum[i] *= f[i];
+                }
+#pragma unroll
+                for (int e = 0; e < NG; ++e) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[e][0][i] *= f[i & 1];
+                        o[e][1][i] *= f[i & 1];
+                    }
+                    if (W == W_MID) mid[e / 2][2 * (e & 1)] *= f[0], mid[e / 2][2 * (e & 1) + 1] *= f[1];
+                    olo[e][0] *= f[0];
+                    olo[e][1] *= f[1];
+                }
+            }
+        }
+        // ---- d 2^(7 - E), or d, in d's place; one below 0 has codes of 0 only (f16 rounded the group's minimum up past its
+        // maximum) and counts as 0
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < GP / 2; ++e) {
+                const __half2 a = bits_h2(v0[h][e]), b = bits_h2(v1[h][e]), zero = bits_h2(0u);
+                v0[h][e] = h2_bits(SUB ? __hfma2_relu(a, down_e[e], zero) : __hmax2_nan(a, zero));
+                v1[h][e] = h2_bits(SUB ? __hfma2_relu(b, down_e[e], zero) : __hmax2_nan(b, zero));
+            }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float p[4];
@@ -646,42 +700,54 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             halves<NG>(vr + (vrow2 + 8) * R::row, vd);
 #pragma unroll
             for (int e = 0; e < NG; ++e) {
-                const __half2 n0 = __hmul2(bits_h2(v0[h][e / 2]), down_e), n1 = __hmul2(bits_h2(v1[h][e / 2]), down_e);   // d 2^-E
+                const float da = e & 1 ? half_at<1>(v0[h][e / 2]) : half_at<0>(v0[h][e / 2]);
+                const float db = e & 1 ? half_at<1>(v1[h][e / 2]) : half_at<0>(v1[h][e / 2]);
                 float la = e & 1 ? half_at<1>(u0[h][e / 2]) : half_at<0>(u0[h][e / 2]);
                 float lb = e & 1 ? half_at<1>(u1[h][e / 2]) : half_at<0>(u1[h][e / 2]);
                 if (W != W_HALF) {
-                    la = fmaf(8.0f, e & 1 ? half_at<1>(v0[h][e / 2]) : half_at<0>(v0[h][e / 2]), la);
-                    lb = fmaf(8.0f, e & 1 ? half_at<1>(v1[h][e / 2]) : half_at<0>(v1[h][e / 2]), lb);
+                    // 8, or 8 2^(E - 7): the exponents of that and of 2^(7 - E) add up to 3
+                    const float k = W == W_MID ? (e & 1 ? half_at<1>(0x84008400u - h2_bits(down_e[e / 2])) : half_at<0>(0x84008400u - h2_bits(down_e[e / 2]))) : 8.0f;
+                    la = fmaf(k, da, la);
+                    lb = fmaf(k, db, lb);
                 }
                 olo[e][0] = fmaf(p[0], la, fmaf(p[2], lb, olo[e][0]));
                 olo[e][1] = fmaf(p[1], la, fmaf(p[3], lb, olo[e][1]));
                 uint32_t ra[4], rc[4];
-                codes8<SUB, W == W_PAIR ? 8 : 0>(__byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410), ra);
-                codes8<SUB, W == W_PAIR ? 8 : 0>(__byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410), rc);
+                const uint32_t wa = __byte_perm(va[e / 2], vb[e / 2], e & 1 ? 0x7632 : 0x5410);
+                const uint32_t wc = __byte_perm(vc[e / 2], vd[e / 2], e & 1 ? 0x7632 : 0x5410);
+                if constexpr (W == W_PARTS) {
+                    codes8_mid(wa, ra);
+                    codes8_mid(wc, rc);
+                    float x[4] = {p[0] * da, p[1] * da, p[2] * db, p[3] * db};
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) {
+                        const __nv_bfloat162 y0 = __floats2bfloat162_rn(x[0], x[1]), y1 = __floats2bfloat162_rn(x[2], x[3]);
+                        const uint32_t b0 = transpose8(b2_bits(y0)), b1 = transpose8(b2_bits(y1));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) mma16_bf16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
+                        x[0] -= __low2float(y0);
+                        x[1] -= __high2float(y0);
+                        x[2] -= __low2float(y1);
+                        x[3] -= __high2float(y1);
+                    }
+                    continue;
+                }
+                codes8<SUB>(wa, ra);
+                codes8<SUB>(wc, rc);
                 __half2 hi0, hi1;
-                float x[4];
                 if (W == W_HALF) {
-                    hi0 = __hmul2(p0, e & 1 ? __high2half2(n0) : __low2half2(n0));
-                    hi1 = __hmul2(p1, e & 1 ? __high2half2(n1) : __low2half2(n1));
+                    hi0 = __hmul2(p0, e & 1 ? __high2half2(bits_h2(v0[h][e / 2])) : __low2half2(bits_h2(v0[h][e / 2])));
+                    hi1 = __hmul2(p1, e & 1 ? __high2half2(bits_h2(v1[h][e / 2])) : __low2half2(bits_h2(v1[h][e / 2])));
                 } else {
-                    const float da = e & 1 ? __high2float(n0) : __low2float(n0), db = e & 1 ? __high2float(n1) : __low2float(n1);
-                    x[0] = p[0] * da;
-                    x[1] = p[1] * da;
-                    x[2] = p[2] * db;
-                    x[3] = p[3] * db;
-                    hi0 = __floats2half2_rn(x[0], x[1]);
-                    hi1 = __floats2half2_rn(x[2], x[3]);
+                    hi0 = __floats2half2_rn(p[0] * da, p[1] * da);
+                    hi1 = __floats2half2_rn(p[2] * db, p[3] * db);
                 }
                 const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
-                if (W == W_MID) mma16(mid[e], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);   // -8, even and odd dims
-                if (W == W_PAIR) {
-                    const float2 y0 = __half22float2(hi0), y1 = __half22float2(hi1);
-                    const uint32_t c0 = transpose8(h2_bits(__floats2half2_rn(x[0] - y0.x, x[1] - y0.y)));
-                    const uint32_t c1 = transpose8(h2_bits(__floats2half2_rn(x[2] - y1.x, x[3] - y1.y)));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], c0, c1);
+                if (W == W_MID) {   // -8 in the upper or lower 8 rows
+                    const uint32_t a = e & 1 ? 0u : 0x80088008u, b = e & 1 ? 0x80088008u : 0u;
+                    mma16(mid[e / 2], a, b, a, b, b0, b1);
                 }
             }
         }
@@ -712,10 +778,11 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         }
 #pragma unroll
         for (int e = 0; e < NG; ++e) {
-            const float up = __int_as_float((127 + top_e) << 23) * kCode, ev = SUB ? 16.0f * up : up;   // odd and even dimensions
-            const float lo = olo[e][i] + (W == W_MID ? ev * mid[e][i] : 0.0f), lo1 = olo[e][i] + (W == W_MID ? up * mid[e][2 + i] : 0.0f);
+            // odd and even dimensions
+            const float up = SUB ? over2(kCode, half_at<0>(h2_bits(down_e[e / 2]) >> (e & 1 ? 16 : 0))) : 1.0f, ev = SUB ? 16.0f * up : up;
+            const float lo = olo[e][i] + (W == W_MID ? ev * mid[e / 2][2 * (e & 1) + i] : 0.0f);
             *reinterpret_cast<float4*>(so + (warp * 8 + h) * (D + 4) + 32 * e + 4 * g) =
-                make_float4(fmaf(ev, o[e][0][i], lo), fmaf(up, o[e][0][2 + i], lo1), fmaf(ev, o[e][1][i], lo), fmaf(up, o[e][1][2 + i], lo1));
+                make_float4(fmaf(ev, o[e][0][i], lo), fmaf(up, o[e][0][2 + i], lo), fmaf(ev, o[e][1][i], lo), fmaf(up, o[e][1][2 + i], lo));
         }
     }
     __syncthreads();

@@ -933,3 +933,51 @@ def test_attention_over_groups_of_one_value(env, t, value):
     out = host(attention(env, c, t, q, H, [0], [n - 1], n, 0.1)).reshape(H, D)
     want, *size = expect(host(q).reshape(H, D).astype(np.float64), kk, vv, step, H, 0.1)
     near(out, want, size, t)
+
+
+def outlier_slack(t, n, step):
+    """What rounding to f16 may add for 16-bit types where the steps of a group lie far apart: a weight times its step is held to
+    2^-25 of 2^(E - 7), 2^E the largest step's power of two, and meets codes of up to 15, against a sum of weights of 2 or
+    more; n keys."""
+    if t == "f32":
+        return 0.0
+    return n * 15 * 2.0 ** -26 * 2.0 ** (np.floor(np.log2(step.max(0))) - 7)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_attention_over_groups_far_apart(env, t, D):
+    """V's groups of one head 2^12 to 2^22 apart: each keeps the precision that it has alone."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(D)
+    H, HKV, n = 4, 2, 200
+    G, scale = H // HKV, 1.0 / np.sqrt(D)
+    k, v = (rng.standard_normal((n, HKV, D)).astype(np.float32) for _ in range(2))
+    sizes = np.array([2.0 ** 10, 2.0 ** -2, 2.0 ** -12, 2.0 ** -8])[:D // 32].repeat(32)
+    c, kk, vv, step = appended(env, k, (v * sizes).astype(np.float32))
+    q = dev(torch, rng.standard_normal((1, H * D)).astype(np.float32), t)
+    out = host(attention(env, c, t, q, H, [0], [n - 1], n, scale)).reshape(H, D)
+    want, *size = expect(host(q).reshape(H, D).astype(np.float64), kk, vv, step, H, scale)
+    near(out, want, size, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("at", [0, 37, 59])
+def test_attention_beside_a_key_of_huge_values(env, t, at):
+    """One key whose V is 2^20 times the others' and whose weight is e^-64: it takes no bits from them."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(at)
+    H, D, n = 4, 128, 60
+    k = np.zeros((n, 1, D), np.float32)
+    v = np.tile(rng.standard_normal((1, 1, D)), (n, 1, 1)).astype(np.float32) * 2.0 ** -7
+    k[at, 0, 0] = -64
+    v[at] *= 2.0 ** 20
+    c, kk, vv, step = appended(env, k, v)
+    q = torch.zeros((1, H * D), device="cuda").to(dtype(torch, t))
+    q.view(H, D)[:, 0] = 1.0
+    out = host(attention(env, c, t, q, H, [0], [n - 1], n, 1.0)).reshape(H, D)
+    want, mean, ext, coarse = expect(host(q).reshape(H, D).astype(np.float64), kk, vv, step, H, 1.0)
+    # the outlier's own score is exact enough: its weight does not matter; the others' scores are 0
+    tol = plain.allowed(want, mean, ext * 0, t, 2.0 ** -22 if t == "f32" else 2.0 ** -11, 0.0, coarse) + outlier_slack(t, n, step[:, 0])
+    off = np.abs(out - want)
+    assert (off <= tol).all(), (off / tol).max()
