@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_co
 // CTAs of four warps (53), scores of the next pages under this one's products.
 constexpr int kAtWarps = 8, kSlots = 2;
 constexpr int kMaxCluster = 8;
-constexpr float kNoRef = -1e30f;   // before the first key: finite, so that a key outside (-inf) weighs 0 against it
+constexpr float kNoRef = -3.4028235e38f;   // before the first key: below every score, and finite, so that a key outside (-inf) weighs 0
 
 // key of row r of the 16-row operand tiles
 __device__ __forceinline__ int kv4_key(int r) { return (r & 8) | (r & 1 ? 4 + (((r >> 1) & 3) ^ 1) : (r >> 1) & 3); }

@@ -981,3 +981,21 @@ def test_attention_beside_a_key_of_huge_values(env, t, at):
     tol = plain.allowed(want, mean, ext * 0, t, 2.0 ** -22 if t == "f32" else 2.0 ** -11, 0.0, coarse) + outlier_slack(t, n, step[:, 0])
     off = np.abs(out - want)
     assert (off <= tol).all(), (off / tol).max()
+
+
+@pytest.mark.parametrize("t,size,scale,cap,n,H", [
+    ("f32", 1e32, 0.1, 0.0, 1, 4), ("f32", 1e34, 0.1, 0.0, 600, 8), ("f32", 1e36, 0.5, 0.0, 3000, 1), ("f16", 1.0, 1e30, 0.0, 90, 8),
+    ("bf16", 2.0 ** 110, 0.1, 0.0, 400, 8), ("bf16", 1e35, 0.5, 1e30, 600, 8), ("f16", 100.0, 1e29, 1e30, 33, 4),
+])
+def test_attention_of_scores_far_below_zero(env, t, size, scale, cap, n, H):
+    """Scores that are finite, equal, and lower than -1e30: the weights are equal. One split, clusters, a second launch."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(n)
+    D = 128
+    k = np.ones((n, 1, D), np.float32)
+    v = rng.standard_normal((n, 1, D)).astype(np.float32)
+    c, kk, vv, step = appended(env, k, v)
+    q = torch.full((1, H * D), -size, device="cuda").to(dtype(torch, t))
+    out = host(attention(env, c, t, q, H, [0], [n - 1], n, scale, cap)).reshape(H, D)
+    want, mean, ext, coarse = expect(np.zeros((H, D)), kk, vv, step, H, 1.0)
+    near(out, want, (mean, ext, coarse), t)
