@@ -82,7 +82,7 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* c, int type, const void* q, con
     // in place means the same rows
     if (q && q == q_out && (type != out_type || ldq != ldq_out)) return -1;
     if ((k == k_out || v == v_out) && (type != out_type || ldkv != ldkv_out)) return -1;
-    const int rc = on_device({c->pool, c->page_table, q, k, tok_pos, rope_cos, q_out, k_out});
+    const int rc = on_device({c->pool, c->page_table, c->err, q, k, tok_pos, rope_cos, q_out, k_out ? k_out : v_out});
     if (rc) return rc;
     return fbk_kv4_append(*c, type, q, k, v, ldq, ldkv, T, H, tok_seq, tok_pos, rot, neox ? 1 : 0, rope_cos, rope_sin, n_rope,
                           out_type, q_out, ldq_out, k_out, v_out, ldkv_out, static_cast<cudaStream_t>(stream));
@@ -105,7 +105,7 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* c, int type, const void* q, 
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
     const size_t need = fbk_kv4_attention_workspace(T, H, HKV, D, max_keys);
     if (need && (!workspace || workspace_bytes < need)) return -1;
-    const int rc = on_device({c->pool, c->page_table, q, tok_pos, out, need ? workspace : nullptr});
+    const int rc = on_device({c->pool, c->page_table, c->err, q, tok_pos, out, need ? workspace : nullptr});
     if (rc) return rc;
     return fbk_kv4_attention(*c, type, q, ldq, T, H, tok_seq, tok_pos, max_keys, scale, softcap, window, out, ldo, workspace,
                              static_cast<cudaStream_t>(stream));

@@ -130,7 +130,8 @@ FISH_API int fbx_attention_static(const float* q, const void* k, const void* v, 
  * (including a buffer that is not memory of the current device, and an address
  * or row stride that is not a multiple of 16 bytes), or a positive CUDA error;
  * of k and v, of tok_seq and tok_pos, of the two tables and of k_out and v_out
- * one is looked at, and the other has to lie in memory of the same kind. With
+ * one is looked at where both are given, and the other has to lie in memory of
+ * the same kind. With
  * no tokens or rows nothing is done, and buffers may be NULL.
  * `type` is an element type: 0 F32, 1 F16, 30 BF16 (ggml's ids). Row strides
  * (ld..) are in elements. No counterpart in the reference, whose cache is f32

@@ -999,3 +999,52 @@ def test_attention_of_scores_far_below_zero(env, t, size, scale, cap, n, H):
     out = host(attention(env, c, t, q, H, [0], [n - 1], n, scale, cap)).reshape(H, D)
     want, mean, ext, coarse = expect(np.zeros((H, D)), kk, vv, step, H, 1.0)
     near(out, want, (mean, ext, coarse), t)
+
+
+def test_host_arrays_are_refused_wherever_they_stand(env):
+    """A host array in any place that is looked at: -1, and nothing is launched. Each place in turn, all others good; of the
+    pairs the one that is looked at, and the other where it stands alone."""
+    lib, torch, native = env
+    H, HKV, D, n = 8, 2, 128, 64
+    c = Cache(env, [n], HKV, D)
+    keep = np.zeros(1 << 16, np.uint8)
+    addr = (keep.ctypes.data + 15) // 16 * 16
+    x = torch.randn((1, (H + 2 * HKV) * D), device="cuda")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cos, sin = (dev(torch, a) for a in tables(n, D))
+    out = torch.full((3, H * D), 7.0, device="cuda")
+    ws = torch.zeros(lib.fbx_kv4_attention_workspace(1, H, HKV, D, 1 << 17), dtype=torch.uint8, device="cuda")
+    pool = c.pool.clone()
+
+    def handle(**k):
+        h = {f: getattr(c.handle, f) for f, _ in native.Kv4Cache._fields_}
+        return native.Kv4Cache(**{**h, **k})
+
+    def append(h=None, **k):
+        p, ld = x.data_ptr(), x.shape[1]
+        a = dict(type=0, q=p, k=p + 4 * H * D, v=p + 4 * (H + HKV) * D, ldq=ld, ldkv=ld, T=1, H=H, seq=zero.data_ptr(),
+                 pos=zero.data_ptr(), rot=D, neox=0, cos=cos.data_ptr(), sin=sin.data_ptr(), n_rope=n, out=0, q_out=out.data_ptr(),
+                 ldqo=H * D, k_out=out[1].data_ptr(), v_out=out[2].data_ptr(), ldkvo=HKV * D)
+        a.update(k)
+        return lib.fbx_kv4_append(h or c.handle, *a.values(), None)
+
+    def attend(h=None, **k):
+        a = dict(type=0, q=x.data_ptr(), ldq=H * D, T=1, H=H, seq=zero.data_ptr(), pos=zero.data_ptr(), keys=1 << 17, scale=0.1,
+                 cap=0.0, window=0, out=out.data_ptr(), ldo=H * D, ws=ws.data_ptr(), size=ws.numel())
+        a.update(k)
+        return lib.fbx_kv4_attention(h or c.handle, *a.values(), None)
+
+    assert ws.numel() > 0   # a second launch joins the splits
+    for bad in ({"pool": addr}, {"page_table": addr}, {"err": addr}):
+        assert append(handle(**bad)) == -1 and attend(handle(**bad)) == -1
+    for bad in ({"q": addr}, {"k": addr}, {"pos": addr}, {"cos": addr}, {"q_out": addr}, {"k_out": addr},
+                {"k_out": None, "v_out": addr}, {"k_out": addr, "v_out": None}):
+        assert append(**bad) == -1
+    for bad in ({"q": addr}, {"pos": addr}, {"out": addr}, {"ws": addr}):
+        assert attend(**bad) == -1
+    torch.cuda.synchronize()
+    assert bool((out == 7).all()) and torch.equal(c.pool, pool)
+    # each output of k and v alone
+    assert append(k_out=None) == 0 and append(v_out=None) == 0
+    assert append(handle(err=None), k_out=None, v_out=None) == 0 and attend(handle(err=None)) == 0
+    torch.cuda.synchronize()
