@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <climits>
+#include <initializer_list>
 
 #include "kernels/kv4.cuh"
 
@@ -14,6 +15,12 @@ using namespace fb;
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// arrays of 32-bit values; null passes
+bool aligned4(std::initializer_list<const void*> ps) {
+    uintptr_t all = 0;
+    for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
+    return (all & 3) == 0;
+}
 size_t type_bytes(int type) { return type == T_F32 ? 4 : type == T_F16 || type == T_BF16 ? 2 : 0; }
 constexpr float kMost = 1e30f;
 // what scores are multiplied by stays finite
@@ -47,7 +54,7 @@ int on_device(std::initializer_list<const void*> ps) {
 }
 
 bool cache_ok(const fbx_kv4_cache* c) {
-    if (!c || !c->pool || !c->page_table || !aligned16(c->pool)) return false;
+    if (!c || !c->pool || !c->page_table || !aligned16(c->pool) || !aligned4({c->page_table, c->err})) return false;
     const size_t layer = fbx_kv4_layer_bytes(c->n_head_kv, c->head_dim);
     return layer && c->n_pages > 0 && c->table_stride > 0 && c->n_seqs > 0 && c->layer_offset >= 0 &&
            c->layer_offset % 16 == 0 && c->page_stride % 16 == 0 && c->page_stride - c->layer_offset >= (int64_t)layer;
@@ -79,6 +86,7 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* c, int type, const void* q, con
     if ((k_out || v_out) && !stride_ok(ldkv_out, (int64_t)HKV * D, out_type)) return -1;
     for (const void* p : {q, k, v, (const void*)q_out, (const void*)k_out, (const void*)v_out})
         if (!aligned16(p)) return -1;
+    if (!aligned4({tok_seq, tok_pos, rope_cos, rope_sin})) return -1;
     // in place means the same rows
     if (q && q == q_out && (type != out_type || ldq != ldq_out)) return -1;
     if ((k == k_out || v == v_out) && (type != out_type || ldkv != ldkv_out)) return -1;
@@ -102,7 +110,7 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* c, int type, const void* q, 
     const int D = c->head_dim, HKV = c->n_head_kv;
     if (H <= 0 || H > 65535 || H % HKV || !scale_ok(scale, softcap) || window < 0) return -1;
     if (!stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldo, (int64_t)H * D, type)) return -1;
-    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || !aligned4({tok_seq, tok_pos})) return -1;
     const size_t need = fbk_kv4_attention_workspace(T, H, HKV, D, max_keys);
     if (need && (!workspace || workspace_bytes < need)) return -1;
     const int rc = on_device({c->pool, c->page_table, c->err, q, tok_pos, out, need ? workspace : nullptr});
@@ -122,7 +130,7 @@ FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const vo
     if (!stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldkv, (int64_t)HKV * D, type) ||
         !stride_ok(ldo, (int64_t)H * D, type))
         return -1;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return -1;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned4({cu_seqlens})) return -1;
     const int rc = on_device({q, k, cu_seqlens, out});
     if (rc) return rc;
     return fbk_attention_packed(type, q, ldq, k, v, ldkv, n_rows, cu_seqlens, n_seqs, H, HKV, D, scale, softcap, window, out,

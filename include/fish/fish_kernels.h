@@ -127,8 +127,9 @@ FISH_API int fbx_attention_static(const float* q, const void* k, const void* v, 
  * cudaStream_t of the current device, NULL = default stream) without waiting
  * for it; they allocate nothing, so they can be captured into a graph from the
  * first call on. They return 0, -1 for arguments that cannot be right
- * (including a buffer that is not memory of the current device, and an address
- * or row stride that is not a multiple of 16 bytes), or a positive CUDA error;
+ * (including a buffer that is not memory of the current device, an address or
+ * row stride of rows that is not a multiple of 16 bytes, and an address of an
+ * array of 32-bit values that is not one of 4), or a positive CUDA error;
  * of k and v, of tok_seq and tok_pos, of the two tables and of k_out and v_out
  * one is looked at where both are given, and the other has to lie in memory of
  * the same kind. With

@@ -140,3 +140,16 @@ def test_empty_calls_need_no_buffers(lib):
 @pytest.mark.parametrize("bad", [dict(softcap=1e-31), dict(scale=1e20, softcap=1e-15), dict(scale=2e30), dict(softcap=2e30)])
 def test_scales_that_could_overflow_are_refused(lib, bad):
     assert attend(lib, **bad) == -1 and packed(lib, **bad) == -1
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_arrays_of_32_bit_values_off_their_boundary_are_refused(lib, off):
+    """Sequences, positions, tables, the page table, the error word and the lengths: an unaligned load would fault."""
+    at = 4096 + off
+    for bad in (dict(seq=at), dict(pos=at), dict(cos=at), dict(sin=at)):
+        assert append(lib, **bad) == -1
+    for bad in (dict(seq=at), dict(pos=at)):
+        assert attend(lib, **bad) == -1
+    for bad in (dict(page_table=at), dict(err=at)):
+        assert append(lib, cache(**bad)) == -1 and attend(lib, cache(**bad)) == -1
+    assert packed(lib, cu=at) == -1
