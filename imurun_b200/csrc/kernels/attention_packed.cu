@@ -219,14 +219,26 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
     return *reinterpret_cast<float2*>(&r);
 }
-// Waits of the roles. A wait that runs out (some 10 ms at least) marks the CTA: every role then goes through its loops without
-// waiting, on whatever lies in shared and tensor memory, and the CTA ends.
-__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n)
-        if ((n & 255) == 0 && (*abort || n >= 1u << 22)) {
-            *abort = 1;
-            break;
+// Waits of the roles. Some last as long as a job, which has no bound, so a wait runs out after kTries tries (0.2 s at least) in
+// which the CTA made no progress: state[1], which the warp of the products counts up at every key tile, stood still. The most
+// that the CTA does between two tiles is to look up a job past a million empty sequences, some 30 ms. A wait that ran out
+// marks the CTA (state[0]): every role goes through its loops without waiting, on whatever lies in shared and tensor memory,
+// and the CTA ends. Tries and not the clock: its reading at every wait's place cost short prompts 1 us of 23.
+constexpr uint32_t kTries = 1u << 24;
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* state) {
+    int at = -1;
+    for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
+        if ((n & 255) != 0) continue;
+        if (state[0]) break;
+        if (n >= kTries) {
+            if (state[1] == at) {
+                state[0] = 1;
+                break;
+            }
+            at = state[1];
+            n = 0;
         }
+    }
 }
 __device__ __forceinline__ uint32_t ones(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }   // the low n bits
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -297,14 +309,14 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + M::bar);
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + M::bar + 8 * M::B_COUNT);
-    volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-    volatile int* s_odd = s_abort + 1;   // [2 NJ] jobs (counted from 1) in which values that are not finite were met
+    volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);   // and the progress: see wait()
+    volatile int* s_odd = s_abort + 2;   // behind the progress: [2 NJ] jobs (counted from 1) in which values that are not finite were met
     volatile int4* s_job = reinterpret_cast<volatile int4*>(s_tmem + 12);   // [NJ] jobs, with the kv head
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = A.R, G = A.G;
     pdl_trigger();
     if (threadIdx.x == kSoft) {
-        *s_abort = 0;
+        s_abort[0] = s_abort[1] = 0;
         for (int i = 0; i < 2 * NJ; ++i) s_odd[i] = 0;
         for (int i = 0; i < M::B_COUNT; ++i) {
             mbar_init(&bar[i], i >= B_EMPTY && i < B_CLEAN ? 33 : i >= B_CLEAN && i < B_S ? 32 : i >= B_P && i < B_O ? 128 : i >= B_TAKEN ? 11 : 1);
@@ -403,6 +415,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
             uint32_t fresh[2] = {1, 1};
             for (int j = ks.j0; j < ks.j1; ++j) {   // V_j and K_{j+NB} in place i
                 const bool more = j + 1 < ks.j1;
+                if (who) s_abort[1] = i;
                 if (ks.masked(j)) {
                     const int z = i % NS;
                     wait(&bar[B_CLEAN + z], clean >> z & 1, s_abort);

@@ -213,8 +213,8 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
  * division, so sums stay finite for values of v up to 10^36 / n_rows. The
  * tiles, and with them the last bits of a row, go by the batch's lengths. Rows
  * of out outside every sequence stay as they were. The kernel's waits for its
- * own copies and products are bounded (some 10 ms each): if one ran out, rows
- * of out would be NaN or stay as they were. */
+ * own copies and products end after 0.2 s or more in which it made no progress:
+ * if one ran out, rows of out would be NaN or stay as they were. */
 FISH_API int fbx_attention_packed(int type, const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
                                   int n_rows, const int32_t* cu_seqlens, int n_seqs, int H, int HKV, int D, float scale,
                                   float softcap, int window, void* out, int64_t ldo, void* stream);

@@ -1048,3 +1048,31 @@ def test_host_arrays_are_refused_wherever_they_stand(env):
     assert append(k_out=None) == 0 and append(v_out=None) == 0
     assert append(handle(err=None), k_out=None, v_out=None) == 0 and attend(handle(err=None)) == 0
     torch.cuda.synchronize()
+
+
+def rows64(torch, rows, q, k, v, H, HKV, D, scale, start=0):
+    """packed64 of some rows (counted from their sequence's first row `start`)."""
+    G = H // HKV
+    want, mean, ext = [], [], []
+    for r in rows:
+        x = q[start + r].view(HKV, G, D).double()
+        kk, vv = (y[start:start + r + 1].view(r + 1, HKV, D).transpose(0, 1).double() for y in (k, v))
+        s = x @ kk.transpose(1, 2) * scale
+        w = torch.softmax(s, -1)
+        want.append((w @ vv).reshape(-1))
+        mean.append((w @ vv.abs()).reshape(-1))
+        ext.append((x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(-1) * scale)
+    return [torch.stack(y).cpu().numpy() for y in (want, mean, ext)]
+
+
+def test_packed_prompt_of_a_million_rows(env):
+    """A job of 8192 key tiles, some 10 ms: the warps that wait for its end wait as long as it goes on."""
+    lib, torch, _ = env
+    n, D = (1 << 20) + 77, 64
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn((n, D), device="cuda", generator=gen).bfloat16() for _ in range(3))
+    cu = dev(torch, np.array([0, n], np.int32))
+    out = packed(env, "bf16", q, k, v, cu, 1, 1, D, 0.125)
+    rows = [0, 1, 127, 128, 5000, n // 3, n // 2, n - 400, n - 130, n - 77, n - 2, n - 1]
+    check_packed(host(out[rows]), *rows64(torch, rows, q, k, v, 1, 1, D, 0.125), 1, D, "bf16", 0.0, len(rows))
+    assert bool(torch.isfinite(out).all())
