@@ -20,8 +20,8 @@
 //   9           TMA: Q, then K and V tiles of BK rows through a ring;
 //   10          tiles of V in which some row does not see some key: values that
 //               are not finite are taken out before the product (0 x inf is
-//               NaN) and the job is marked; rows that do see them add them at
-//               the end;
+//               NaN) and their rows noted; rows that do see them add them at
+//               the end, from the noted rows alone;
 //   11          looks up the jobs to come.
 // Tensor memory: S0 S1 (128 columns each), O0 O1. Key tiles have 128 rows or 64.
 // With 128 a tile's scores take its 128 columns, P the first 64 of them, and the
@@ -79,7 +79,11 @@ struct Smem {
     static constexpr int ring = 2 * qtile, out = ring + NS * place, bar = out + 8 * 4096;   // out: 32 rows x 128 bytes a warp
     enum { B_Q = 0, B_QFREE, B_FULL, B_EMPTY = B_FULL + NS, B_CLEAN = B_EMPTY + NS, B_S = B_CLEAN + NS, B_P = B_S + 4, B_O = B_P + 4,
            B_END = B_O + 2, B_DRAIN = B_END + 2, B_JOB, B_TAKEN = B_JOB + NJ, B_COUNT = B_TAKEN + NJ };
-    static constexpr int bytes = bar + 8 * B_COUNT + 48 + 16 * NJ + 1024;
+    // rows of a job's masked tiles, a bit each: up to 255 neighbouring keys at either end
+    static constexpr int words = 2 * ((254 + BK - 1) / BK + 1) * (BK / 32);
+    static_assert(words <= 32, "a lane clears a word");
+    static constexpr int bytes = bar + 8 * B_COUNT + 48 + 16 * NJ + 4 * 2 * NJ * words + 1024;
+    static_assert(bytes <= 232448, "shared memory");
 };
 
 struct Job {
@@ -106,6 +110,10 @@ struct Keys {
     }
     __device__ __forceinline__ bool active(int x, int j) const { return j >= from[x] && j < to[x]; }
     __device__ __forceinline__ bool masked(int j) const { return j >= upper || j <= lower; }
+    // how many masked tiles come before the masked tile j, and the next masked tile
+    __device__ __forceinline__ int place(int j) const { return j - j0 - (j > lower ? max(0, upper - max(j0, lower + 1)) : 0); }
+    __device__ __forceinline__ int next(int j) const { return j < lower ? j + 1 : max(j + 1, upper); }
+    __device__ __forceinline__ int first() const { return masked(j0) ? j0 : upper; }
 };
 
 // The jobs of all sequences from the longest to the shortest: a sequence of n jobs has one on each of the levels 0 .. n - 1
@@ -288,6 +296,37 @@ struct Args {
     int64_t ldkv;
 };
 
+// Adds to the row i of a job, which is written, the values that are not finite and that it sees in the noted rows. Not inlined:
+// it hardly ever runs, and its code in the way of the others' costs long prompts 2 %.
+template <class E, int D, int BK>
+__device__ __noinline__ void add_not_finite(E* out, const E* v, int64_t ldkv, const Job& job, int R, int window, int i, const uint32_t* rows) {
+    const Keys<BK> ks(job, R, window);
+#pragma unroll 1
+    for (int d = 0; d < D; d += 16) {
+        float sum[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
+#pragma unroll 1
+        for (int j = ks.first(); j < ks.j1; j = ks.next(j))
+#pragma unroll 1
+            for (int n = 0; n < BK / 32; ++n)
+#pragma unroll 1
+                for (uint32_t bits = rows[ks.place(j) * (BK / 32) + n]; bits; bits &= bits - 1) {
+                    const int k = j * BK + 32 * n + __ffs(bits) - 1;
+                    if (k > i || (window > 0 && k <= i - window)) continue;
+                    uint4 w[2];
+                    const E* x = reinterpret_cast<const E*>(w);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) w[e] = reinterpret_cast<const uint4*>(v + k * ldkv + d)[e];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sum[e] += fabsf(to_f32<E>(x[e])) < INFINITY ? 0.0f : to_f32<E>(x[e]);
+                }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (sum[e] != 0.0f) out[d + e] = from_f32<E>(to_f32<E>(out[d + e]) + sum[e]);   // also where it is NaN
+    }
+}
+
 }  // namespace pk
 
 template <class E, int D, int BK, bool CAP>
@@ -310,8 +349,9 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + M::bar);
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + M::bar + 8 * M::B_COUNT);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);   // and the progress: see wait()
-    volatile int* s_odd = s_abort + 2;   // behind the progress: [2 NJ] jobs (counted from 1) in which values that are not finite were met
+    volatile int* s_odd = s_abort + 2;   // behind the progress: [2 NJ] jobs (counted from 1) in whose masked tiles values that are not finite were met
     volatile int4* s_job = reinterpret_cast<volatile int4*>(s_tmem + 12);   // [NJ] jobs, with the kv head
+    uint32_t* s_rows = s_tmem + 12 + 4 * NJ;   // [2 NJ][words] the rows of those, tile after tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = A.R, G = A.G;
     pdl_trigger();
@@ -476,6 +516,8 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         int i = 0;
         for (int q = 0; find(q, &job, &hk); ++q) {
             const Keys ks(job, R, A.window);
+            uint32_t* rows = s_rows + q % (2 * NJ) * M::words;
+            bool marked = false;
             for (int j = ks.j0; j < ks.j1 + NB; ++j, ++i) {   // V_{j-NB} in place i
                 // every place in its turn, and released by this warp too: a phase passed over could be taken for another
                 full(i);
@@ -494,15 +536,31 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                         acc[3] = __hfma2(Pair<E>::of(w.w), Pair<E>::zero(), acc[3]);
                     }
                     const auto all = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
-                    if (!__hbeq2(all, all)) {
+                    if (__any_sync(0xffffffffu, !__hbeq2(all, all))) {
+                        if (!marked) {
+                            if (lane < M::words) rows[lane] = 0;
+                            __syncwarp();
+                            marked = true;
+                        }
+                        const int own = job.s1 - job.s0 - (j - NB) * BK;   // rows of the tile that are the sequence's
 #pragma unroll 1
                         for (int e = lane; e < M::tile / 16; e += 32) {
                             uint4 w = t[e];
                             uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-                            for (int k = 0; k < 4; ++k) u[k] &= ~((not_finite2<E>(u[k]) >> 15) * 0xFFFFu);
+                            uint32_t some = 0;
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t odd = not_finite2<E>(u[k]);
+                                some |= odd;
+                                u[k] &= ~((odd >> 15) * 0xFFFFu);
+                            }
+                            if (!some) continue;
                             t[e] = w;
+                            const int r = e / 8 % BK;
+                            if (r < own) {
+                                atomicOr(rows + ks.place(j - NB) * (BK / 32) + r / 32, 1u << r % 32);
+                                s_odd[q % (2 * NJ)] = q + 1;
+                            }
                         }
-                        s_odd[q % (2 * NJ)] = q + 1;
                     }
                     fence_async_smem();
                     mbar_arrive(&bar[B_CLEAN + i % NS]);
@@ -623,7 +681,6 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         const float inv = *s_abort ? NAN : 1.0f / l;   // nobody takes what a wait that ran out left for an answer
         // 64 columns of the warp's 32 rows at a time by way of shared memory, so that a store instruction writes whole lines
         const uint64_t dst = live ? reinterpret_cast<uint64_t>(static_cast<E*>(A.out) + (int64_t)(job.s0 + i) * A.ldo + (int64_t)(hk * G + row % G) * D) : 0;
-        const E* v = static_cast<const E*>(A.v) + (int64_t)job.s0 * A.ldkv + (int64_t)hk * D;
         uint8_t* stage = sm + M::out + (threadIdx.x >> 5) * 4096;
 #pragma unroll 1   // run once a job: little code rather than many instruction fetches
         for (int c = 0; c < D; c += 64) {
@@ -635,14 +692,6 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                 tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] *= inv;
-                if (odd && live) {
-                    for (int k = A.window > 0 ? max(0, i - A.window + 1) : 0; k <= i; ++k)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float y = to_f32<E>(v[k * A.ldkv + c + 32 * h + e]);
-                            if (!(fabsf(y) < INFINITY)) o[e] += y;
-                        }
-                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * h + e) ^ (lane & 7)) << 4)) =
@@ -658,6 +707,9 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
             }
             __syncwarp();
         }
+        if (odd && live)
+            add_not_finite<E, D, BK>(reinterpret_cast<E*>(dst), static_cast<const E*>(A.v) + (int64_t)job.s0 * A.ldkv + (int64_t)hk * D,
+                                     A.ldkv, job, A.R, A.window, i, s_rows + q % (2 * NJ) * M::words);
         tc_fence_before();   // O is read before the next job's first weights are handed over
         }
         tc_fence_before();

@@ -209,7 +209,8 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
  * 0.. to at most n_rows; empty sequences are fine), and row i sees the rows of
  * its sequence up to itself, or with window > 0 the last `window` of them. scale
  * and softcap as above. Nothing in rows that a query does not see reaches its
- * output, infinities and NaN included. Weights are up to 2^8 before the
+ * output, infinities and NaN included; where it sees one in a dimension of v,
+ * that dimension of its output is infinite or NaN. Weights are up to 2^8 before the
  * division, so sums stay finite for values of v up to 10^36 / n_rows. The
  * tiles, and with them the last bits of a row, go by the batch's lengths. Rows
  * of out outside every sequence stay as they were. The kernel's waits for its

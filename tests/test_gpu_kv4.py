@@ -1076,3 +1076,42 @@ def test_packed_prompt_of_a_million_rows(env):
     rows = [0, 1, 127, 128, 5000, n // 3, n // 2, n - 400, n - 130, n - 77, n - 2, n - 1]
     check_packed(host(out[rows]), *rows64(torch, rows, q, k, v, 1, 1, D, 0.125), 1, D, "bf16", 0.0, len(rows))
     assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("t,D,lens,window", [("bf16", 128, [40000, 700], 0), ("f16", 64, [33000, 100, 50], 0), ("f16", 128, [300, 36000, 9], 20000),
+                                            ("bf16", 96, [3000] * 20, 1500)])
+def test_packed_infinities_in_long_prompts(env, t, D, lens, window):
+    """An infinity or NaN near the end of a long prompt, and a sequence of NaN behind it: rows that do not see them keep every
+    bit, rows that do are not finite in that dimension alone."""
+    lib, torch, _ = env
+    H, HKV = 4, 2
+    N, ends = sum(lens), np.cumsum(lens)
+    s = int(np.argmax(lens))
+    a, z = int(ends[s]) - lens[s], int(ends[s])
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v = (torch.randn((N, w * D), device="cuda", generator=gen).to(dtype(torch, t)) for w in (H, HKV, HKV))
+    cu = dev(torch, np.concatenate([[0], ends]).astype(np.int32))
+    clean = packed(env, t, q, k, v, cu, H, HKV, D, 0.1, 0.0, window)
+    assert bool(torch.isfinite(clean).all())
+    for row, what in ((z - 1, np.inf), (z - 200, -np.inf), (z - 333, np.nan), (a + 5, np.inf)):
+        vv = v.clone()
+        vv[row, D + 7] = what          # kv head 1, dimension 7
+        vv[z:] = np.nan                # every later sequence
+        out = packed(env, t, q, k, vv, cu, H, HKV, D, 0.1, 0.0, window)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        for h in (2, 3):
+            hit[row:min(z, row + window) if window else z, h * D + 7] = True
+        hit[z:] = True
+        assert torch.equal(out[~hit], clean[~hit]) and not bool(torch.isfinite(out[hit]).any())
+
+
+def test_packed_prompt_of_nan_values(env):
+    """Every value of one kv head NaN: its heads give NaN, the others what they give without."""
+    lib, torch, _ = env
+    n, H, HKV, D = 9000, 4, 2, 128
+    q, k, v = (torch.randn((n, w * D), device="cuda").half() for w in (H, HKV, HKV))
+    cu = dev(torch, np.array([0, 4000, n], np.int32))
+    clean = packed(env, "f16", q, k, v, cu, H, HKV, D, 0.1)
+    v[:, :D] = np.nan
+    out = packed(env, "f16", q, k, v, cu, H, HKV, D, 0.1)
+    assert bool(torch.isnan(out[:, :2 * D]).all()) and torch.equal(out[:, 2 * D:], clean[:, 2 * D:])
