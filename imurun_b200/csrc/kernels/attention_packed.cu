@@ -36,9 +36,14 @@
 // the jobs are no more than the SMs the longest one is all the time, and 128 it is:
 // one prompt of 512 rows 18 - 17, 20 - 18, 20.5 - 19.5 (those with cold caches).
 //
-// The reference m_i is raised only when a tile's maximum exceeds it by 2^8 (the
-// weights stay below 256, exact in both types' range), so the accumulator is
-// rescaled a few times a row, not once a tile.
+// The reference m_i is raised only when a tile's maximum exceeds it by 2^kSlack,
+// so the accumulator is rescaled a few times a row, not once a tile. Weights are
+// rounded to the values' type for the product, their sum is not: relative errors
+// of 2^-11 or 2^-8 that differ from key to key and average out. f16's range is
+// small, so there all weights are 2^11 times as large (at most 2^15): they keep
+// their bits down to 2^-25 of the row's largest, and those below 2^-36 are lost,
+// for a slack of 2^4 instead of 2^8, which takes 0.5 us of 22 at 64 prompts of
+// 0-300 rows and nothing of longer ones.
 //
 // What bounds it: long prompts the tensor core under the power limit. One of
 // 16384 rows, 64 heads in 8 groups, D = 128: 3.84 ms, 1.15 PFLOP/s; the same
@@ -67,7 +72,9 @@ namespace pk {
 constexpr int kHalf = 128 * 128;         // 128 rows x 64 values of 16 bits: one SW128 box
 constexpr int kSoft = 256, kThreads = kSoft + 128;
 constexpr int NJ = 4;                    // jobs looked up ahead
-constexpr float kRaise = 8.0f;
+// weights are 2^(c s - m + kUp), up to 2^(kSlack + kUp)
+template <class E> struct Range { static constexpr float kSlack = 8.0f, kUp = 0.0f; };
+template <> struct Range<__half> { static constexpr float kSlack = 4.0f, kUp = 11.0f; };
 
 // BK keys a tile, NB = 128 / BK places of a tile's scores in tensor memory, NS ring places of a V and a K tile
 template <int D, int BK>
@@ -625,7 +632,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < C; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
             const float mx = max3(mm[0], mm[2], C > 4 ? max3(mm[C - 4], mm[C - 2], mm[C - 2]) : mm[0]);
-            const bool raise = mx != -INFINITY && !((mx - m) * A.c <= kRaise);   // from -inf, and to NaN, too
+            const bool raise = mx != -INFINITY && !((mx - m) * A.c <= Range<E>::kSlack);   // from -inf, and to NaN, too
             if (__any_sync(0xffffffffu, raise)) {
                 const float f = raise ? ex2((m - mx) * A.c) : 1.0f;
                 if (raise) m = mx;
@@ -647,7 +654,7 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
                     }
                 }
             }
-            const float mc = m == -INFINITY ? 0.0f : -m * A.c;
+            const float mc = m == -INFINITY ? 0.0f : __fmaf_rd(-m, A.c, Range<E>::kUp);   // down: no weight passes the bound
             const float2 c2 = make_float2(A.c, A.c), mc2 = make_float2(mc, mc);
             float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll

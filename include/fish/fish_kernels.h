@@ -211,7 +211,9 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
  * and softcap as above. Nothing in rows that a query does not see reaches its
  * output, infinities and NaN included; where it sees one in a dimension of v,
  * that dimension of its output is infinite or NaN. Weights are up to 2^8 before the
- * division, so sums stay finite for values of v up to 10^36 / n_rows. The
+ * division (F16: 2^15), so sums stay finite for values of v up to 10^36 /
+ * n_rows. They are rounded to the type before they meet v, and in F16 those
+ * below 2^-36 of their row's largest count as nothing there. The
  * tiles, and with them the last bits of a row, go by the batch's lengths. Rows
  * of out outside every sequence stay as they were. The kernel's waits for its
  * own copies and products end after 0.2 s or more in which it made no progress:

@@ -1115,3 +1115,20 @@ def test_packed_prompt_of_nan_values(env):
     v[:, :D] = np.nan
     out = packed(env, "f16", q, k, v, cu, H, HKV, D, 0.1)
     assert bool(torch.isnan(out[:, :2 * D]).all()) and torch.equal(out[:, 2 * D:], clean[:, 2 * D:])
+
+
+def test_packed_one_key_above_thousands(env):
+    """One key 17.5 nats above all others, with a V of 0: what the row gives is the others', whose weights are 2^-25 each."""
+    lib, torch, _ = env
+    n, H, D = 8192, 2, 64
+    for t in ("f16", "bf16"):
+        q, k = (torch.zeros((n, w * D), device="cuda").to(dtype(torch, t)) for w in (H, 1))
+        v = torch.rand((n, D), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(dtype(torch, t)) + 0.5
+        q[:, ::D] = 1.0
+        k[0, 0] = 17.5
+        v[0] = 0
+        cu = dev(torch, np.array([0, n], np.int32))
+        out = packed(env, t, q, k, v, cu, H, 1, D, 1.0)
+        want, mean, ext = packed64(torch, q, k, v, [n], H, 1, D, 1.0, 0.0, 0)
+        # products of 17.5 and 1 and sums with zeros are exact; the weight, once rounded, carries the exponential's error alone
+        check_packed(host(out), want, mean, ext * 0, H, D, t, 0.0, n)
