@@ -632,7 +632,9 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < C; e += 2) mm[e] = max3(mm[e], max3(mm[e + 1], s[e / 2][15], s[e / 2][31]), mm[e]);
             const float mx = max3(mm[0], mm[2], C > 4 ? max3(mm[C - 4], mm[C - 2], mm[C - 2]) : mm[0]);
-            const bool raise = mx != -INFINITY && !((mx - m) * A.c <= Range<E>::kSlack);   // from -inf, and to NaN, too
+            // not for MMA rows that are nobody's: what lies there (groups that do not divide 128: an earlier kernel's shared memory)
+            // may be NaN, and would have the warp rescale at every tile
+            const bool raise = live && mx != -INFINITY && !((mx - m) * A.c <= Range<E>::kSlack);   // from -inf, and to NaN, too
             if (__any_sync(0xffffffffu, raise)) {
                 const float f = raise ? ex2((m - mx) * A.c) : 1.0f;
                 if (raise) m = mx;

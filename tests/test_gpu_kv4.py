@@ -1132,3 +1132,20 @@ def test_packed_one_key_above_thousands(env):
         want, mean, ext = packed64(torch, q, k, v, [n], H, 1, D, 1.0, 0.0, 0)
         # products of 17.5 and 1 and sums with zeros are exact; the weight, once rounded, carries the exponential's error alone
         check_packed(host(out), want, mean, ext * 0, H, D, t, 0.0, n)
+
+
+@pytest.mark.parametrize("t,H,HKV", [("f16", 14, 2), ("bf16", 6, 2), ("f16", 50, 1)])
+def test_packed_groups_that_leave_rows_over(env, t, H, HKV):
+    """Groups that do not divide a tile's 128 rows leave some that are nobody's, and hold what an earlier call left there: NaN
+    does not reach the others."""
+    lib, torch, _ = env
+    D, n = 128, 900
+    gen = torch.Generator(device="cuda").manual_seed(H)
+    q, k, v = (torch.randn((n, w * D), device="cuda", generator=gen).to(dtype(torch, t)) for w in (H, HKV, HKV))
+    cu = dev(torch, np.array([0, 333, n], np.int32))
+    clean = packed(env, t, q, k, v, cu, H, HKV, D, 0.1)
+    check_packed(host(clean), *packed64(torch, q, k, v, [333, n - 333], H, HKV, D, 0.1, 0.0, 0), H, D, t, 0.0, n)
+    nan = torch.full((20000, 4 * D), float("nan"), device="cuda", dtype=q.dtype)
+    bad = packed(env, t, nan, nan[:, :D].contiguous(), nan[:, :D].contiguous(), dev(torch, np.array([0, 20000], np.int32)), 4, 1, D, 0.1)
+    assert bool(torch.isnan(bad).all())
+    assert torch.equal(packed(env, t, q, k, v, cu, H, HKV, D, 0.1), clean)
