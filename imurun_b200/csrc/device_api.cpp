@@ -79,7 +79,11 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* c, int type, const void* q, con
     if (!k || !v || !tok_seq || !tok_pos) return -1;
     const int D = c->head_dim, HKV = c->n_head_kv;
     if ((q == nullptr) != (q_out == nullptr)) return -1;
-    if (rot < 0 || rot > D || rot % 2 || n_rope <= 0 || (rot > 0 && (!rope_cos || !rope_sin))) return -1;
+    if (rot < 0 || rot > D || rot % 2 || (rot > 0 && (n_rope <= 0 || !rope_cos || !rope_sin))) return -1;
+    if (rot == 0) {   // no tables, and so none to bound a position
+        rope_cos = rope_sin = nullptr;
+        n_rope = INT_MAX;
+    }
     if (q && (H <= 0 || H > 65535 || !stride_ok(ldq, (int64_t)H * D, type) || !stride_ok(ldq_out, (int64_t)H * D, out_type)))
         return -1;
     if (!stride_ok(ldkv, (int64_t)HKV * D, type)) return -1;

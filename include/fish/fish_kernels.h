@@ -169,7 +169,8 @@ FISH_API size_t fbx_kv4_layer_bytes(int n_head_kv, int head_dim);
 
 /* A step's T tokens into the cache: RoPE (the first `rot` dimensions, pairs
  * (2i, 2i+1) or with neox (i, i + rot/2), from the f32 tables [n_rope][rot/2]
- * at the token's position; rot 0 turns nothing) of q and k in 32 bits, then the
+ * at the token's position; rot 0 turns nothing and looks at neither the tables
+ * nor n_rope) of q and k in 32 bits, then the
  * quantised k and v into the row of each token's position. Token t belongs to
  * sequence tok_seq[t] and sits at tok_pos[t]; a negative tok_pos marks a
  * padding row, which is skipped. Tokens may come in any order; no (sequence,

@@ -1149,3 +1149,24 @@ def test_packed_groups_that_leave_rows_over(env, t, H, HKV):
     bad = packed(env, t, nan, nan[:, :D].contiguous(), nan[:, :D].contiguous(), dev(torch, np.array([0, 20000], np.int32)), 4, 1, D, 0.1)
     assert bool(torch.isnan(bad).all())
     assert torch.equal(packed(env, t, q, k, v, cu, H, HKV, D, 0.1), clean)
+
+
+def test_append_without_rotation_needs_no_tables(env):
+    """rot 0: no table, no bound on positions from one, the same cache and outputs as with tables."""
+    lib, torch, _ = env
+    H, HKV, D, T = 4, 2, 128, 70
+    qkv = torch.randn((T, (H + 2 * HKV) * D), device="cuda")
+    cos, sin = (dev(torch, x) for x in tables(T, 2))
+    a, b = (Cache(env, [T], HKV, D, seed=1) for _ in range(2))
+    rc, q_out, k_out, v_out = call_append(env, a, "f32", qkv, H, [0] * T, list(range(T)), 0, False, cos, sin, "f32")
+    assert rc == 0
+    got = [torch.zeros_like(x) for x in (q_out, k_out, v_out)]
+    where = [dev(torch, x.astype(np.int32)) for x in (np.zeros(T), np.arange(T))]
+    x, ld = qkv.data_ptr(), qkv.shape[1]
+    for n_rope in (1, 0):
+        assert lib.fbx_kv4_append(b.handle, 0, x, x + 4 * H * D, x + 4 * (H + HKV) * D, ld, ld, T, H, where[0].data_ptr(),
+                                  where[1].data_ptr(), 0, 1, None, None, n_rope, 0, got[0].data_ptr(), H * D, got[1].data_ptr(),
+                                  got[2].data_ptr(), HKV * D, None) == 0
+        torch.cuda.synchronize()
+        assert int(b.err) == 0 and torch.equal(a.pool, b.pool)
+        assert all(torch.equal(x, y) for x, y in zip(got, (q_out, k_out, v_out)))

@@ -153,3 +153,11 @@ def test_arrays_of_32_bit_values_off_their_boundary_are_refused(lib, off):
     for bad in (dict(page_table=at), dict(err=at)):
         assert append(lib, cache(**bad)) == -1 and attend(lib, cache(**bad)) == -1
     assert packed(lib, cu=at) == -1
+
+
+def test_append_without_rotation_asks_for_no_tables(lib):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("addresses that are no memory")
+    assert append(lib, rot=0, n_rope=0) > 0 and append(lib, rot=0, n_rope=-1, cos=None, sin=3) > 0
+    assert append(lib, rot=2, n_rope=0) == -1 and append(lib, rot=2, n_rope=-1) == -1
