@@ -537,11 +537,12 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     const int lrow = 4 * (t & 1);
     const bool lhas = 2 * (t & 1) < GP;
     const uint32_t lkeep = NG == 3 && (t & 1) ? 0xFFFFu : 0xFFFFFFFFu;   // not the padding
-    for (int j = 0; j < n; ++j) {
+    int j = 0;
+    for (; j < n; ++j) {
         if ((j & 15) == 16 - kSlots) ids_next = look_up((j & ~15) + 16);
         const uint32_t parity = (uint32_t)(j / kSlots) & 1u;
-        ok = ok && mbar_wait_soon(&bar[j % kSlots], parity, nullptr);
-        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait_soon(&bar[j % kSlots], parity));
+        if (!ok) break;
         const uint8_t* rec0 = ring + (j % kSlots) * 2 * R::bytes;
         // ---- scores of keys row and row + 8 (0, 1 and 2, 3) of both pages, heads 2 t, 2 t + 1, in log2 units
         float s[2][4];
@@ -755,7 +756,11 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         if (j + kSlots < n) issue(j + kSlots, ((j + kSlots) & ~15) == (j & ~15) ? ids : ids_next);
         if ((j & 15) == 15) ids = ids_next;
     }
-    if (!__all_sync(0xffffffffu, ok) && c.err && lane == 0) atomicExch(c.err, 7);   // a copy did not arrive in time
+    if (!ok) {   // a copy did not arrive in time: it and the one behind it may still be under way, and nobody gets an answer
+        for (int k = j; k < j + kSlots && k < n; ++k) mbar_wait_bounded(&bar[k % kSlots], (uint32_t)(k / kSlots) & 1u);
+        sum[0] = sum[1] = NAN;
+        if (c.err && lane == 0) atomicExch(c.err, 7);
+    }
     // ---- the lanes' sums over keys (those of other g), then the warps
 #pragma unroll
     for (int w = 4; w <= 16; w <<= 1) {

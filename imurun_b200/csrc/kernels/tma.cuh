@@ -70,15 +70,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 }
 // Bounded wait for the shortest time from the phase's end to the return: the
 // clock, whose reading takes longer than a wake-up, is looked at once in 256
-// tries (a try waits by itself for a while). abort may be null.
-__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort) {
+// tries (a try waits by itself for a while).
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
     unsigned long long t0 = 0;
     for (unsigned i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255) == 0) {
             const unsigned long long t = gtimer();
             if (t0 == 0) t0 = t;
-            if ((abort && *abort) || (long long)(t - t0) > kWaitNs) return false;
+            if ((long long)(t - t0) > kWaitNs) return false;
         }
     }
 }

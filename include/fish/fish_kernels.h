@@ -157,7 +157,8 @@ typedef struct {
     const int32_t* page_table;   /* [n_seqs][table_stride]: page of position 16 i of sequence s at s * table_stride + i */
     int32_t* err;                /* nullable, one int, set on the device: 5 a page outside the pool, 6 a token's
                                     sequence or position outside the tables (nothing out of range is read or
-                                    written), 7 a copy on the device did not arrive in time */
+                                    written), 7 a copy on the device did not arrive in time (what depends on it
+                                    is NaN) */
     int64_t page_stride;         /* bytes from page to page, a multiple of 16 */
     int64_t layer_offset;        /* bytes from a page's start to this layer's records, a multiple of 16 */
     int32_t n_pages, table_stride, n_seqs;
