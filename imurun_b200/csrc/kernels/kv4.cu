@@ -502,11 +502,9 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     }
     __syncthreads();
     // B operands of the scores
-    uint32_t qb[PL][NG][4];
+    uint32_t qb[NG][4];
 #pragma unroll
-    for (int p = 0; p < PL; ++p)
-#pragma unroll
-        for (int e = 0; e < NG; ++e) words<4>(sm + M::q + ((8 * p + g) * QS + 32 * e + 8 * t) * 2, qb[p][e]);
+    for (int e = 0; e < NG; ++e) words<4>(sm + M::q + (g * QS + 32 * e + 8 * t) * 2, qb[e]);
     // and of sum_g lo sum(q_g): the sums' high parts against k = 0..3, their low parts against k = 4..7
     const uint32_t qsb = *reinterpret_cast<const uint32_t*>(sm + M::qs + (t >> 1) * 64 + g * 8 + (t & 1) * 4);
     constexpr float kLog2e = 1.4426950408889634f;
@@ -565,10 +563,13 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 codes8<SUB>(w0[e], a);
                 codes8<SUB>(w1[e], b);
                 float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int p = 0; p < PL; ++p) {
-                    mma16(x, a[0], b[0], a[1], b[1], qb[p][e][0], qb[p][e][1]);
-                    mma16(x, a[2], b[2], a[3], b[3], qb[p][e][2], qb[p][e][3]);
+                mma16(x, a[0], b[0], a[1], b[1], qb[e][0], qb[e][1]);
+                mma16(x, a[2], b[2], a[3], b[3], qb[e][2], qb[e][3]);
+                if (PL == 2) {   // the low parts stay in shared memory: registers are full
+                    uint32_t ql[4];
+                    words<4>(sm + M::q + ((8 + g) * QS + 32 * e + 8 * t) * 2, ql);
+                    mma16(x, a[0], b[0], a[1], b[1], ql[0], ql[1]);
+                    mma16(x, a[2], b[2], a[3], b[3], ql[2], ql[3]);
                 }
                 const float da = e & 1 ? half_at<1>(d0[e / 2]) : half_at<0>(d0[e / 2]);
                 const float db = e & 1 ? half_at<1>(d1[e / 2]) : half_at<0>(d1[e / 2]);
