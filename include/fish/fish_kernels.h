@@ -195,7 +195,8 @@ FISH_API int fbx_kv4_append(const fbx_kv4_cache* cache, int type, const void* q,
  * rows of padding tokens (negative tok_pos) stay as they were, and a token
  * that sees nothing that can be read gets zeros. max_keys, an upper bound on
  * tok_pos + 1, sizes the split of long contexts (any value gives the right
- * result). workspace: 16-byte aligned, at least
+ * result; the split goes by T and the heads too, and the last bits of a row with
+ * it). T is at most 65535, H too. workspace: 16-byte aligned, at least
  * fbx_kv4_attention_workspace bytes (NULL where that is 0), not shared by calls
  * that may overlap; needs no clearing. */
 FISH_API size_t fbx_kv4_attention_workspace(int T, int H, int n_head_kv, int head_dim, int max_keys);

@@ -1170,3 +1170,65 @@ def test_append_without_rotation_needs_no_tables(env):
         torch.cuda.synchronize()
         assert int(b.err) == 0 and torch.equal(a.pool, b.pool)
         assert all(torch.equal(x, y) for x, y in zip(got, (q_out, k_out, v_out)))
+
+
+# more heads than the warps of a CTA have in one turn: type, out, T, lens, H, HKV, D, rot, neox, layers, layer
+APPENDS_OF_SEVERAL_TURNS = [
+    ("f16", "f16", 150, [150], 28, 4, 128, 128, True, 1, 0),
+    ("bf16", "bf16", 149, [149], 64, 8, 128, 128, False, 1, 0),
+    ("f16", "f32", 148, [148], 90, 3, 128, 128, False, 1, 0),     # more than five turns of 16 heads: fetched again
+    ("f32", "f32", 148, [148], 40, 4, 128, 128, False, 1, 0),     # more than two
+    ("f32", "bf16", 148, [148], 40, 4, 128, 20, True, 1, 0),
+    ("bf16", "f16", 148, [148], 33, 4, 96, 96, True, 1, 0),       # a ragged last turn, 8 lanes of a warp idle
+    ("bf16", "f16", 148, [148], 85, 2, 96, 32, False, 1, 0),
+    ("f16", "bf16", 148, [148], 37, 3, 64, 22, True, 1, 0),
+    ("bf16", "bf16", 148, [148], 160, 4, 64, 64, True, 1, 0),
+]
+
+
+@pytest.mark.parametrize("case", APPENDS_OF_SEVERAL_TURNS, ids=lambda c: "-".join(map(str, c[:9])))
+def test_append_of_many_heads_matches_the_format(env, case):
+    test_append_matches_the_format_bit_for_bit(env, *case)
+
+
+@pytest.mark.parametrize("t,H,HKV,D,rot,neox", [("bf16", 64, 8, 128, 128, True), ("f16", 90, 3, 128, 64, False), ("f32", 40, 4, 96, 20, True),
+                                               ("f16", 28, 4, 128, 128, True), ("f32", 40, 4, 128, 128, False)])
+def test_append_of_many_heads_in_place(env, t, H, HKV, D, rot, neox):
+    lib, torch, _ = env
+    T = 160
+    cos, sin = (dev(torch, x) for x in tables(T, rot))
+    seq, pos = dev(torch, np.zeros(T, np.int32)), dev(torch, np.arange(T, dtype=np.int32))
+    qkv = torch.randn((T, (H + 2 * HKV) * D), device="cuda").to(dtype(torch, t))
+    a, b = (Cache(env, [T], HKV, D, seed=1) for _ in range(2))
+    rc, *want = call_append(env, a, t, qkv, H, [0] * T, list(range(T)), rot, neox, cos, sin, t)
+    assert rc == 0
+    x, ld, es = qkv.clone(), qkv.shape[1], qkv.element_size()
+    p = [x.data_ptr() + es * D * o for o in (0, H, H + HKV)]
+    assert lib.fbx_kv4_append(b.handle, plain.TYPE[t], *p, ld, ld, T, H, seq.data_ptr(), pos.data_ptr(), rot, int(neox), cos.data_ptr(),
+                              sin.data_ptr(), T, plain.TYPE[t], p[0], ld, p[1], p[2], ld, None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(x, torch.cat(want, 1)) and torch.equal(a.pool, b.pool)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_attention_of_a_token_alone_and_among_others(env, t):
+    """How a context is split goes by the whole call, and a row's last bits with it: alone it is as near to 64 bits as among
+    others, and the same call gives the same bits."""
+    lib, torch, _ = env
+    H, HKV, D, lens = 8, 2, 128, [2000, 333, 40, 1] * 12
+    c, k, v, d, at = filled(env, lens, HKV, D, seed=41)
+    T = len(lens)
+    q = torch.randn((T, H * D), device="cuda", generator=torch.Generator(device="cuda").manual_seed(41)).to(dtype(torch, t))
+    together = attention(env, c, t, q, H, list(range(T)), [n - 1 for n in lens], max(lens), 0.1)
+    assert torch.equal(together, attention(env, c, t, q, H, list(range(T)), [n - 1 for n in lens], max(lens), 0.1))
+    for s in (0, 1, 2, 3, T - 4):
+        alone = attention(env, c, t, q[s:s + 1], H, [s], [lens[s] - 1], lens[s], 0.1)[0]
+        rows = slice(int(at[s]), int(at[s]) + lens[s])
+        x = q[s].view(HKV, H // HKV, D).double()
+        kk, vv, dd = (y[rows].transpose(0, 1) for y in (k, v, d))
+        w = torch.softmax(x @ kk.transpose(1, 2) * 0.1, -1)
+        want, mean, coarse = (z.reshape(H, D).cpu().numpy() for z in (w @ vv, w @ vv.abs(), w @ dd))
+        ext = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(H).cpu().numpy() * 0.1
+        for got in (alone, together[s]):
+            near(host(got).reshape(H, D), want, (mean, ext, coarse), t)
+    assert int(c.err) == 0
