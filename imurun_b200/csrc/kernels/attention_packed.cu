@@ -293,7 +293,7 @@ template <> struct Pair<__nv_bfloat16> {
 
 struct Args {
     const int32_t* cu;
-    int B, n_rows, HKV, G, R;
+    int B, n_rows, HKV, G, R, jobs;   // jobs: as many as there can be
     float c;        // scores to log2 units
     float pre;      // soft cap: 2 log2(e) scale / cap, and c = cap log2(e)
     int window;
@@ -506,7 +506,10 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         for (int n = 0;; ++n) {
             if (n >= NJ) wait(&bar[B_TAKEN + n % NJ], (uint32_t)(n / NJ - 1) & 1, s_abort);
             const uint32_t id = (uint32_t)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), unit = id / (uint32_t)A.HKV;
-            job = finder.find((int)unit);
+            // lengths that are none (decreasing) may name the same rows over and over: no more jobs than rows can have, and
+            // counts that stay far below 2^31
+            if (id < (uint32_t)A.jobs) job = finder.find((int)unit);
+            else job.s1 = 0;
             if (__any_sync(0xffffffffu, *s_abort)) job.s1 = 0;
             if (lane == 0) {
                 s_job[n % NJ].x = job.s0;
@@ -785,10 +788,10 @@ cudaError_t launch_packed(const void* q, int64_t ldq, const void* k, const void*
         __atomic_fetch_or(&set, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
     }
     constexpr float kLog2e = 1.4426950408889634f;
-    pk::Args a{cu, B, n_rows, HKV, G, R, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
-               window, out, ldo, v, ldkv};
     const int64_t jobs = most_jobs(n_rows, B, H, HKV);
     if (jobs > INT_MAX / 2) return cudaErrorInvalidValue;
+    pk::Args a{cu, B, n_rows, HKV, G, R, (int)jobs, CAP ? softcap * kLog2e : scale * kLog2e, CAP ? 2.0f * kLog2e * scale / softcap : 0.0f,
+               window, out, ldo, v, ldkv};
     return fbk_launch_early(k_attention_packed<E, D, BK, CAP>, dim3((unsigned)std::min<int64_t>(jobs, kSMs)), dim3(pk::kThreads), (size_t)M::bytes, st, 1, qm,
                       km, vm, a);
 }

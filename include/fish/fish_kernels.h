@@ -209,7 +209,8 @@ FISH_API int fbx_kv4_attention(const fbx_kv4_cache* cache, int type, const void*
  * rows of q [n_rows][H*D], k and v [n_rows][HKV*D] (F16 or BF16; D 64, 96 or
  * 128; H a multiple of HKV, at most 128 times it): sequence s has the rows cu_seqlens[s] ..
  * cu_seqlens[s+1] - 1 (device array of n_seqs + 1 non-decreasing values from
- * 0.. to at most n_rows; empty sequences are fine), and row i sees the rows of
+ * 0.. to at most n_rows; empty sequences are fine; with other values nothing
+ * outside the buffers is touched, and rows of out are anything), and row i sees the rows of
  * its sequence up to itself, or with window > 0 the last `window` of them. scale
  * and softcap as above. Nothing in rows that a query does not see reaches its
  * output, infinities and NaN included; where it sees one in a dimension of v,

@@ -1232,3 +1232,27 @@ def test_attention_of_a_token_alone_and_among_others(env, t):
         for got in (alone, together[s]):
             near(host(got).reshape(H, D), want, (mean, ext, coarse), t)
     assert int(c.err) == 0
+
+
+@pytest.mark.parametrize("count", [200, 1 << 20])
+def test_packed_lengths_that_go_back_and_forth(env, count):
+    """Lengths that name the same rows again and again (which the caller must not give): as much work as proper ones can be,
+    inside the buffers; a proper call after it is right."""
+    lib, torch, _ = env
+    H, HKV, D, N = 2, 1, 64, 20000
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v = (torch.randn((N, w * D), device="cuda", generator=gen).half() for w in (H, HKV, HKV))
+    cu = torch.zeros(count + 1, dtype=torch.int32, device="cuda")
+    cu[1::2] = N
+    guard = torch.full((N + 256, H * D), 7.0, device="cuda", dtype=torch.float16)
+    t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    t[0].record()
+    packed(env, "f16", q, k, v, cu, H, HKV, D, 0.1, out=guard[128:128 + N])
+    t[1].record()
+    torch.cuda.synchronize()
+    # at most N / 128 + min(count, N) jobs, each of at most N / 64 key tiles of some 2 us on one of 148 SMs: 0.1 s; times 20
+    assert t[0].elapsed_time(t[1]) < 2000
+    assert bool((guard[:128] == 7).all()) and bool((guard[128 + N:] == 7).all()) and bool(torch.isfinite(guard).all())
+    cu = dev(torch, np.array([0, 300, 800], np.int32))
+    out = packed(env, "f16", q[:800], k[:800], v[:800], cu, H, HKV, D, 0.1)
+    check_packed(host(out), *packed64(torch, q[:800], k[:800], v[:800], [300, 500], H, HKV, D, 0.1, 0.0, 0), H, D, "f16", 0.0, 800)
