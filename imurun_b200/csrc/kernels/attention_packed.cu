@@ -361,7 +361,6 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
     uint32_t* s_rows = s_tmem + 12 + 4 * NJ;   // [2 NJ][words] the rows of those, tile after tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = A.R, G = A.G;
-    pdl_trigger();
     if (threadIdx.x == kSoft) {
         s_abort[0] = s_abort[1] = 0;
         for (int i = 0; i < 2 * NJ; ++i) s_odd[i] = 0;
@@ -370,12 +369,14 @@ __global__ void __launch_bounds__(pk::kThreads, 1)
         }
         mbar_fence_init();
     }
-    // tensor memory only after the wait: a kernel that this one follows, and waits for, may still need its own
+    // tensor memory only after the wait: a kernel that this one follows, and waits for, may still need its own; and a kernel
+    // that follows this one may only begin once this one has it: it could take it, and then wait for this one
     pdl_wait();
     if (warp == 8) tmem_alloc(s_tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_trigger();
     const uint32_t tmem = *s_tmem;
     // job n of this CTA, for a whole warp; false past the last
     auto find = [&](int n, Job* job, int* hk) {

@@ -1256,3 +1256,39 @@ def test_packed_lengths_that_go_back_and_forth(env, count):
     cu = dev(torch, np.array([0, 300, 800], np.int32))
     out = packed(env, "f16", q[:800], k[:800], v[:800], cu, H, HKV, D, 0.1)
     check_packed(host(out), *packed64(torch, q[:800], k[:800], v[:800], [300, 500], H, HKV, D, 0.1, 0.0, 0), H, D, "f16", 0.0, 800)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_packed_between_matrix_products(env, D):
+    """Packed attention in a row with matrix products, which use tensor memory too, eager and captured: each gets what it needs,
+    whichever begins early."""
+    lib, torch, _ = env
+    H, HKV, lens = 16, 4, [500, 3, 700]
+    N = sum(lens)
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v = (torch.randn((N, w * D), device="cuda", generator=gen).bfloat16() for w in (H, HKV, HKV))
+    w = (torch.randn((H * D, H * D), device="cuda", generator=gen) * (H * D) ** -0.5).bfloat16()
+    cu = dev(torch, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    outs = [torch.zeros((N, H * D), device="cuda", dtype=q.dtype) for _ in range(4)]
+
+    def chain(st):
+        x = q
+        for out in outs:
+            assert lib.fbx_attention_packed(30, x.data_ptr(), H * D, k.data_ptr(), v.data_ptr(), HKV * D, N, cu.data_ptr(), 3, H, HKV,
+                                            D, 0.1, 0.0, 0, out.data_ptr(), H * D, st) == 0
+            x = torch.matmul(out, w)
+        return x
+
+    want = chain(None).clone()
+    kept = [o.clone() for o in outs]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(torch.cuda.current_stream().cuda_stream)
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(outs, kept))
+    check_packed(host(outs[0]), *packed64(torch, q, k, v, lens, H, HKV, D, 0.1, 0.0, 0), H, D, "bf16", 0.0, N)
