@@ -250,9 +250,9 @@ __global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_co
 // and d 2^(7 - E) <= 2^8 the products stay in f16's range whatever the values'
 // size is, and d keeps all its bits down to 2^-20 of its group's largest.
 //
-// Roundings: 16-bit queries go in as one f16 part, scaled by a power of two (a
-// value that is less than 2^-25 of its head's largest counts as nothing), f32
-// ones as two (2^-22, and 2^-25 of the head's largest). Weights p d of f32 calls
+// Roundings: 16-bit queries go in as one f16 part, scaled by a power of two
+// (exact down to 2^-23 of the head's largest), f32 ones as two (2^-22, and 2^-34
+// of the head's largest), and so the sums of a group's queries. Weights p d of f32 calls
 // are three bf16 parts (2^-24, in f32's range, so groups and keys of any size
 // lie beside one another without an exponent). They meet codes of -8..7 with
 // lo + 8 d in lo's place: sums that are all of one sign, and of which lo takes
@@ -463,8 +463,8 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
     };
     for (int j = 0; j < kSlots && j < n; ++j) issue(j, ids);
 
-    // the queries: warp w brings head g0 + w to at most 2 in size, as f16 parts, dimensions 32 e + 8 t + n in the order
-    // (0, 4), (1, 5), (2, 6), (3, 7) of n that a lane's operands have
+    // the queries: warp w brings head g0 + w to 2^9 .. 2^10 in size (16 times that, and sums of 32, are still f16), as f16 parts,
+    // dimensions 32 e + 8 t + n in the order (0, 4), (1, 5), (2, 6), (3, 7) of n that a lane's operands have
     constexpr int QS = AtSmem<D>::q_row;
     {
         float top = 0.0f;
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
         top = warp_max(top);
         int ex = (int)(__float_as_uint(top) >> 23) - 127;
         if (ex == 128 || top == 0.0f) ex = 0;
-        ex = min(max(ex, -120), 120);
+        ex = max(ex, -110) - 9;
         const float down = __int_as_float((127 - ex) << 23);
         __half* sq = reinterpret_cast<__half*>(sm + M::q) + warp * QS + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
         __half* ss = reinterpret_cast<__half*>(sm + M::qs) + warp * 4;

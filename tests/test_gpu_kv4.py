@@ -1292,3 +1292,19 @@ def test_packed_between_matrix_products(env, D):
         torch.cuda.synchronize()
         assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(outs, kept))
     check_packed(host(outs[0]), *packed64(torch, q, k, v, lens, H, HKV, D, 0.1, 0.0, 0), H, D, "bf16", 0.0, N)
+
+
+@pytest.mark.parametrize("t,apart", [("f32", 12), ("f16", 20), ("bf16", 20)])
+def test_attention_of_queries_far_apart(env, t, apart):
+    """Queries of one group 2^apart below another's, and keys as much above: both have the same part in the scores."""
+    lib, torch, _ = env
+    rng = np.random.default_rng(apart)
+    H, HKV, D, n = 4, 2, 128, 200
+    k, v = (rng.standard_normal((n, HKV, D)).astype(np.float32) for _ in range(2))
+    size = np.array([0, apart, apart // 2, apart], np.float64).repeat(32)   # binary orders
+    k = (k * 2.0 ** (size - apart // 2)).astype(np.float32)
+    c, kk, vv, step = appended(env, k, v)
+    q = dev(torch, (rng.standard_normal((1, H * D)) * np.tile(2.0 ** (apart // 2 - size), H)).astype(np.float32), t)
+    out = host(attention(env, c, t, q, H, [0], [n - 1], n, 0.1)).reshape(H, D)
+    want, *bound = expect(host(q).reshape(H, D).astype(np.float64), kk, vv, step, H, 0.1)
+    near(out, want, bound, t)
