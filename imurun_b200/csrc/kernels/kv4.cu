@@ -720,17 +720,24 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 if constexpr (W == W_PARTS) {
                     codes8_mid(wa, ra);
                     codes8_mid(wc, rc);
-                    float x[4] = {p[0] * da, p[1] * da, p[2] * db, p[3] * db};
+                    // a page's sums start at 0 and are added in f32: sums over a long context in the tensor core, whose additions cut
+                    // off, would all come out a little small (4e-5 after 16000 keys of a warp)
+                    float x[4] = {p[0] * da, p[1] * da, p[2] * db, p[3] * db}, y[2][4] = {};
 #pragma unroll
                     for (int part = 0; part < 3; ++part) {
-                        const __nv_bfloat162 y0 = __floats2bfloat162_rn(x[0], x[1]), y1 = __floats2bfloat162_rn(x[2], x[3]);
-                        const uint32_t b0 = transpose8(b2_bits(y0)), b1 = transpose8(b2_bits(y1));
+                        const __nv_bfloat162 z0 = __floats2bfloat162_rn(x[0], x[1]), z1 = __floats2bfloat162_rn(x[2], x[3]);
+                        const uint32_t b0 = transpose8(b2_bits(z0)), b1 = transpose8(b2_bits(z1));
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) mma16_bf16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
-                        x[0] -= __low2float(y0);
-                        x[1] -= __high2float(y0);
-                        x[2] -= __low2float(y1);
-                        x[3] -= __high2float(y1);
+                        for (int u = 0; u < 2; ++u) mma16_bf16(y[u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);
+                        x[0] -= __low2float(z0);
+                        x[1] -= __high2float(z0);
+                        x[2] -= __low2float(z1);
+                        x[3] -= __high2float(z1);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[e][0][i] += y[0][i];
+                        o[e][1][i] += y[1][i];
                     }
                     continue;
                 }

@@ -1308,3 +1308,30 @@ def test_attention_of_queries_far_apart(env, t, apart):
     out = host(attention(env, c, t, q, H, [0], [n - 1], n, 0.1)).reshape(H, D)
     want, *bound = expect(host(q).reshape(H, D).astype(np.float64), kk, vv, step, H, 0.1)
     near(out, want, bound, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_attention_of_many_tokens_over_one_long_context(env, t):
+    """131000 keys that no call splits, as there are tokens enough: 16000 a warp, V's values all of one sign."""
+    lib, torch, _ = env
+    n, T, H, D = 131000, 300, 8, 64
+    c = Cache(env, [n], 1, D, seed=1)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.cat([torch.randn((n, D), device="cuda", generator=gen),
+                   torch.empty((n, D), device="cuda").exponential_(generator=gen)], 1).contiguous()
+    held = [torch.empty((n, D), device="cuda") for _ in range(2)]
+    where = [torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")]
+    assert lib.fbx_kv4_append(c.handle, 0, None, x.data_ptr(), x.data_ptr() + 4 * D, 0, 2 * D, n, 0, where[0].data_ptr(),
+                              where[1].data_ptr(), 0, 0, None, None, 0, 0, None, 0, held[0].data_ptr(), held[1].data_ptr(), D,
+                              None) == 0
+    q = torch.randn((T, H * D), device="cuda", generator=gen).to(dtype(torch, t))
+    out = attention(env, c, t, q, H, [0] * T, [n - 1] * T, n, 0.1)
+    k, v = (y.double() for y in held)
+    y = x[:, D:].view(n, D // 32, 32)
+    d = ((y.amax(-1) - y.amin(-1)) / 15 * 1.001).double().repeat_interleave(32, -1)   # no less than the d that is stored
+    for r in (0, 150, T - 1):
+        a = q[r].view(H, D).double()
+        w = torch.softmax(a @ k.T * 0.1, -1)
+        want, mean, coarse = ((w @ z).cpu().numpy() for z in (v, v, d))
+        ext = (a.abs() @ k.abs().T).amax(-1).cpu().numpy() * 0.1
+        near(host(out[r]).reshape(H, D), want, (mean, ext, coarse), t)
