@@ -1335,3 +1335,16 @@ def test_attention_of_many_tokens_over_one_long_context(env, t):
         want, mean, coarse = ((w @ z).cpu().numpy() for z in (v, v, d))
         ext = (a.abs() @ k.abs().T).amax(-1).cpu().numpy() * 0.1
         near(host(out[r]).reshape(H, D), want, (mean, ext, coarse), t)
+
+
+@pytest.mark.parametrize("t,D,n", [("f16", 64, 131072), ("f16", 96, 100000), ("f16", 128, 131072), ("bf16", 128, 131072), ("f16", 64, 1 << 20)])
+def test_packed_long_prompts_of_one_sign(env, t, D, n):
+    """Values around 1, so that every key adds to the accumulator: it loses nothing on the way that the sum of the weights keeps."""
+    lib, torch, _ = env
+    gen = torch.Generator(device="cuda").manual_seed(n + D)
+    q, k, v = (torch.randn((n, D), device="cuda", generator=gen) for _ in range(3))
+    q, k, v = (x.to(dtype(torch, t)) for x in (q, k, 1 + 0.1 * v))
+    cu = dev(torch, np.array([0, n], np.int32))
+    out = packed(env, t, q, k, v, cu, 1, 1, D, D ** -0.5)
+    rows = [0, 777, 16384, n // 3, n // 2, n - 100, n - 2, n - 1]
+    check_packed(host(out[rows]), *rows64(torch, rows, q, k, v, 1, 1, D, D ** -0.5), 1, D, t, 0.0, len(rows))
