@@ -252,12 +252,12 @@ __global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_co
 //
 // Roundings: 16-bit queries go in as one f16 part, scaled by a power of two
 // (exact down to 2^-23 of the head's largest), f32 ones as two (2^-22, and 2^-34
-// of the head's largest), and so the sums of a group's queries. Weights p d of f32 calls
-// are three bf16 parts (2^-24, in f32's range, so groups and keys of any size
-// lie beside one another without an exponent). They meet codes of -8..7 with
-// lo + 8 d in lo's place: sums that are all of one sign, and of which lo takes
-// most away again, would leave the adder's truncation several times as large in
-// the result. For f16 outputs p d is rounded once and meets codes of -8..7 too
+// of the head's largest), and so the sums of a group's queries. Weights p d of
+// f32 calls are three bf16 parts (2^-24, in f32's range, so groups and keys of
+// any size lie beside one another without an exponent), and a page's sums of
+// them are added in f32. They meet codes of -8..7 with lo + 8 d in lo's place:
+// sums that are all of one sign, and of which lo takes most away again, would
+// leave the adder's truncation several times as large in the result. For f16 outputs p d is rounded once and meets codes of -8..7 too
 // (8 sum(p d) is taken off by one more MMA a group), else the rounding would be
 // the larger part of the error; for bf16, whose own step is 8 times as wide, p
 // is rounded first and codes stay 0..15. In both a p d below 2^-14 of 2^(E - 7),
@@ -265,13 +265,14 @@ __global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_co
 // more.
 //
 // Measured at D = 128: 32 tokens of 4097-5100 bf16 keys, 64 heads in 8 groups,
-// 46 us, 4.1 TB/s; 64 of 2049-2180 f16 keys, 28 heads in 4 groups, 26 us, 3.3
+// 46 us, 4.1 TB/s; 64 of 2049-2180 f16 keys, 28 heads in 4 groups, 27 us, 3.25
 // TB/s (256 CTAs on 148 SMs: those with two are busy for 40000 cycles, 139 a page,
 // those with one for 24000; 6000 more are the page ids, the queries and the
-// merge); one of 131071 bf16 keys 39 us; one of 577 f32 keys 7.3 us, 6.9 in a
-// graph. Tried and slower: equal shares of all pages for 296 CTAs (47 us at 64 x
-// 2100), two to eight splits of 256 pairs (37 to 63) or of 384 (55 against 45),
-// CTAs of four warps (53), scores of the next pages under this one's products.
+// merge); one of 131071 bf16 keys 39 us; one of 577 f32 keys 7.4 us, 6.6 in a
+// graph; f32 at the shapes of the second and third 50 and 79 us. Tried and
+// slower: equal shares of all pages for 296 CTAs (47 us at 64 x 2100), two to
+// eight splits of 256 pairs (37 to 63) or of 384 (55 against 45), CTAs of four
+// warps (53), scores of the next pages under this one's products.
 constexpr int kAtWarps = 8, kSlots = 2;
 constexpr int kMaxCluster = 8;
 constexpr float kNoRef = -3.4028235e38f;   // before the first key: below every score, and finite, so that a key outside (-inf) weighs 0
