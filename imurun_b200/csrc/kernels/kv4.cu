@@ -257,18 +257,20 @@ __global__ void __launch_bounds__(256, FEW ? 5 : 4) k_kv4_append(const __grid_co
 // any size lie beside one another without an exponent), and a page's sums of
 // them are added in f32. They meet codes of -8..7 with lo + 8 d in lo's place:
 // sums that are all of one sign, and of which lo takes most away again, would
-// leave the adder's truncation several times as large in the result. For f16 outputs p d is rounded once and meets codes of -8..7 too
-// (8 sum(p d) is taken off by one more MMA a group), else the rounding would be
-// the larger part of the error; for bf16, whose own step is 8 times as wide, p
-// is rounded first and codes stay 0..15. In both a p d below 2^-14 of 2^(E - 7),
-// and a p below 2^-14, is held to 2^-25 of that, where a warp's largest p is 2 or
-// more.
+// leave the adder's truncation several times as large in the result. For 16 bits
+// p d is rounded once, to f16. For f16 outputs it meets codes of -8..7 too (8
+// sum(p d) is taken off by one more MMA a group), else that rounding would be the
+// larger part of the error; for bf16, whose own step is 8 times as wide, codes
+// stay 0..15 (centred ones: 53 us against 48 at 32 tokens, error against 64 bits
+// 1.67e-3 against 1.74e-3, of which 1.65e-3 are the output's own rounding). In
+// both a p d below 2^-14 of 2^(E - 7) is held to 2^-25 of that, where a warp's
+// largest p is 2 or more.
 //
 // Measured at D = 128: 32 tokens of 4097-5100 bf16 keys, 64 heads in 8 groups,
-// 46 us, 4.1 TB/s; 64 of 2049-2180 f16 keys, 28 heads in 4 groups, 27 us, 3.25
+// 48 us, 4.0 TB/s; 64 of 2049-2180 f16 keys, 28 heads in 4 groups, 27 us, 3.25
 // TB/s (256 CTAs on 148 SMs: those with two are busy for 40000 cycles, 139 a page,
 // those with one for 24000; 6000 more are the page ids, the queries and the
-// merge); one of 131071 bf16 keys 39 us; one of 577 f32 keys 7.4 us, 6.6 in a
+// merge); one of 131071 bf16 keys 41 us; one of 577 f32 keys 7.4 us, 6.6 in a
 // graph; f32 at the shapes of the second and third 50 and 79 us. Tried and
 // slower: equal shares of all pages for 296 CTAs (47 us at 64 x 2100), two to
 // eight splits of 256 pairs (37 to 63) or of 384 (55 against 45), CTAs of four
@@ -400,10 +402,10 @@ struct AtSmem {
 };
 
 // how the weights of an element type go into the products with V (see above)
-enum : int { W_PARTS, W_MID, W_HALF };
+enum : int { W_PARTS, W_MID, W_CODE };
 template <class E> struct AtWeights { static constexpr int mode = W_PARTS; };
 template <> struct AtWeights<__half> { static constexpr int mode = W_MID; };
-template <> struct AtWeights<__nv_bfloat16> { static constexpr int mode = W_HALF; };
+template <> struct AtWeights<__nv_bfloat16> { static constexpr int mode = W_CODE; };
 
 template <class E, int D>
 __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid_constant__ AtArgs A) {
@@ -693,7 +695,6 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
             for (int i = 0; i < 4; ++i) p[i] = at_ex2(s[h][i] - ref[i & 1]);
             sum[0] += p[0] + p[2];
             sum[1] += p[1] + p[3];
-            const __half2 p0 = __floats2half2_rn(p[0], p[1]), p1 = __floats2half2_rn(p[2], p[3]);
             // ---- V: pairs of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the tile, 4 dims a group
             uint32_t va[(NG + 1) / 2], vb[(NG + 1) / 2], vc[(NG + 1) / 2], vd[(NG + 1) / 2];
             const uint8_t* vr = rec0 + h * R::bytes + R::v + piece;
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 const float db = e & 1 ? half_at<1>(v1[h][e / 2]) : half_at<0>(v1[h][e / 2]);
                 float la = e & 1 ? half_at<1>(u0[h][e / 2]) : half_at<0>(u0[h][e / 2]);
                 float lb = e & 1 ? half_at<1>(u1[h][e / 2]) : half_at<0>(u1[h][e / 2]);
-                if (W != W_HALF) {
+                if (W != W_CODE) {
                     // 8, or 8 2^(E - 7): the exponents of that and of 2^(7 - E) add up to 3
                     const float k = W == W_MID ? (e & 1 ? half_at<1>(0x84008400u - h2_bits(down_e[e / 2])) : half_at<0>(0x84008400u - h2_bits(down_e[e / 2]))) : 8.0f;
                     la = fmaf(k, da, la);
@@ -744,14 +745,7 @@ __global__ void __launch_bounds__(32 * kAtWarps, 2) k_kv4_attention(const __grid
                 }
                 codes8<SUB>(wa, ra);
                 codes8<SUB>(wc, rc);
-                __half2 hi0, hi1;
-                if (W == W_HALF) {
-                    hi0 = __hmul2(p0, e & 1 ? __high2half2(bits_h2(v0[h][e / 2])) : __low2half2(bits_h2(v0[h][e / 2])));
-                    hi1 = __hmul2(p1, e & 1 ? __high2half2(bits_h2(v1[h][e / 2])) : __low2half2(bits_h2(v1[h][e / 2])));
-                } else {
-                    hi0 = __floats2half2_rn(p[0] * da, p[1] * da);
-                    hi1 = __floats2half2_rn(p[2] * db, p[3] * db);
-                }
+                const __half2 hi0 = __floats2half2_rn(p[0] * da, p[1] * da), hi1 = __floats2half2_rn(p[2] * db, p[3] * db);
                 const uint32_t b0 = transpose8(h2_bits(hi0)), b1 = transpose8(h2_bits(hi1));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) mma16(o[e][u], ra[2 * u], ra[2 * u + 1], rc[2 * u], rc[2 * u + 1], b0, b1);

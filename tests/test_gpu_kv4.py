@@ -1348,3 +1348,25 @@ def test_packed_long_prompts_of_one_sign(env, t, D, n):
     out = packed(env, t, q, k, v, cu, 1, 1, D, D ** -0.5)
     rows = [0, 777, 16384, n // 3, n // 2, n - 100, n - 2, n - 1]
     check_packed(host(out[rows]), *rows64(torch, rows, q, k, v, 1, 1, D, D ** -0.5), 1, D, t, 0.0, len(rows))
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_attention_rounds_a_weight_once(env, t, D):
+    """Contexts of a few keys and many heads, whose outputs are often much smaller than the values: what is left there is the
+    rounding of a weight times its step, once."""
+    lib, torch, _ = env
+    H, HKV, lens = 160, 8, [2, 3, 2, 5, 1, 13, 2, 388] * 12
+    for seed in range(4):
+        c, k, v, d, at = filled(env, lens, HKV, D, seed=100 + seed, spread=20.0 + seed)
+        T = len(lens)
+        q = (torch.randn((T, H * D), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)) / 20).to(dtype(torch, t))
+        out = host(attention(env, c, t, q, H, list(range(T)), [n - 1 for n in lens], max(lens), D ** -0.5))
+        for s in range(T):
+            rows = slice(int(at[s]), int(at[s]) + lens[s])
+            x = q[s].view(HKV, H // HKV, D).double()
+            kk, vv, dd = (y[rows].transpose(0, 1) for y in (k, v, d))
+            w = torch.softmax(x @ kk.transpose(1, 2) * D ** -0.5, -1)
+            want, mean, coarse = (z.reshape(H, D).cpu().numpy() for z in (w @ vv, w @ vv.abs(), w @ dd))
+            ext = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1).reshape(H).cpu().numpy() * D ** -0.5
+            near(out[s].reshape(H, D), want, (mean, ext, coarse), t)
